@@ -168,6 +168,85 @@ int mk_gemm_ar_launch(const void* A, const void* B, const mk_symm_view* C,
                       const mk_symm_view* barrier, const mk_symm_view* C_final, int M, int N,
                       int K, uint32_t epoch, int b_layout, void* stream);
 
+/* ---- products with 4-bit weights: the single-token and small-batch forms of the products above.
+ * One GPU each; a tensor-parallel rank runs them on its own shard.  No counterpart in the
+ * reference.
+ *
+ * mk_w4 describes a matrix [N, K] of codes 0..15 with one scale (and, with zeros = 1, one whole
+ * zero point 0..15; else 8) per row and group of `group` columns:
+ *   w[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group].
+ * `data` is a device buffer of mk_w4_bytes() bytes, 16-byte aligned, in the library's own layout;
+ * mk_w4_pack or mk_w4_quantize fills it once.  dtype is the type of the scales and of the
+ * activations that the products take.  N and K may be any positive number; a group that reaches
+ * past K is short.  The struct itself is read during the call only. */
+#define MK_BF16 0
+#define MK_FP16 1
+#define MK_FP32 2
+
+#define MK_W4_PLAIN 0   /* outputs are the rows                                               */
+#define MK_W4_GATE_UP 1 /* rows [0, N/2) gate, [N/2, N) up: mk_w4_gemm_swiglu                   */
+#define MK_W4_ROTARY 2  /* rows are heads of head_dim features: mk_w4_gemm_rotary               */
+
+typedef struct mk_w4 {
+  void* data;
+  int N, K;
+  int group;  /* 32, 64 or 128 */
+  int dtype;  /* MK_BF16 or MK_FP16 */
+  int zeros;  /* 0: every zero point is 8; 1: zero points are stored */
+  int form;   /* MK_W4_* */
+  /* MK_W4_ROTARY only (0 otherwise): the first rotated_heads heads have their first rotary_dim
+   * features turned, in pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved = 1.
+   * head_dim and rotary_dim are even. */
+  int head_dim, rotary_dim, rotated_heads, interleaved;
+} mk_w4;
+
+/* Bytes of the packed buffer (data is not looked at), or a negative status. */
+long long mk_w4_bytes(const mk_w4* w);
+/* Lays out codes [N, (K + 1) / 2] (two per byte, the even column in the low half), scales
+ * [N, ceil(K / group)] of w's dtype and zero points (bytes, same shape; NULL when w->zeros = 0).
+ * Contiguous device buffers.  A zero point above 15 is taken modulo 16. */
+int mk_w4_pack(const mk_w4* w, const uint8_t* codes, const void* scales, const uint8_t* zero_points,
+               void* stream);
+/* Rounds a matrix [N, K] (row stride ld elements, dtype MK_*) to 4 bits.  Without zero points
+ * scale = T(max |w| / 7) and code = clamp(round(w / scale), -8, 7) + 8; with them
+ * scale = T((hi - lo) / 15), lo = min(w, 0), hi = max(w, 0), zero = clamp(round(-lo / scale), 0, 15),
+ * code = clamp(round(w / scale) + zero, 0, 15).  Divisions in fp32, ties to even, T = w's dtype.
+ * A group whose scale is 0 holds zeros; one with a value that is not finite, or whose scale
+ * exceeds T, gets a scale that is not finite, so that its products show it. */
+int mk_w4_quantize(const mk_w4* w, const void* src, long long ld, int src_dtype, void* stream);
+/* The matrix [N, K] that w stands for, in the order of rows given to pack or quantise, rounded
+ * once to out_dtype; row stride ld elements. */
+int mk_w4_dequantize(const mk_w4* w, void* out, long long ld, int out_dtype, void* stream);
+
+/* C[M, N] = A[M, K] * W^T.  A and C have w's dtype and row strides lda, ldc (elements); fp32 sums,
+ * rounded once.  M = 0 does nothing.  w->form = MK_W4_PLAIN. */
+int mk_w4_gemm(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
+               void* stream);
+/* H[M, N/2] = silu(A * G^T) * (A * U^T) with w->form = MK_W4_GATE_UP: the single-token form of
+ * mk_ag_gemm_swiglu_launch. */
+int mk_w4_gemm_swiglu(const void* A, long long lda, const mk_w4* w, void* H, long long ldh, int M,
+                      void* stream);
+/* C[M, N] = A * W^T with w->form = MK_W4_ROTARY, row m's rotated heads turned by positions[m]
+ * before the rounding (see mk_rotary).  positions: M values, 32-bit, or 64-bit with pos64 = 1. */
+int mk_w4_gemm_rotary(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
+                      const void* positions, int pos64, const float* inv_freq, float scale,
+                      void* stream);
+
+/* ---- rotary positions on rows of heads, the step after a query/key projection (for instance on
+ * the output of mk_ag_gemm_launch).  No counterpart in the reference.
+ * x, y: [rows, heads, head_dim], features contiguous, row and head strides in elements; y may be
+ * x.  Pair i < rotary_dim / 2 of every head of row m, features (i, i + rotary_dim / 2) or, with
+ * interleaved = 1, (2 i, 2 i + 1), becomes
+ *   scale * (a cos - b sin, b cos + a sin), angle = positions[m] * inv_freq[i];
+ * inverse = 1 turns the other way: times the same scale, the gradient of the forward call.  The other
+ * features are copied.  The angle is reduced in 64 bits, so positions need no table and lose nothing
+ * when they are far.  positions: rows values, 32-bit, or 64-bit with pos64 = 1, any sign.
+ * dtype MK_*; computed in fp32, rounded once. */
+int mk_rotary(const void* x, long long x_row, long long x_head, void* y, long long y_row,
+              long long y_head, long long rows, int heads, int head_dim, int rotary_dim, int dtype,
+              const void* positions, int pos64, const float* inv_freq, float scale, int interleaved,
+              int inverse, void* stream);
+
 /* Reads the 4 status words {code, where, detail0, detail1} of an operator's synchronisation
  * buffer (synchronous device-to-host copy).  Returns MK_ERR_DEVICE_WAIT when code != 0. */
 int mk_op_status(const mk_symm_view* sync, uint32_t out4[4]);

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_char_p, c_int, c_longlong, c_size_t, c_uint32,
+from ctypes import (POINTER, Structure, c_char_p, c_float, c_int, c_longlong, c_size_t, c_uint32,
                     c_void_p)
 from pathlib import Path
 
@@ -19,6 +19,9 @@ MK_B_KN = 1
 MK_AG_READY_WORDS = 65536
 MK_RS_SYNC_WORDS = 524288
 MK_AR_BARRIER_WORDS = 2 * 1024 * 1024
+
+MK_BF16, MK_FP16, MK_FP32 = 0, 1, 2
+MK_W4_PLAIN, MK_W4_GATE_UP, MK_W4_ROTARY = 0, 1, 2
 
 OP_GEMM, OP_AG, OP_RS, OP_AR = 0, 1, 2, 3
 
@@ -50,6 +53,13 @@ class SymmView(Structure):
         ("peer", c_void_p * MK_MAX_WORLD),
         ("mc", c_void_p),
     ]
+
+
+class W4View(Structure):
+    """mk_w4: a matrix of 4-bit weights in the library's layout."""
+    _fields_ = [("data", c_void_p)] + [(n, c_int) for n in (
+        "N", "K", "group", "dtype", "zeros", "form", "head_dim", "rotary_dim", "rotated_heads",
+        "interleaved")]
 
 
 class Plan(Structure):
@@ -98,6 +108,19 @@ _SIGNATURES = {
     "mk_gemm_ar_launch": (c_int, [c_void_p, c_void_p, POINTER(SymmView), POINTER(SymmView),
                                   POINTER(SymmView), c_int, c_int, c_int, c_uint32, c_int,
                                   c_void_p]),
+    "mk_w4_bytes": (c_longlong, [POINTER(W4View)]),
+    "mk_w4_pack": (c_int, [POINTER(W4View), c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mk_w4_quantize": (c_int, [POINTER(W4View), c_void_p, c_longlong, c_int, c_void_p]),
+    "mk_w4_dequantize": (c_int, [POINTER(W4View), c_void_p, c_longlong, c_int, c_void_p]),
+    "mk_w4_gemm": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong, c_int,
+                           c_void_p]),
+    "mk_w4_gemm_swiglu": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong,
+                                  c_int, c_void_p]),
+    "mk_w4_gemm_rotary": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong,
+                                  c_int, c_void_p, c_int, c_void_p, c_float, c_void_p]),
+    "mk_rotary": (c_int, [c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_longlong,
+                          c_longlong, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
+                          c_float, c_int, c_int, c_void_p]),
     "mk_op_status": (c_int, [POINTER(SymmView), POINTER(c_uint32)]),
     "mk_op_status_clear": (c_int, [POINTER(SymmView), c_void_p]),
     "mk_set_option": (c_int, [c_char_p, c_longlong]),

@@ -9,6 +9,12 @@ namespace mkb {
 // Records a printf-style message for mk_last_error() and returns `code`.
 int set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 
+// Number of SMs of the current device (cached); an error if it is not an sm_100 device.
+int device_sm_count(int* out);
+
+// The "pdl" option: launch with programmatic stream serialization.
+bool option_pdl();
+
 // Looks up a driver API symbol through the runtime.  Returns MK_OK or MK_ERR_CUDA.
 int driver_entry(const char* symbol, void** fn);
 

@@ -171,6 +171,11 @@ static Options options_snapshot() {
   return g_opt;
 }
 
+bool option_pdl() {
+  std::lock_guard<std::mutex> g(g_opt_mu);
+  return g_opt.pdl != 0;
+}
+
 static int make_plan(const Options& o, int op, int rank, int world, int M, int N, int K,
                      int b_layout, int num_sms, Plan* out, int epilogue = EPI_NONE) {
   if (op < OP_GEMM || op > OP_AR) return set_error(MK_ERR_INVALID, "unknown op %d", op);
@@ -336,7 +341,7 @@ static int encode_2d_bf16(CUtensorMap* map, const void* base, uint64_t inner, ui
 // ------------------------------------------------------------------------------------------
 // launch
 // ------------------------------------------------------------------------------------------
-static int device_sm_count(int* out) {
+int device_sm_count(int* out) {
   static int cached[64];
   int dev = 0;
   MKB_CUDA(cudaGetDevice(&dev));

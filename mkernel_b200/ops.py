@@ -141,6 +141,244 @@ def ag_gemm_swiglu_launch(A: DistBuffer, A_copy_ready: DistBuffer, B_gate_up: to
                                                        W * Ms, N2, K, _stream()))
 
 
+_W4_FORMS = {"plain": _lib.MK_W4_PLAIN, "gate_up": _lib.MK_W4_GATE_UP, "rotary": _lib.MK_W4_ROTARY}
+_DTYPES = {torch.bfloat16: _lib.MK_BF16, torch.float16: _lib.MK_FP16, torch.float32: _lib.MK_FP32}
+
+
+class W4Weight:
+    """A matrix [N, K] of 4-bit weights in the library's layout, made once by ``w4_quantize`` or
+    ``w4_pack`` and taken by ``w4_gemm``, ``w4_gemm_swiglu`` or ``w4_gemm_rotary`` (according to
+    ``form``).  ``data`` is the packed buffer, ``dtype`` the type of its scales and of the activations."""
+
+    def __init__(self, N: int, K: int, group: int, dtype: torch.dtype, zero_points: bool, device,
+                 form: str = "plain", head_dim: int = 0, rotary_dim: int = 0, rotated_heads: int = 0,
+                 interleaved: bool = False):
+        _require(form in _W4_FORMS, f"form must be one of {sorted(_W4_FORMS)}")
+        _require(dtype in (torch.bfloat16, torch.float16), "4-bit weights have bfloat16 or float16 scales")
+        _require(form == "rotary" or not (head_dim or rotary_dim or rotated_heads or interleaved),
+                 "head_dim, rotary_dim, rotated_heads and interleaved belong to form 'rotary'")
+        self.shape, self.group, self.dtype, self.form = (int(N), int(K)), int(group), dtype, form
+        self.zero_points = bool(zero_points)
+        self.rotary_dim = int(rotary_dim)
+        self.view = _lib.W4View(None, int(N), int(K), self.group, _DTYPES[dtype], int(self.zero_points),
+                                _W4_FORMS[form], int(head_dim), int(rotary_dim), int(rotated_heads),
+                                int(bool(interleaved)))
+        self.view_ref = ctypes.byref(self.view)
+        nbytes = _lib.check(_lib.lib().mk_w4_bytes(self.view_ref))
+        self.data = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self.device = self.data.device
+        self.view.data = self.data.data_ptr()
+
+    def dequantize(self, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The matrix these weights stand for, rows in the order given to ``w4_quantize`` or
+        ``w4_pack``, in ``out``'s type (by default a new tensor of this weight's type)."""
+        if out is None:
+            out = torch.empty(self.shape, dtype=self.dtype, device=self.device)
+        _require(out.device == self.device and out.dtype in _DTYPES and tuple(out.shape) == self.shape
+                 and out.stride(1) == 1 and out.stride(0) >= self.shape[1],
+                 f"out must be {self.shape} on {self.device}, bfloat16, float16 or float32, rows contiguous")
+        with _on_device(self.device):
+            _lib.check(_lib.lib().mk_w4_dequantize(self.view_ref, out.data_ptr(), out.stride(0),
+                                                   _DTYPES[out.dtype], _stream()))
+        return out
+
+
+def w4_quantize(weight: torch.Tensor, group: int = 128, zero_points: bool = False,
+                dtype: torch.dtype | None = None, **form) -> W4Weight:
+    """Round ``weight`` [N, K] (bfloat16, float16 or float32, rows contiguous) to 4 bits with one
+    scale, and with ``zero_points`` one whole zero point, per row and ``group`` (32, 64 or 128) columns.
+    ``dtype``: type of the scales and of the products' activations, by default the weight's.
+    ``form``: nothing for ``w4_gemm``; ``form="gate_up"`` for ``w4_gemm_swiglu`` (gate rows, then up
+    rows); ``form="rotary", head_dim=, rotary_dim=, rotated_heads=, interleaved=`` for
+    ``w4_gemm_rotary``."""
+    _require(isinstance(weight, torch.Tensor) and weight.is_cuda and weight.dim() == 2 and
+             weight.dtype in _DTYPES, "weight must be a CUDA matrix of bfloat16, float16 or float32")
+    _require(weight.stride(1) == 1 or weight.shape[1] == 1, "weight's rows must be contiguous")
+    dtype = dtype or (weight.dtype if weight.dtype != torch.float32 else torch.bfloat16)
+    N, K = weight.shape
+    W = W4Weight(N, K, group, dtype, zero_points, weight.device, **form)
+    with _on_device(weight.device):
+        _lib.check(_lib.lib().mk_w4_quantize(W.view_ref, weight.data_ptr(), max(weight.stride(0), K),
+                                             _DTYPES[weight.dtype], _stream()))
+    return W
+
+
+def w4_pack(codes: torch.Tensor, scales: torch.Tensor, zero_points: torch.Tensor | None = None, *,
+            K: int, **form) -> W4Weight:
+    """Lay out weights that are in 4 bits already: ``codes`` uint8 [N, (K + 1) // 2], two per byte, the even
+    column in the low half; ``scales`` [N, ceil(K / group)] bfloat16 or float16; ``zero_points`` uint8 of
+    the same shape (without: 8).  The group (32, 64 or 128) follows from the shapes.  ``form`` as in
+    ``w4_quantize``."""
+    for t, n in ((codes, "codes"), (scales, "scales")) + (((zero_points, "zero_points"),) if zero_points is not None else ()):
+        _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.is_contiguous()
+                 and t.device == codes.device, f"{n} must be a contiguous CUDA matrix on the codes' device")
+    _require(codes.dtype == torch.uint8, "codes must be uint8")
+    _require(zero_points is None or zero_points.dtype == torch.uint8, "zero_points must be uint8")
+    N, K = codes.shape[0], int(K)
+    _require(tuple(codes.shape) == (N, (K + 1) // 2), f"codes must be [N, {(K + 1) // 2}] for K={K}")
+    # where two groups give as many scales there is one scale a row, and it means the same
+    group = next((g for g in (128, 64, 32) if -(-K // g) == scales.shape[1]), 0)
+    _require(group > 0 and scales.shape[0] == N,
+             f"scales must be [N, ceil(K / group)] with a group of 32, 64 or 128 (K={K})")
+    _require(zero_points is None or zero_points.shape == scales.shape, "zero_points must have the scales' shape")
+    W = W4Weight(N, K, group, scales.dtype, zero_points is not None, codes.device, **form)
+    with _on_device(codes.device):
+        _lib.check(_lib.lib().mk_w4_pack(W.view_ref, codes.data_ptr(), scales.data_ptr(),
+                                         zero_points.data_ptr() if zero_points is not None else None,
+                                         _stream()))
+    return W
+
+
+def _w4_operands(A: torch.Tensor, W: W4Weight, C: torch.Tensor, n_out: int) -> None:
+    _require(isinstance(W, W4Weight), "W must be a W4Weight (w4_quantize, w4_pack)")
+    dev, dtype = W.device, W.dtype
+    _require(A.device == dev and C.device == dev, f"A and C must be on the weights' device {dev}")
+    _require(A.dtype == dtype and C.dtype == dtype, f"A and C must be {dtype} like the weights' scales")
+    _require(A.dim() == 2 and A.shape[1] == W.shape[1], f"A must be [M, {W.shape[1]}]")
+    _require(C.dim() == 2 and C.shape[0] == A.shape[0] and C.shape[1] == n_out,
+             f"C must be [{A.shape[0]}, {n_out}]")
+    _require((A.stride(1) == 1 or A.shape[1] == 1) and (C.stride(1) == 1 or n_out == 1),
+             "rows of A and C must be contiguous")
+
+
+def _rows(t: torch.Tensor) -> int:
+    """Row stride of a matrix; a single row may have any."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def w4_gemm(A: torch.Tensor, W: W4Weight, C: torch.Tensor) -> None:
+    """C[M, N] = A[M, K] @ W^T with 4-bit weights: the single-token and small-batch form of
+    ``gemm_bf16``.  A and C in the type of W's scales, any row strides; fp32 sums, rounded once."""
+    _w4_operands(A, W, C, W.shape[0])
+    with _on_device(W.device):
+        _lib.check(_lib.lib().mk_w4_gemm(A.data_ptr(), _rows(A), W.view_ref, C.data_ptr(), _rows(C),
+                                         A.shape[0], _stream()))
+
+
+def w4_gemm_swiglu(A: torch.Tensor, W: W4Weight, H: torch.Tensor) -> None:
+    """H[M, N/2] = silu(A @ G^T) * (A @ U^T), W of form "gate_up": the single-token form of
+    ``ag_gemm_swiglu_launch``."""
+    _w4_operands(A, W, H, W.shape[0] // 2)
+    with _on_device(W.device):
+        _lib.check(_lib.lib().mk_w4_gemm_swiglu(A.data_ptr(), _rows(A), W.view_ref, H.data_ptr(),
+                                                _rows(H), A.shape[0], _stream()))
+
+
+def _rotary_operands(positions: torch.Tensor, inv_freq: torch.Tensor, rows: int, pairs: int, dev) -> None:
+    _require(positions.device == dev and inv_freq.device == dev, f"positions and inv_freq must be on {dev}")
+    _require(positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous() and
+             tuple(positions.shape) == (rows,), f"positions must be contiguous int32 or int64 [{rows}]")
+    _require(inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and inv_freq.dim() == 1 and
+             (pairs < 0 or inv_freq.shape[0] == pairs),
+             "inv_freq must be contiguous float32 [rotary_dim / 2]")
+
+
+def w4_gemm_rotary(A: torch.Tensor, W: W4Weight, C: torch.Tensor, positions: torch.Tensor,
+                   inv_freq: torch.Tensor, scale: float = 1.0) -> None:
+    """C[M, N] = A @ W^T, W of form "rotary": the query/key/value projection of M tokens with the
+    rotated heads of row m turned by positions[m] before the rounding (see ``rotary``)."""
+    _w4_operands(A, W, C, W.shape[0])
+    _rotary_operands(positions, inv_freq, A.shape[0], W.rotary_dim // 2, W.device)
+    with _on_device(W.device):
+        _lib.check(_lib.lib().mk_w4_gemm_rotary(A.data_ptr(), _rows(A), W.view_ref, C.data_ptr(),
+                                                _rows(C), A.shape[0], positions.data_ptr(),
+                                                positions.dtype == torch.int64, inv_freq.data_ptr(),
+                                                scale, _stream()))
+
+
+def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+           Y: torch.Tensor | None = None, *, interleaved: bool = False, inverse: bool = False,
+           scale: float = 1.0) -> torch.Tensor:
+    """Turn the first 2 * len(inv_freq) features of every head of X [rows, heads, head_dim] by
+    positions[row] * inv_freq (radians) and multiply them by ``scale``; pairs are (i, i + rotary_dim / 2),
+    or neighbours with ``interleaved``.  Into Y, or in place without one; Y shares no memory with X unless
+    it is X.  ``inverse`` turns back, which is the gradient: dX = rotary(dY, ..., inverse=True).
+    Features contiguous, any row and head strides: the queries and keys of a projection
+    [rows, (heads + ...) * head_dim] are a view of its output."""
+    Y = X if Y is None else Y
+    _require(isinstance(X, torch.Tensor) and X.is_cuda and X.dtype in _DTYPES and X.dim() == 3,
+             "X must be a CUDA tensor [rows, heads, head_dim] of bfloat16, float16 or float32")
+    _require(Y.device == X.device and Y.dtype == X.dtype and Y.shape == X.shape,
+             "Y must have X's device, type and shape")
+    rows, heads, dim = X.shape
+    _require(dim == 1 or (X.stride(2) == 1 and Y.stride(2) == 1), "features of X and Y must be contiguous")
+    _rotary_operands(positions, inv_freq, rows, -1, X.device)
+    if Y is not X:
+        _require(not _overlap(X, Y), "Y must be X or share no memory with it")
+    _require(_distinct(Y), "two elements of Y share memory")
+    with _on_device(X.device):
+        _lib.check(_lib.lib().mk_rotary(X.data_ptr(), X.stride(0), X.stride(1), Y.data_ptr(),
+                                        Y.stride(0), Y.stride(1), rows, heads, dim,
+                                        2 * inv_freq.shape[0], _DTYPES[X.dtype], positions.data_ptr(),
+                                        positions.dtype == torch.int64, inv_freq.data_ptr(), scale,
+                                        interleaved, inverse, _stream()))
+    return Y
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    size = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+    return t.data_ptr(), t.data_ptr() + size * t.element_size()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    if a.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _distinct(t: torch.Tensor) -> bool:
+    """No two elements of [rows, heads, dim] (features contiguous) at one address: one of the two
+    outer dimensions steps over everything inside it."""
+    if t.is_contiguous():
+        return True
+    (rows, heads, dim), (sr, sh, _) = t.shape, t.stride()
+    by_row = (heads < 2 or sh >= dim) and (rows < 2 or sr >= (heads - 1) * sh + dim)
+    by_head = (rows < 2 or sr >= dim) and (heads < 2 or sh >= (rows - 1) * sr + dim)
+    return by_row or by_head
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | None = None,
+                       factor: float = 1.0, original_length: int = 0, low: float = 1.0,
+                       high: float = 32.0, device="cuda") -> tuple[torch.Tensor, float]:
+    """(inv_freq, scale) for ``rotary`` and ``w4_gemm_rotary``: base ** (-2 i / rotary_dim), changed for
+    contexts ``factor`` times longer than the ``original_length`` that a model was trained on:
+      None          as they are
+      "linear"      every frequency divided by factor
+      "base"        the base raised by factor ** (d / (d - 2)): the last pair is divided by factor, the
+                    first one kept
+      "parts"       by how many turns a pair makes over original_length: above ``high`` kept, below
+                    ``low`` divided by factor, linear in the pair's index between; scale is
+                    0.1 ln(factor) + 1
+      "wavelength"  the same ends, linear in the number of turns between them; scale 1
+    Computed in 64 bits, returned as float32."""
+    import math
+    d = int(rotary_dim)
+    _require(d >= 2 and d % 2 == 0, "rotary_dim must be even and positive")
+    _require(base > 1.0 and factor >= 1.0, "base must be above 1, factor at least 1")
+    _require(scaling in (None, "linear", "base", "parts", "wavelength"), f"unknown scaling {scaling!r}")
+    scale = 1.0
+    if scaling == "base":
+        _require(d > 2, "scaling 'base' needs more than one pair")
+        base = base * factor ** (d / (d - 2))
+    i = torch.arange(d // 2, dtype=torch.float64)
+    freq = float(base) ** (-2.0 * i / d)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling in ("parts", "wavelength"):
+        _require(original_length > 0 and high > low > 0, "needs original_length > 0 and high > low > 0")
+        if scaling == "parts":
+            def index(turns):     # of the pair that makes so many turns over the original length
+                return d * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+            first, last = max(math.floor(index(high)), 0), min(math.ceil(index(low)), d - 1)
+            keep = 1 - ((i - first) / max(last - first, 1e-3)).clamp(0, 1)
+            scale = 0.1 * math.log(factor) + 1.0
+        else:
+            keep = ((original_length * freq / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        freq = freq * keep + freq / factor * (1 - keep)
+    return freq.to(torch.float32).to(device), scale
+
+
 class TpMlp:
     """The tensor-parallel MLP as two fused launches on one stream:
     AllGather+GEMM(gate, up) with the SwiGLU epilogue -> H, then GEMM+ReduceScatter(down) on H.
@@ -148,7 +386,8 @@ class TpMlp:
     second one's set-up overlaps the first one's tail; captured in a CUDA graph they are two
     nodes.  All buffers are allocated once, collectively (same order on every rank):
       x:    DistBuffer [W, M/W, K]    rank r fills x.data_[r]
-      out:  rows [rank*M/W, (rank+1)*M/W) of y.data_ (the reduced slice)"""
+      out:  rows [rank*M/W, (rank+1)*M/W) of y.data_ (the reduced slice)
+    A decode step's few tokens take ``forward_tokens`` with weights in 4 bits."""
 
     def __init__(self, M: int, K: int, I_local: int, N_out: int, local_rank: int,
                  local_world_size: int):
@@ -165,6 +404,8 @@ class TpMlp:
         gemm_rs_blackwell_prepare(None, None, self.y, self.sync)
         self.w_gate_up = None
         self.w_down = None
+        self.w4_gate_up = None
+        self.w4_down = None
 
     def load_weights(self, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> None:
         """w_gate, w_up: [I_local, K]; w_down: [N_out, I_local] (this rank's shards)."""
@@ -181,6 +422,29 @@ class TpMlp:
         gemm_rs_blackwell_launch(self.h.view(self.M, self.I), self.w_down, self.y, self.sync)
         Ms = self.M // self.W
         return self.y.data_[self.rank * Ms:(self.rank + 1) * Ms]
+
+    def load_weights_w4(self, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+                        group: int = 128, zero_points: bool = False) -> None:
+        """Round this rank's shards (shapes as in ``load_weights``, any I_local) to 4 bits for
+        ``forward_tokens``; independent of the weights of ``forward``."""
+        _require(tuple(w_gate.shape) == tuple(w_up.shape) == (self.I, self.K),
+                 f"w_gate and w_up must be [{self.I},{self.K}]")
+        _require(tuple(w_down.shape) == (self.N, self.I), f"w_down must be [{self.N},{self.I}]")
+        self.w4_gate_up = w4_quantize(torch.cat((w_gate, w_up)), group, zero_points, form="gate_up")
+        self.w4_down = w4_quantize(w_down, group, zero_points)
+
+    def forward_tokens(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The MLP of a few tokens x [m, K] (any m; a decode step) with the 4-bit weights: two launches
+        on the current stream.  Returns out [m, N_out], this rank's part of the sum over ranks -- the
+        whole result when there is one rank; with more the caller sums it over them."""
+        _require(self.w4_gate_up is not None, "call load_weights_w4 first")
+        m = x.shape[0]
+        h = torch.empty((m, self.I), device=x.device, dtype=x.dtype)
+        if out is None:
+            out = torch.empty((m, self.N), device=x.device, dtype=x.dtype)
+        w4_gemm_swiglu(x, self.w4_gate_up, h)
+        w4_gemm(h, self.w4_down, out)
+        return out
 
     def free(self) -> None:
         for b in (self.x, self.ready, self.y, self.sync):
