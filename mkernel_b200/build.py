@@ -80,7 +80,7 @@ def build(force: bool = False, verbose: bool = False, diag: bool = False) -> Pat
         return lib
     tmp = lib.with_suffix(f".so.tmp.{os.getpid()}")
     flags = NVCC_FLAGS + (["-DMKB_DIAG"] if diag else [])
-    cmd = [_nvcc(), *flags, "-o", str(tmp), *map(str, sources())]
+    cmd = [_nvcc(), *flags, "--threads", "0", "-o", str(tmp), *map(str, sources())]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         tmp.unlink(missing_ok=True)

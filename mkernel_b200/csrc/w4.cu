@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/mkernel_b200.h"
 #include "host_util.h"
@@ -15,11 +16,12 @@ namespace mkb {
 // ------------------------------------------------------------------------------------------
 // laying the weights out
 // ------------------------------------------------------------------------------------------
-// One CTA of 256 threads per chunk.  Thread = (row of the strip, segment of 32 columns); the four
-// segments of a row are neighbouring lanes, so a group of 64 or 128 columns is reduced by shuffles.
-// Codes pass through shared memory once to change from row order to the layout's order.
+// The unit of all three kernels is what a lane of the product holds of one tile and quarter of a
+// block: 8 consecutive columns of a pair of rows, 8 bytes of codes.  Sixteen neighbouring threads
+// take a block's 128 columns, so rows are read and written in whole 256-byte pieces, a group
+// is reduced by shuffles, and nothing passes through shared memory.
 constexpr int kW4PackThreads = 256;
-constexpr int kW4CodePitch = kW4Block + 4;   // bytes; 33 words: rows start in different banks
+constexpr int kW4Units = kW4Strip / 2 * kW4Block / 8;   // of a chunk
 
 struct W4PackParams {
   W4Form form;
@@ -31,178 +33,233 @@ struct W4PackParams {
   // quantise
   const void* src;
   long long ld;
-  int vec;   // source rows are 16-byte aligned
+  int vec;   // 16-byte accesses to whole units are aligned
 };
 
-// Row (within a strip) of pair p, member j, in the order of the layout's tiles.
-__device__ __forceinline__ int w4_tile_row(int p, int j) { return (p / 8) * 16 + j * 8 + p % 8; }
-
-// Writes a chunk from codes [64 tile rows][128 columns] in shared memory.
-__device__ __forceinline__ void w4_store_codes(const uint8_t* sh, uint8_t* chunk) {
-  const int tid = threadIdx.x;
-  const int lane = tid & 31, ht = tid >> 5;          // ht: half (bit 2) and tile (bits 0, 1)
-  const int g = lane >> 2, t = lane & 3;
-  const uint8_t* base = sh + ((ht & 3) * 16 + g) * kW4CodePitch + (ht >> 2) * 64;
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int col = 32 * (j >> 1) + 8 * t + 4 * (j & 1);
-    uint32_t v = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        v |= (uint32_t)base[(i & 1) * 8 * kW4CodePitch + col + 2 * (i >> 1) + e] << (4 * i + 16 * e);
-    w[j] = v;
-  }
-  reinterpret_cast<uint4*>(chunk)[tid] = make_uint4(w[0], w[1], w[2], w[3]);
+// Unit u of a chunk: pair of rows, column of the block, and where its codes lie.
+struct W4Unit { int pair, col, offset; };
+__device__ __forceinline__ W4Unit w4_unit(int u) {
+  const int pair = u >> 4, hq = u >> 2 & 3, t = u & 3;
+  return {pair, hq * 32 + t * 8, (((hq >> 1) * 4 + (pair >> 3)) * 32 + (pair & 7) * 4 + t) * 16 + (hq & 1) * 8};
 }
 
-// Place of (tile row, group of the block) among a chunk's scales, in 16-bit units.
-__device__ __forceinline__ int w4_scale_slot(int row, int group) {
-  return group * kW4Strip + (row & 7) * 8 + (row >> 4) * 2 + ((row >> 3) & 1);
+// A unit's word of four codes each of the pair's rows, from bytes c (lowest: first column).
+__device__ __forceinline__ uint32_t w4_word(uint32_t first, uint32_t second) {
+  // columns 0, 1, 2, 3 go to bits 0, 16, 8, 24
+  return __byte_perm(first, 0, 0x3120) | __byte_perm(second, 0, 0x3120) << 4;
+}
+
+// Place of the scales of a pair (two 16-bit values) in a group of the block, in bytes.
+__device__ __forceinline__ int w4_scale_offset(int pair, int group) {
+  return kW4CodeBytes + group * 128 + (pair & 7) * 16 + (pair >> 3) * 4;
 }
 
 template <typename T>
-__device__ __forceinline__ void w4_store_scale(const W4Form& f, uint8_t* chunk, int row, int group,
-                                               uint16_t scale, int zero) {
-  uint16_t* s = reinterpret_cast<uint16_t*>(chunk + kW4CodeBytes);
-  const int slot = w4_scale_slot(row, group);
-  s[slot] = scale;
-  if (f.zeros)
-    s[(kW4Block / f.group) * kW4Strip + slot] = (uint16_t)((W4Traits<T>::kMagic & 0xffff) + zero);
+__device__ __forceinline__ uint16_t w4_offset_bits(int zero) {
+  const T v = W4Traits<T>::from_float(-zero * W4Traits<T>::kUnit);
+  return *reinterpret_cast<const uint16_t*>(&v);
 }
 
+template <typename T>
+__device__ __forceinline__ void w4_store_scales(const W4Form& f, uint8_t* chunk, const W4Unit& u, const uint16_t (&s)[2],
+                                                const int (&zero)[2]) {
+  uint8_t* p = chunk + w4_scale_offset(u.pair, u.col / f.group);
+  *reinterpret_cast<uint32_t*>(p) = s[0] | (uint32_t)s[1] << 16;
+  if (f.zeros)
+    *reinterpret_cast<uint32_t*>(p + kW4Block / f.group * 128) =
+        w4_offset_bits<T>(zero[0]) | (uint32_t)w4_offset_bits<T>(zero[1]) << 16;
+}
+
+// Codes behind the matrix are 8 and their scales 0, whoever lays them out.
 template <typename T>
 __global__ void __launch_bounds__(kW4PackThreads) w4_pack_kernel(W4PackParams p) {
-  __shared__ uint8_t sh[kW4Strip * kW4CodePitch];
   const W4Form& f = p.form;
   const int strip = blockIdx.x / f.blocks, block = blockIdx.x % f.blocks;
   uint8_t* chunk = p.data + (size_t)blockIdx.x * f.chunk_bytes;
-  const int row = threadIdx.x >> 2, seg = threadIdx.x & 3;
-  const int pair = (row >> 4) * 8 + (row & 7);
-  const int n = w4_row(f, strip, pair, (row >> 3) & 1);
-  const long long k0 = (long long)block * kW4Block + seg * 32;
-  const long long row_bytes = ((long long)f.K + 1) / 2;
-  for (int c = 0; c < 32; c += 2) {
-    const bool in = n >= 0 && k0 + c < f.K;
-    const uint8_t b = in ? __ldg(p.codes + n * row_bytes + (k0 + c) / 2) : 0x88;
-    sh[row * kW4CodePitch + seg * 32 + c] = b & 15;
-    sh[row * kW4CodePitch + seg * 32 + c + 1] = k0 + c + 1 < f.K ? b >> 4 : 8;
+  const long long row_bytes = ((long long)f.K + 1) / 2, groups = ((long long)f.K + f.group - 1) / f.group;
+  for (int i = threadIdx.x; i < kW4Units; i += kW4PackThreads) {
+    const W4Unit u = w4_unit(i);
+    const long long k = (long long)block * kW4Block + u.col;
+    uint32_t nibbles[2];   // of 8 columns
+    uint16_t scale[2];
+    int zero[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = w4_row(f, strip, u.pair, j);
+      nibbles[j] = 0x88888888u;
+      scale[j] = 0;
+      zero[j] = 8;
+      if (n >= 0 && k < f.K) {
+        const uint8_t* c = p.codes + n * row_bytes + k / 2;
+        uint32_t v = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v |= (k + 2 * e < f.K ? (uint32_t)__ldg(c + e) : 0x88u) << (8 * e);
+        if (k + 8 > f.K) {
+          const uint32_t mask = (1u << (4 * (int)(f.K - k))) - 1;
+          v = (v & mask) | (0x88888888u & ~mask);
+        }
+        nibbles[j] = v;
+        if (u.col % f.group == 0) {
+          scale[j] = __ldg(p.scales + n * groups + k / f.group);
+          if (f.zeros) zero[j] = __ldg(p.zero_points + n * groups + k / f.group) & 15;
+        }
+      }
+    }
+    // columns 0, 1, 2, 3 of each four from nibbles to bytes
+    uint32_t low[2], high[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      low[j] = __byte_perm(nibbles[j] & 0x0f0f, (nibbles[j] >> 4) & 0x0f0f, 0x5140);
+      high[j] = __byte_perm((nibbles[j] >> 16) & 0x0f0f, (nibbles[j] >> 20) & 0x0f0f, 0x5140);
+    }
+    *reinterpret_cast<uint2*>(chunk + u.offset) = make_uint2(w4_word(low[0], low[1]), w4_word(high[0], high[1]));
+    if (u.col % f.group == 0) w4_store_scales<T>(f, chunk, u, scale, zero);
   }
-  const int segs = f.group / 32;
-  if (seg % segs == 0) {
-    const long long groups = ((long long)f.K + f.group - 1) / f.group;
-    const long long gi = k0 / f.group;
-    const bool in = n >= 0 && k0 < f.K;
-    const uint16_t s = in ? __ldg(p.scales + n * groups + gi) : 0;
-    const int z = in && f.zeros ? __ldg(p.zero_points + n * groups + gi) & 15 : 8;
-    w4_store_scale<T>(f, chunk, row, seg / segs, s, z);
-  }
-  __syncthreads();
-  w4_store_codes(sh, chunk);
 }
 
-// Quantiser: reads the matrix once, writes the chunk.  Bound by memory: 2 (or 4) bytes in, 0.53
-// out per weight.
-template <typename S>
-__device__ __forceinline__ float w4_src(const S* p) { return (float)__ldg(p); }
+__device__ __forceinline__ float w4_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float w4_min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
-template <typename T, typename S>
+// w / s rounded to fp32, given r = 1 / s.  For w and s of 16 bits a quotient that is not half way between
+// two whole numbers is much further from there than fp32's last place, and one that is, is exact: one
+// correction of w r by its remainder (Markstein's last step) rounds the same way as the division.
+__device__ __forceinline__ float w4_quotient(float w, float s, float r) {
+  const float q = w * r;
+  return __fmaf_rn(__fmaf_rn(-q, s, w), r, q);
+}
+
+// Quantiser: reads the matrix once and writes the chunk.  Memory bounds it (2 or 4 bytes in, 0.53 out a
+// weight), arithmetic closely behind: hence the quotient above and the rounding by an addition.
+template <typename T, typename S, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParams p) {
-  __shared__ uint8_t sh[kW4Strip * kW4CodePitch];
   const W4Form& f = p.form;
   const int strip = blockIdx.x / f.blocks, block = blockIdx.x % f.blocks;
   uint8_t* chunk = p.data + (size_t)blockIdx.x * f.chunk_bytes;
-  const int row = threadIdx.x >> 2, seg = threadIdx.x & 3;
-  const int pair = (row >> 4) * 8 + (row & 7);
-  const int n = w4_row(f, strip, pair, (row >> 3) & 1);
-  const long long k0 = (long long)block * kW4Block + seg * 32;
-  const S* src = static_cast<const S*>(p.src) + (long long)(n < 0 ? 0 : n) * p.ld + k0;
-  float w[32];
-  if (n >= 0 && p.vec && k0 + 32 <= f.K) {
-    constexpr int kPer = 16 / sizeof(S);
+#pragma unroll 1
+  for (int c = threadIdx.x; c < kW4Units; c += kW4PackThreads) {
+    const W4Unit u = w4_unit(c);
+    const int k = block * kW4Block + u.col;
+    const bool whole = p.vec && k + 8 <= f.K;
+    float w[2][8];
+    bool row[2];
 #pragma unroll
-    for (int c = 0; c < 32; c += kPer) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + c));
-      const S* e = reinterpret_cast<const S*>(&v);
+    for (int j = 0; j < 2; ++j) {
+      const int n = w4_row(f, strip, u.pair, j);
+      row[j] = n >= 0;
+      const S* src = static_cast<const S*>(p.src) + (long long)(n < 0 ? 0 : n) * p.ld + k;
+      if (row[j] && whole) {
+        constexpr int kPer = 16 / sizeof(S);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) w[c + i] = (float)e[i];
+        for (int e = 0; e < 8; e += kPer) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + e));
+          const S* x = reinterpret_cast<const S*>(&v);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) w[j][e + i] = (float)x[i];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[j][e] = row[j] && k + e < f.K ? (float)__ldg(src + e) : 0.0f;
+      }
     }
-  } else {
+    uint16_t scale_bits[2];
+    int zeros[2];
+    uint32_t low[2], high[2];
 #pragma unroll
-    for (int c = 0; c < 32; ++c) w[c] = n >= 0 && k0 + c < f.K ? w4_src(src + c) : 0.0f;
-  }
-  float lo = 0.0f, hi = 0.0f;
-  bool finite = true;
-#pragma unroll
-  for (int c = 0; c < 32; ++c) {
-    lo = fminf(lo, w[c]);
-    hi = fmaxf(hi, w[c]);
-    finite = finite && isfinite(w[c]);
-  }
-  for (int d = 1; d < f.group / 32; d *= 2) {
-    lo = fminf(lo, __shfl_xor_sync(~0u, lo, d));
-    hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, d));
-    finite = __shfl_xor_sync(~0u, (int)finite, d) && finite;
-  }
-  const float range = f.zeros ? __fdiv_rn(hi - lo, 15.0f) : __fdiv_rn(fmaxf(fabsf(lo), hi), 7.0f);
-  T scale_t = W4Traits<T>::from_float(finite ? range : __int_as_float(0x7fc00000));
-  const uint16_t scale_bits = *reinterpret_cast<uint16_t*>(&scale_t);
-  const float scale = W4Traits<T>::to_float(scale_bits);
-  const float divisor = scale == 0.0f ? 1.0f : scale;
-  const float zero = f.zeros ? fminf(fmaxf(rintf(__fdiv_rn(-lo, divisor)), 0.0f), 15.0f) : 8.0f;
-#pragma unroll
-  for (int c = 0; c < 32; c += 4) {
-    uint32_t v = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float q = fminf(fmaxf(rintf(__fdiv_rn(w[c + i], divisor)) + zero, 0.0f), 15.0f);
-      if (n < 0 || k0 + c + i >= f.K) q = 8.0f;   // behind the matrix: as pack leaves it
-      v |= (uint32_t)(int)q << (8 * i);
-    }
-    *reinterpret_cast<uint32_t*>(sh + row * kW4CodePitch + seg * 32 + c) = v;
-  }
-  const int segs = f.group / 32;
-  if (seg % segs == 0)
-    w4_store_scale<T>(f, chunk, row, seg / segs, scale_bits, n >= 0 && k0 < f.K ? (int)zero : 8);
-  __syncthreads();
-  w4_store_codes(sh, chunk);
-}
-
-// The matrix back from its layout: one CTA per chunk, one 16-byte access of codes per thread, whose
-// 8 consecutive columns of a row leave as one 16-byte store (two for fp32 output).
-template <typename T, typename O>
-__global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Form f, const uint8_t* data, O* out,
-                                                            long long ld, int vec) {
-  const int strip = blockIdx.x / f.blocks, block = blockIdx.x % f.blocks;
-  const uint8_t* chunk = data + (size_t)blockIdx.x * f.chunk_bytes;
-  const int lane = threadIdx.x & 31, ht = threadIdx.x >> 5;
-  const int g = lane >> 2, t = lane & 3, tile = ht & 3;
-  const uint4 c = __ldg(reinterpret_cast<const uint4*>(chunk) + threadIdx.x);
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-  const uint16_t* s = reinterpret_cast<const uint16_t*>(chunk + kW4CodeBytes);
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int row = tile * 16 + j * 8 + g;
-    const int n = w4_row(f, strip, tile * 8 + g, j);
-    if (n < 0) continue;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int col = (ht >> 2) * 64 + q * 32 + 8 * t;
-      const long long k = (long long)block * kW4Block + col;
-      if (k >= f.K) continue;
-      const int slot = w4_scale_slot(row, col / f.group);
-      const float scale = W4Traits<T>::to_float(__ldg(s + slot));
-      const int zero = f.zeros ? (int)__ldg(s + (kW4Block / f.group) * kW4Strip + slot) -
-                                     (int)(W4Traits<T>::kMagic & 0xffff)
-                               : 8;
-      O v[8];
+    for (int j = 0; j < 2; ++j) {
+      float lo = 0.0f, hi = 0.0f;   // symmetric: hi is the largest magnitude
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int code = (w[2 * q + (e >> 2)] >> (4 * (j + 2 * ((e >> 1) & 1)) + 16 * (e & 1))) & 15;
-        const float x = (float)(code - zero) * scale;
-        v[e] = (O)x;   // to the nearest, ties to even
+        if (ZEROS) lo = w4_min_nan(lo, w[j][e]);
+        hi = w4_max_nan(hi, ZEROS ? w[j][e] : fabsf(w[j][e]));
+      }
+#pragma unroll
+      for (int d = 1; d < GROUP / 8; d *= 2) {
+        if (ZEROS) lo = w4_min_nan(lo, __shfl_xor_sync(~0u, lo, d));
+        hi = w4_max_nan(hi, __shfl_xor_sync(~0u, hi, d));
+      }
+      float range = ZEROS ? __fdiv_rn(hi - lo, 15.0f) : __fdiv_rn(hi, 7.0f);
+      if (!isfinite(hi) || !isfinite(lo)) range = __int_as_float(0x7fc00000);
+      const T scale_t = W4Traits<T>::from_float(range);
+      scale_bits[j] = *reinterpret_cast<const uint16_t*>(&scale_t);
+      const float scale = W4Traits<T>::to_float(scale_bits[j]);
+      const float divisor = scale == 0.0f ? 1.0f : scale;
+      zeros[j] = 8;
+      if (ZEROS && row[j] && k < f.K) zeros[j] = (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, divisor)), 0.0f), 15.0f);
+      // fp32 weights, and scales whose remainders could be lost among the subnormals, are divided
+      if (sizeof(S) == 2 && divisor >= 0x1p-90f && divisor <= 0x1p90f) {
+        const float inverse = __fdiv_rn(1.0f, divisor);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[j][e] = w4_quotient(w[j][e], divisor, inverse);
+      } else {
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          // one division at a time, in a loop that keeps w in registers
+          float q = __fdiv_rn(w[j][0], divisor);
+#pragma unroll
+          for (int i = 0; i < 7; ++i) w[j][i] = w[j][i + 1];
+          w[j][7] = q;
+        }
+      }
+      // quotient + 1.5 2^23 is the rounded quotient in the low bits (ties to even)
+      constexpr float kRound = 12582912.0f;
+      const float least = kRound - zeros[j], most = kRound + (15 - zeros[j]);
+      uint32_t b[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(fminf(fmaxf(w[j][e] + kRound, least), most));
+      // low bytes, each a two's complement number of -15..15: plus the zero point, none carries
+      const uint32_t add = zeros[j] * 0x01010101u;
+      low[j] = __vadd4(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410), add);
+      high[j] = __vadd4(__byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410), add);
+      if (!row[j] || k + 8 > f.K) {   // behind the matrix: as pack leaves it
+        const int n = row[j] ? max(0, f.K - k) : 0;
+        const uint32_t keep_low = n >= 4 ? ~0u : (1u << (8 * n)) - 1;
+        const uint32_t keep_high = n >= 8 ? ~0u : n <= 4 ? 0u : (1u << (8 * (n - 4))) - 1;
+        low[j] = (low[j] & keep_low) | (0x08080808u & ~keep_low);
+        high[j] = (high[j] & keep_high) | (0x08080808u & ~keep_high);
+      }
+    }
+    *reinterpret_cast<uint2*>(chunk + u.offset) = make_uint2(w4_word(low[0], low[1]), w4_word(high[0], high[1]));
+    if (u.col % GROUP == 0) w4_store_scales<T>(f, chunk, u, scale_bits, zeros);
+  }
+}
+
+// The matrix back from its layout, 8 consecutive columns of a row as one 16-byte store (two for fp32).
+template <typename T, typename O>
+__global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f, const uint8_t* data, O* out,
+                                                                       long long ld, int vec) {
+  const int strip = blockIdx.x / f.blocks, block = blockIdx.x % f.blocks;
+  const uint8_t* chunk = data + (size_t)blockIdx.x * f.chunk_bytes;
+#pragma unroll
+  for (int c = 0; c < kW4Units / kW4PackThreads; ++c) {
+    const W4Unit u = w4_unit(c * kW4PackThreads + threadIdx.x);
+    const long long k = (long long)block * kW4Block + u.col;
+    if (k >= f.K) continue;
+    const uint2 code = __ldg(reinterpret_cast<const uint2*>(chunk + u.offset));
+    const uint8_t* sp = chunk + w4_scale_offset(u.pair, u.col / f.group);
+    const float2 scale = W4Traits<T>::to_float2(__ldg(reinterpret_cast<const uint32_t*>(sp)));
+    float2 off = make_float2(-8.0f, -8.0f);
+    if (f.zeros) {
+      off = W4Traits<T>::to_float2(__ldg(reinterpret_cast<const uint32_t*>(sp + kW4Block / f.group * 128)));
+      off = make_float2(off.x / W4Traits<T>::kUnit, off.y / W4Traits<T>::kUnit);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = w4_row(f, strip, u.pair, j);
+      if (n < 0) continue;
+      alignas(16) O v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // columns 0, 1, 2, 3 are bits 0, 16, 8, 24
+        const uint32_t q = ((e & 4 ? code.y : code.x) >> (4 * j + 16 * (e & 1) + 4 * (e & 2))) & 15;
+        v[e] = (O)(((float)q + (j ? off.y : off.x)) * (j ? scale.y : scale.x));   // to the nearest, ties to even
       }
       O* dst = out + (long long)n * ld + k;
       if (vec && k + 8 <= f.K) {
@@ -232,6 +289,7 @@ struct W4Params {
   long long ldc;
   int M;
   int vec;        // rows of A are 16-byte aligned and K is a multiple of 8
+  int stage_bytes;
   int split;      // CTAs of a cluster, which share a strip along K
   int epilogue;
   RotaryArgs rotary;
@@ -261,169 +319,281 @@ __device__ __forceinline__ void w4_epilogue(const W4Params& p, int strip, int pa
   if (n1 >= 0) row[n1] = W4Traits<T>::from_float(v.y);
 }
 
-__device__ __forceinline__ uint4 w4_ld_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
+// d = a b (fresh) or d += a b.
 template <typename T>
-__device__ __forceinline__ void w4_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (sizeof(T) == 2 && W4Traits<T>::kMagic == 0x43004300u) {
+__device__ __forceinline__ void w4_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool fresh) {
+  const float c0 = fresh ? 0.0f : d[0], c1 = fresh ? 0.0f : d[1], c2 = fresh ? 0.0f : d[2], c3 = fresh ? 0.0f : d[3];
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "{%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   } else {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "{%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   }
 }
 
-// Eight consecutive activations of a token, zeros outside of [M, K].
-template <typename T>
-__device__ __forceinline__ uint4 w4_ld_x(const W4Params& p, int token, long long k) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (token < p.M && k < p.form.K) {
-    const uint16_t* x = static_cast<const uint16_t*>(p.A) + (long long)token * p.lda + k;
-    if (p.vec) {
-      v = __ldg(reinterpret_cast<const uint4*>(x));
-    } else {
-      uint16_t e[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = k + i < p.form.K ? __ldg(x + i) : (uint16_t)0;
-      v.x = e[0] | (uint32_t)e[1] << 16;
-      v.y = e[2] | (uint32_t)e[3] << 16;
-      v.z = e[4] | (uint32_t)e[5] << 16;
-      v.w = e[6] | (uint32_t)e[7] << 16;
-    }
-  }
-  return v;
-}
-
-// C^T = W A^T with the weights as the 16-row operand and up to 8 NT tokens as columns.  A warp walks
-// the chunks of one strip, its share of K; codes go from memory straight into the registers that
-// the matrix instruction takes them from, as whole numbers (code - zero), which the 16-bit types
-// hold exactly.  The sums of a group are exact products added in fp32, then times the group's
-// scale in fp32: no weight is rounded on the way.  The warps of a CTA and the CTAs of a cluster share a strip
-// along K and add up in a fixed order through (distributed) shared memory.
-constexpr int kW4Warps = 4;
+// C^T = W A^T with the weights as the 16-row operand and up to 8 NT tokens as columns.  A warp takes
+// every so many-th chunk of one strip; codes go to the matrix instruction as whole numbers
+// (code - zero, times a power of two), which the 16-bit types hold exactly.  The sums of a group are exact products
+// added in fp32, then times the group's scale in fp32: no weight is rounded on the way.  The warps
+// of a CTA and the CTAs of a cluster share a strip along K and add up in a fixed order through
+// (distributed) shared memory.
+//
+// What bounds it is bytes in flight, so a warp keeps kW4Stages chunks, each with the activations that
+// meet it, in a shared-memory ring of its own that asynchronous 16-byte copies fill.  A lane copies
+// just the pieces that it will itself use, so the ring needs no barrier between warps and no
+// registers while the copies fly; lanes meet only over the scales, which four of them share.
+constexpr int kW4Stages = 2;      // the kernel switches between two offsets
+constexpr int kW4SmemMax = 227 * 1024;
 constexpr int kW4Pitch = 34;   // float2 per token: the four tokens a warp writes at once hit different banks
 
-template <typename T, int NT, int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(kW4Warps * 32) w4_stream_kernel(const __grid_constant__ W4Params p) {
-  __shared__ float2 red[kW4Warps][NT * 8][kW4Pitch];
+// Bytes of a stage: codes of `tiles` of a chunk's four tiles, all its scales, then 256 bytes of
+// activations for each of `tokens`.
+__host__ __device__ constexpr int w4_stage_bytes(int chunk, int tiles, int tokens) {
+  return chunk - (4 - tiles) * 1024 + tokens * 256;
+}
+
+// Place of 8 activations (quarter hq of the block, lane t) of a token behind the chunk.  Odd tokens swap
+// quarters, so that the two tokens that eight lanes read at once lie in different banks.
+__device__ __forceinline__ int w4_x_slot(int token, int hq, int t) {
+  return token * 256 + ((hq ^ (token & 1)) * 64) + t * 16;
+}
+
+// Starts the copies of TILES tiles of a chunk (`chunk`: the address of the first, plus this lane's
+// 16 bytes; `tail`: that of the chunk's scales) and of the activations of block `block` into a stage.
+// x: column 8 t of this lane's token (g of each eight).
+template <int NT, int TILES, int TAIL>
+__device__ __forceinline__ void w4_fill(const W4Params& p, const uint8_t* chunk, const uint8_t* tail,
+                                        int block, int token0, const uint16_t* const (&x)[NT], const bool (&have)[NT], int x_even,
+                                        int x_odd, uint32_t stage, uint8_t* stage_ptr, int lane) {
+  const uint32_t dst = stage + lane * 16;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int r = 0; r < TILES; ++r) ptx::cp_async_16(dst + (h * TILES + r) * 512, chunk + (h * 4 + r) * 512);
+#pragma unroll
+  for (int i = 0; i < TAIL; i += 512)
+    if (i + 512 <= TAIL || lane * 16 < TAIL - i) ptx::cp_async_16(dst + TILES * 1024 + i, tail + i);
+  const int k0 = block * kW4Block;
+  if (p.vec && k0 + kW4Block <= p.form.K) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      if (have[n]) {
+        const uint16_t* from = x[n] + k0;
+#pragma unroll
+        for (int hq = 0; hq < 4; ++hq)
+          ptx::cp_async_16(stage + ((hq & 1) ? x_odd : x_even) + n * 2048 + hq * 64, from + hq * 32);
+      }
+  } else {
+    // The last block of K, and rows that no 16-byte access can start on: lanes take consecutive
+    // elements.  Columns behind K are zeroed, so that no product there is a NaN.
+    const uint16_t* A = static_cast<const uint16_t*>(p.A) + k0 + lane;
+    const int tokens = min(NT * 8, p.M - token0);
+    for (int m0 = 0; m0 < tokens; m0 += 8) {
+      uint16_t v[8][4];
+#pragma unroll
+      for (int m = 0; m < 8; ++m) {
+        const uint16_t* row = A + (long long)(token0 + m0 + m) * p.lda;
+#pragma unroll
+        for (int hq = 0; hq < 4; ++hq)
+          v[m][hq] = m0 + m < tokens && k0 + hq * 32 + lane < p.form.K ? __ldg(row + hq * 32) : (uint16_t)0;
+      }
+#pragma unroll
+      for (int m = 0; m < 8; ++m)
+        if (m0 + m < tokens)
+#pragma unroll
+          for (int hq = 0; hq < 4; ++hq)
+            *reinterpret_cast<uint16_t*>(stage_ptr + TILES * 1024 + TAIL + w4_x_slot(m0 + m, hq, 0) + lane * 2) = v[m][hq];
+    }
+  }
+}
+
+// The scales (or offsets) of a lane's rows in TILES tiles.
+__device__ __forceinline__ void w4_ld_tiles(const uint8_t* p, uint32_t (&v)[4]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+__device__ __forceinline__ void w4_ld_tiles(const uint8_t* p, uint32_t (&v)[2]) {
+  const uint2 a = *reinterpret_cast<const uint2*>(p);
+  v[0] = a.x; v[1] = a.y;
+}
+__device__ __forceinline__ void w4_ld_tiles(const uint8_t* p, uint32_t (&v)[1]) {
+  v[0] = *reinterpret_cast<const uint32_t*>(p);
+}
+
+template <typename T, int NT, int TILES, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __grid_constant__ W4Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kGroups = kW4Block / GROUP;
+  constexpr int kTail = kGroups * 128 * (ZEROS ? 2 : 1);
+  constexpr int kChunk = kW4CodeBytes + kTail;
+  constexpr int kCodes = TILES * 1024;   // of a stage
   const W4Form& f = p.form;
-  const int strip = blockIdx.x / p.split;
+  const int warps = blockDim.x >> 5;
+  const int strip = blockIdx.x / p.split / (4 / TILES);
+  const int tile0 = blockIdx.x / p.split % (4 / TILES) * TILES;
   const int rank = blockIdx.x % p.split;
   const int token0 = blockIdx.y * 8 * NT;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* const ring_ptr = smem + warp * p.stage_bytes * kW4Stages;
+  const uint32_t ring = ptx::smem_u32(ring_ptr);
 
+  const int step = p.split * warps;
+  const int first = rank * warps + warp;
+  const size_t chunk_step = (size_t)step * kChunk;
+  const uint8_t* tail = p.data + ((size_t)strip * f.blocks + first) * kChunk + kW4CodeBytes + lane * 16;
+  const uint8_t* chunk = tail - kW4CodeBytes + tile0 * 512;
+  // Before the kernel ahead in the stream has finished nothing is read, but what will be may
+  // already be asked into L2.
+#pragma unroll
+  for (int i = 0; i < kW4Stages; ++i)
+    if (first + i * step < f.blocks)
+      for (int o = lane * 128; o < kChunk; o += 32 * 128)
+        if (TILES == 4 || o >= kW4CodeBytes || (o / 512 % 4 >= tile0 && o / 512 % 4 < tile0 + TILES))
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(tail - kW4CodeBytes - lane * 16 + i * chunk_step + o));
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
-  float acc[4][NT][4];
+  // Columns of the matrix instruction behind the last token compute something that is never stored;
+  // their lanes read another token's activations.
+  const uint16_t* x[NT];
+  bool have[NT];
+  const int last = min(NT * 8, p.M - token0) - 1;
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int n = 0; n < NT; ++n) {
+    have[n] = n * 8 + g <= last;
+    x[n] = static_cast<const uint16_t*>(p.A) + (long long)(token0 + (have[n] ? n * 8 + g : 0)) * p.lda + 8 * t;
+  }
+  const int gx = min(g, last);
+  const int x_even = kCodes + kTail + w4_x_slot(gx, 0, t), x_odd = kCodes + kTail + w4_x_slot(gx, 1, t) - 64;
+#pragma unroll
+  for (int i = 0; i < kW4Stages; ++i) {
+    if (first + i * step < f.blocks)
+      w4_fill<NT, TILES, kTail>(p, chunk, tail, first + i * step, token0, x, have, x_even, x_odd,
+                                ring + i * p.stage_bytes, ring_ptr + i * p.stage_bytes, lane);
+    chunk += chunk_step;
+    tail += chunk_step;
+    ptx::cp_async_commit();
+  }
+
+  float acc[TILES][NT][4];
+#pragma unroll
+  for (int r = 0; r < TILES; ++r)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.0f;
 
-  const uint8_t* data = p.data + (size_t)strip * f.blocks * f.chunk_bytes;
-  for (int block = rank * kW4Warps + warp; block < f.blocks; block += p.split * kW4Warps) {
-    const uint8_t* chunk = data + (size_t)block * f.chunk_bytes;
-    uint4 codes[8], scales[kGroups], offsets[kGroups];
+  int at = 0;   // byte offset of the stage
+  for (int block = first; block < f.blocks; block += step) {
+    ptx::cp_async_wait<kW4Stages - 1>();
+    __syncwarp();
+    const uint8_t* base = ring_ptr + at;
+    const uint8_t* base_codes = base + lane * 16;
+    const uint8_t* base_scales = base + kCodes + g * 16 + tile0 * 4;
+    const uint8_t* base_x[2] = {base + x_even, base + x_odd};
+    float part[TILES][NT][4];
+    uint32_t off[TILES][2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) codes[i] = w4_ld_stream(chunk + (i * 32 + lane) * 16);
+    for (int h = 0; h < 2; ++h) {
+      uint4 codes[TILES];
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-      scales[i] = w4_ld_stream(chunk + kW4CodeBytes + i * 128 + g * 16);
-      if (ZEROS) offsets[i] = w4_ld_stream(chunk + kW4CodeBytes + (kGroups + i) * 128 + g * 16);
-    }
-    float part[4][NT][4];
+      for (int r = 0; r < TILES; ++r) codes[r] = *reinterpret_cast<const uint4*>(base_codes + (h * TILES + r) * 512);
 #pragma unroll
-    for (int hq = 0; hq < 4; ++hq) {          // 32 columns at a time
-      const int gi = hq * 32 / GROUP;
-      uint4 x[NT];
+      for (int q = 0; q < 2; ++q) {          // 32 columns at a time
+        const int hq = h * 2 + q, gi = hq * 32 / GROUP;
+        uint4 xv[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-        x[n] = w4_ld_x<T>(p, token0 + n * 8 + g, (long long)block * kW4Block + hq * 32 + 8 * t);
-      if (hq * 32 % GROUP == 0) {
+        for (int n = 0; n < NT; ++n)
+          // past the last token of a second eight: any finite address of the stage (see above)
+          xv[n] = *reinterpret_cast<const uint4*>(base_x[q] + (n * 8 + g <= last ? n * 2048 : 0) + hq * 64);
+        const bool fresh = hq * 32 % GROUP == 0;
+        if (ZEROS && fresh) {
+          uint32_t both[TILES];
+          w4_ld_tiles(base_scales + (kGroups + gi) * 128, both);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part[r][n][i] = 0.0f;
-      }
-      const uint32_t off[4] = {offsets[gi].x, offsets[gi].y, offsets[gi].z, offsets[gi].w};
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint4 c = codes[(hq >> 1) * 4 + r];
-          const uint32_t word = (hq & 1) ? (s ? c.w : c.z) : (s ? c.y : c.x);
-          uint32_t off0 = W4Traits<T>::kEight, off1 = W4Traits<T>::kEight;
-          if (ZEROS) {
-            off0 = __byte_perm(off[r], 0, 0x1010);
-            off1 = __byte_perm(off[r], 0, 0x3232);
-          }
-          const uint32_t a[4] = {w4_decode<T>(word, 0, off0), w4_decode<T>(word, 1, off1),
-                                 w4_decode<T>(word, 2, off0), w4_decode<T>(word, 3, off1)};
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            w4_mma<T>(part[r][n], a, s ? x[n].z : x[n].x, s ? x[n].w : x[n].y);
-        }
-      }
-      if ((hq + 1) * 32 % GROUP == 0) {
-        const uint32_t sc[4] = {scales[gi].x, scales[gi].y, scales[gi].z, scales[gi].w};
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float s0 = W4Traits<T>::to_float(sc[r] & 0xffff), s1 = W4Traits<T>::to_float(sc[r] >> 16);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            acc[r][n][0] += s0 * part[r][n][0];
-            acc[r][n][1] += s0 * part[r][n][1];
-            acc[r][n][2] += s1 * part[r][n][2];
-            acc[r][n][3] += s1 * part[r][n][3];
+          for (int r = 0; r < TILES; ++r) {
+            off[r][0] = __byte_perm(both[r], 0, 0x1010);
+            off[r][1] = __byte_perm(both[r], 0, 0x3232);
           }
         }
+        // the two instructions of a tile add to one accumulator: other tiles go between them
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int r = 0; r < TILES; ++r) {
+            const uint32_t word = q ? (s ? codes[r].w : codes[r].z) : (s ? codes[r].y : codes[r].x);
+            uint32_t a[4];
+            w4_decode<T>(word, ZEROS ? off[r][0] : W4Traits<T>::kMinusEight,
+                         ZEROS ? off[r][1] : W4Traits<T>::kMinusEight, a);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              w4_mma<T>(part[r][n], a, s ? xv[n].z : xv[n].x, s ? xv[n].w : xv[n].y, fresh && s == 0);
+          }
+        }
+        if ((hq + 1) * 32 % GROUP == 0) {
+          uint32_t sc[TILES];
+          w4_ld_tiles(base_scales + gi * 128, sc);
+#pragma unroll
+          for (int r = 0; r < TILES; ++r) {
+            const float2 sv = W4Traits<T>::to_float2(sc[r]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              acc[r][n][0] += sv.x * part[r][n][0];
+              acc[r][n][1] += sv.x * part[r][n][1];
+              acc[r][n][2] += sv.y * part[r][n][2];
+              acc[r][n][3] += sv.y * part[r][n][3];
+            }
+          }
+        }
       }
     }
+    __syncwarp();
+    const int ahead = block + kW4Stages * step;
+    if (ahead < f.blocks)
+      w4_fill<NT, TILES, kTail>(p, chunk, tail, ahead, token0, x, have, x_even, x_odd, ring + at, ring_ptr + at,
+                                lane);
+    chunk += chunk_step;
+    tail += chunk_step;
+    ptx::cp_async_commit();
+    at = at == 0 ? p.stage_bytes : 0;
   }
 
+  // the warp's sums over its own ring, which nothing is copied into any more
+  float2* red = reinterpret_cast<float2*>(ring_ptr);
+  __syncwarp();
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int r = 0; r < TILES; ++r)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      red[warp][n * 8 + 2 * t][r * 8 + g] = make_float2(acc[r][n][0], acc[r][n][2]);
-      red[warp][n * 8 + 2 * t + 1][r * 8 + g] = make_float2(acc[r][n][1], acc[r][n][3]);
+      constexpr float kBack = 1.0f / W4Traits<T>::kUnit;
+      red[(n * 8 + 2 * t) * kW4Pitch + r * 8 + g] = make_float2(acc[r][n][0] * kBack, acc[r][n][2] * kBack);
+      red[(n * 8 + 2 * t + 1) * kW4Pitch + r * 8 + g] = make_float2(acc[r][n][1] * kBack, acc[r][n][3] * kBack);
     }
   if (p.split > 1) ptx::cluster_sync_all();
   else __syncthreads();
   // the CTAs of a cluster share the entries of the result among themselves
-  const uint32_t red0 = ptx::smem_u32(&red[0][0][0]);
-  for (int e = rank * (kW4Warps * 32) + threadIdx.x; e < NT * 8 * 32; e += p.split * kW4Warps * 32) {
-    const int token = e >> 5, pair = e & 31;
+  const uint32_t red0 = ptx::smem_u32(smem);
+  for (int e = rank * (warps * 32) + threadIdx.x; e < NT * 8 * 8 * TILES; e += step * 32) {
+    const int token = e / (8 * TILES), pair = e % (8 * TILES);
     if (token0 + token >= p.M) break;
     float2 v = make_float2(0.0f, 0.0f);
     for (int c = 0; c < p.split; ++c) {
       const uint32_t base = p.split > 1 ? ptx::map_to_cta(red0, c) : red0;
-#pragma unroll
-      for (int w = 0; w < kW4Warps; ++w) {
-        const float2 a = ptx::ld_cluster_f2(base + ((w * NT * 8 + token) * kW4Pitch + pair) * 8);
+#pragma unroll 4
+      for (int w = 0; w < warps; ++w) {
+        const float2 a = ptx::ld_cluster_f2(base + w * p.stage_bytes * kW4Stages + (token * kW4Pitch + pair) * 8);
         v.x += a.x;
         v.y += a.y;
       }
     }
-    w4_epilogue<T>(p, strip, pair, token0 + token, v);
+    w4_epilogue<T>(p, strip, tile0 * 8 + pair, token0 + token, v);
   }
   if (p.split > 1) ptx::cluster_sync_all();   // nobody leaves while its shared memory is read
 }
@@ -488,17 +658,69 @@ static int w4_launch(K kern, dim3 grid, int threads, int smem, int cluster, cuda
   return MK_OK;
 }
 
-template <typename T, int NT, int GROUP>
-static int w4_stream_launch(const W4Params& p, dim3 grid, cudaStream_t stream) {
-  return p.form.zeros
-             ? w4_launch(w4_stream_kernel<T, NT, GROUP, true>, grid, kW4Warps * 32, 0, p.split, stream, p)
-             : w4_launch(w4_stream_kernel<T, NT, GROUP, false>, grid, kW4Warps * 32, 0, p.split, stream, p);
+// How the few-token product is cut.  All choices follow from how many CTAs there are to fill the SMs;
+// figures are microseconds, 1 token, bf16, group 128, medians of graph replays.
+struct W4StreamPlan { int nt, tiles, warps, split, stage_bytes; long long token_tiles, ctas; };
+
+static W4StreamPlan w4_stream_plan(const W4Form& f, int M, int sms) {
+  W4StreamPlan pl;
+  pl.nt = M <= 8 ? 1 : 2;
+  pl.token_tiles = ((long long)M + 8 * pl.nt - 1) / (8 * pl.nt);
+  const long long units = f.strips * pl.token_tiles;
+  // Four tiles of rows to a warp share each load of activations, but a narrow matrix gives too few
+  // CTAs then: 1280 x 8192 takes 5.6 with 4 tiles (cut along K into clusters), 5.1 with 2, 4.5 with 1;
+  // 3584 x 8192: 6.9, 6.1, 7.0; 8192 x 8192: 9.1, 10.0, 12.3.
+  pl.tiles = units * 2 > sms ? 4 : units * 4 > sms ? 2 : 1;
+  pl.ctas = (long long)f.strips * (4 / pl.tiles);
+  // One CTA to an SM brings as many warps as fit; more CTAs than SMs share them with fewer (28672 x
+  // 8192: 28 with 8 warps, 36 with 16).  A warp without a chunk is of no use.
+  pl.warps = pl.ctas * pl.token_tiles > sms ? 8 : pl.nt == 1 ? 16 : 12;
+  if (pl.warps > f.blocks) pl.warps = f.blocks < 4 ? 4 : f.blocks;
+  // Clusters along K only where most SMs would be idle: one costs 0.7 (1024 x 1024: 2.1 and 2.9).
+  pl.split = 1;
+  while (pl.split < 8 && pl.ctas * pl.token_tiles * pl.split * 4 <= sms && pl.split * 16 <= f.blocks) pl.split *= 2;
+  if (pl.split > 1) pl.warps = 8;
+  pl.ctas *= pl.split;
+  pl.stage_bytes = w4_stage_bytes(f.chunk_bytes, pl.tiles, M < 8 * pl.nt ? M : 8 * pl.nt);
+  // a warp leaves its sums in its ring
+  const int sums = 8 * pl.nt * kW4Pitch * 8;
+  if (pl.stage_bytes * kW4Stages < sums) pl.stage_bytes = sums / kW4Stages;
+  return pl;
 }
-template <typename T, int NT>
-static int w4_stream_group(const W4Params& p, dim3 grid, cudaStream_t stream) {
-  if (p.form.group == 32) return w4_stream_launch<T, NT, 32>(p, grid, stream);
-  if (p.form.group == 64) return w4_stream_launch<T, NT, 64>(p, grid, stream);
-  return w4_stream_launch<T, NT, 128>(p, grid, stream);
+
+template <typename T, int NT, int TILES, int GROUP, bool ZEROS>
+static int w4_stream_launch(const W4Params& p, dim3 grid, int warps, cudaStream_t stream) {
+  auto kern = w4_stream_kernel<T, NT, TILES, GROUP, ZEROS>;
+  static bool attr_set[64];
+  int dev = 0;
+  MKB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    MKB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4SmemMax));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  return w4_launch(kern, grid, warps * 32, warps * kW4Stages * p.stage_bytes, p.split, stream, p);
+}
+template <typename T, int NT, int TILES>
+static int w4_stream_group(const W4Params& p, dim3 grid, int warps, cudaStream_t stream) {
+  const bool z = p.form.zeros;
+  switch (p.form.group) {
+    case 32: return z ? w4_stream_launch<T, NT, TILES, 32, true>(p, grid, warps, stream)
+                      : w4_stream_launch<T, NT, TILES, 32, false>(p, grid, warps, stream);
+    case 64: return z ? w4_stream_launch<T, NT, TILES, 64, true>(p, grid, warps, stream)
+                      : w4_stream_launch<T, NT, TILES, 64, false>(p, grid, warps, stream);
+    default: return z ? w4_stream_launch<T, NT, TILES, 128, true>(p, grid, warps, stream)
+                      : w4_stream_launch<T, NT, TILES, 128, false>(p, grid, warps, stream);
+  }
+}
+template <typename T>
+static int w4_stream_type(const W4Params& p, const W4StreamPlan& pl, dim3 grid, cudaStream_t s) {
+  if (pl.nt == 1)
+    return pl.tiles == 4   ? w4_stream_group<T, 1, 4>(p, grid, pl.warps, s)
+           : pl.tiles == 2 ? w4_stream_group<T, 1, 2>(p, grid, pl.warps, s)
+                           : w4_stream_group<T, 1, 1>(p, grid, pl.warps, s);
+  return pl.tiles == 4   ? w4_stream_group<T, 2, 4>(p, grid, pl.warps, s)
+         : pl.tiles == 2 ? w4_stream_group<T, 2, 2>(p, grid, pl.warps, s)
+                         : w4_stream_group<T, 2, 1>(p, grid, pl.warps, s);
 }
 
 static int w4_product(const char* what, const void* A, long long lda, const mk_w4* w, void* C, long long ldc,
@@ -528,37 +750,44 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.vec = (reinterpret_cast<uintptr_t>(A) & 15) == 0 && lda % 8 == 0 && w->K % 8 == 0;
   p.epilogue = epilogue;
   p.rotary = rotary;
-  const int nt = M <= 8 ? 1 : 2;
-  const long long tiles = ((long long)M + 8 * nt - 1) / (8 * nt);
-  if (tiles > 65535) return set_error(MK_ERR_INVALID, "%s: M=%d is too large", what, M);
-  p.split = 1;
-  while (p.split < 8 && p.form.strips * tiles * p.split < 4LL * sms && p.split * kW4Warps < p.form.blocks)
-    p.split *= 2;
-  const dim3 grid((unsigned)(p.form.strips * p.split), (unsigned)tiles, 1);
+  const W4StreamPlan pl = w4_stream_plan(p.form, M, sms);
+  p.stage_bytes = pl.stage_bytes;
+  p.split = pl.split;
+  if (pl.token_tiles > 65535 || pl.ctas > 0x7fffffffLL)
+    return set_error(MK_ERR_INVALID, "%s: M=%d, N=%d is too large", what, M, w->N);
+  const dim3 grid((unsigned)pl.ctas, (unsigned)pl.token_tiles, 1);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (w->dtype == MK_BF16)
-    return nt == 1 ? w4_stream_group<__nv_bfloat16, 1>(p, grid, s) : w4_stream_group<__nv_bfloat16, 2>(p, grid, s);
-  return nt == 1 ? w4_stream_group<__half, 1>(p, grid, s) : w4_stream_group<__half, 2>(p, grid, s);
+  return w->dtype == MK_BF16 ? w4_stream_type<__nv_bfloat16>(p, pl, grid, s)
+                             : w4_stream_type<__half>(p, pl, grid, s);
+}
+
+template <typename T, typename S>
+static int w4_quantize_group(const W4PackParams& p, unsigned grid, cudaStream_t s) {
+  const bool z = p.form.zeros;
+  auto kern = p.form.group == 32   ? (z ? w4_quantize_kernel<T, S, 32, true> : w4_quantize_kernel<T, S, 32, false>)
+              : p.form.group == 64 ? (z ? w4_quantize_kernel<T, S, 64, true> : w4_quantize_kernel<T, S, 64, false>)
+                                   : (z ? w4_quantize_kernel<T, S, 128, true> : w4_quantize_kernel<T, S, 128, false>);
+  kern<<<grid, kW4PackThreads, 0, s>>>(p);
+  MKB_CUDA(cudaGetLastError());
+  return MK_OK;
 }
 
 template <typename T>
 static int w4_quantize_launch(const W4PackParams& p, int src_dtype, unsigned grid, cudaStream_t s) {
-  if (src_dtype == MK_BF16) w4_quantize_kernel<T, __nv_bfloat16><<<grid, kW4PackThreads, 0, s>>>(p);
-  else if (src_dtype == MK_FP16) w4_quantize_kernel<T, __half><<<grid, kW4PackThreads, 0, s>>>(p);
-  else w4_quantize_kernel<T, float><<<grid, kW4PackThreads, 0, s>>>(p);
-  MKB_CUDA(cudaGetLastError());
-  return MK_OK;
+  if (src_dtype == MK_BF16) return w4_quantize_group<T, __nv_bfloat16>(p, grid, s);
+  if (src_dtype == MK_FP16) return w4_quantize_group<T, __half>(p, grid, s);
+  return w4_quantize_group<T, float>(p, grid, s);
 }
 
 template <typename T>
 static int w4_dequantize_launch(const W4Form& f, const uint8_t* data, void* out, long long ld, int dtype, int vec,
                                 unsigned grid, cudaStream_t s) {
   if (dtype == MK_BF16)
-    w4_dequantize_kernel<T><<<grid, 256, 0, s>>>(f, data, static_cast<__nv_bfloat16*>(out), ld, vec);
+    w4_dequantize_kernel<T><<<grid, kW4PackThreads, 0, s>>>(f, data, static_cast<__nv_bfloat16*>(out), ld, vec);
   else if (dtype == MK_FP16)
-    w4_dequantize_kernel<T><<<grid, 256, 0, s>>>(f, data, static_cast<__half*>(out), ld, vec);
+    w4_dequantize_kernel<T><<<grid, kW4PackThreads, 0, s>>>(f, data, static_cast<__half*>(out), ld, vec);
   else
-    w4_dequantize_kernel<T><<<grid, 256, 0, s>>>(f, data, static_cast<float*>(out), ld, vec);
+    w4_dequantize_kernel<T><<<grid, kW4PackThreads, 0, s>>>(f, data, static_cast<float*>(out), ld, vec);
   MKB_CUDA(cudaGetLastError());
   return MK_OK;
 }

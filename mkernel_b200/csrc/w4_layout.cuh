@@ -15,8 +15,7 @@
 // g + 8 (i % 2), column pair i / 2), element e: (word >> 4 i) & 0x000f000f is the register's two
 // codes in the low bits of its two halves.
 // Scales and offsets of a group: [g][tile][2], 16 bits each, so that a lane takes the eight that
-// belong to its rows with one 16-byte access.  An offset is the 16-bit float of base + zero point
-// (see W4Traits).
+// belong to its rows with one 16-byte access.  An offset is -zero point * kUnit (see W4Traits).
 //
 // A strip's rows are chosen so that rows g and g + 8 of a tile, which end in one thread, are the
 // two rows that an epilogue combines: neighbours 8 apart (plain), gate and up of one output, or
@@ -65,38 +64,59 @@ __host__ __device__ inline int w4_row(const W4Form& f, int strip, int p, int j) 
   return head * f.head_dim + (apart ? i + j * (f.rotary_dim / 2) : 2 * i + j);
 }
 
-// Per type of the scales and activations.  A code 0..15 put into the low mantissa bits of `magic`
-// is magic's value plus the code, exactly; taking away the offset (that value plus the zero
-// point, also exact) leaves code - zero exactly.
+// Per type of the scales and activations.  Up to 8 low bits of a 16-bit float, its exponent otherwise
+// 0, are a subnormal: that whole number of the smallest steps (2^-133 in bf16, 2^-24 in fp16; bf16's eighth
+// bit is the lowest of the exponent, where the steps are still the same).  So a code needs no
+// conversion: masked in place it is a float, and one fused multiply-add scales it up by a power of
+// two and takes the zero point away, exactly.  What comes out is (code - zero) * kUnit, the largest unit
+// that the largest power of two allows; its inverse is multiplied in at the end, also exactly.
 template <typename T> struct W4Traits;
 template <> struct W4Traits<__nv_bfloat16> {
-  using T2 = __nv_bfloat162;
-  static constexpr uint32_t kMagic = 0x43004300u;   // 128, one unit in the last place is 1
-  static constexpr uint32_t kEight = 0x43084308u;   // 136: the offset without zero points
-  static __device__ __forceinline__ float to_float(uint32_t bits) {
-    return __uint_as_float(bits << 16);
+  static constexpr uint32_t kLow = 0x7f007f00u;       // 2^127: a code in bits 0..3
+  static constexpr uint32_t kHigh = 0x7d007d00u;      // 2^123: in bits 4..7, where it is 16 times as much
+  static constexpr uint32_t kMinusEight = 0xbe00be00u;   // -8 kUnit
+  static constexpr float kUnit = 0x1p-6f;
+  static __device__ __forceinline__ float to_float(uint32_t bits) { return __uint_as_float(bits << 16); }
+  static __device__ __forceinline__ float2 to_float2(uint32_t two) {
+    return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
   }
   static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+  }
 };
 template <> struct W4Traits<__half> {
-  using T2 = __half2;
-  static constexpr uint32_t kMagic = 0x64006400u;   // 1024
-  static constexpr uint32_t kEight = 0x64086408u;   // 1032
+  static constexpr uint32_t kLow = 0x78007800u;       // 2^15
+  static constexpr uint32_t kHigh = 0x68006800u;      // 2^11
+  static constexpr uint32_t kMinusEight = 0xa400a400u;
+  static constexpr float kUnit = 0x1p-9f;
   static __device__ __forceinline__ float to_float(uint32_t bits) {
     return __half2float(__ushort_as_half((unsigned short)bits));
   }
+  static __device__ __forceinline__ float2 to_float2(uint32_t two) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&two));
+  }
   static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+  }
 };
 
-// The two codes of operand register i of a word as (code - zero) in T, given the offset twice.
+// The four operand registers of a word, each two codes as (code - zero) kUnit; off0 and off1: -zero kUnit
+// of rows g and g + 8, each twice.  Nibble 0 is row g, nibble 1 row g + 8, nibbles 2 and 3 the next pair
+// of columns.
 template <typename T>
-__device__ __forceinline__ uint32_t w4_decode(uint32_t word, int i, uint32_t offset2) {
-  using T2 = typename W4Traits<T>::T2;
-  uint32_t v;
-  // (word >> 4 i) & 0x000f000f | magic as one three-input operation after the shift
-  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(v) : "r"(word >> (4 * i)), "r"(W4Traits<T>::kMagic));
-  T2 r = __hsub2(*reinterpret_cast<T2*>(&v), *reinterpret_cast<T2*>(&offset2));
-  return *reinterpret_cast<uint32_t*>(&r);
+__device__ __forceinline__ void w4_decode(uint32_t word, uint32_t off0, uint32_t off1, uint32_t (&a)[4]) {
+  using W = W4Traits<T>;
+  const uint32_t next = word >> 8;
+  a[0] = W::fma2(word & 0x000f000fu, W::kLow, off0);
+  a[1] = W::fma2(word & 0x00f000f0u, W::kHigh, off1);
+  a[2] = W::fma2(next & 0x000f000fu, W::kLow, off0);
+  a[3] = W::fma2(next & 0x00f000f0u, W::kHigh, off1);
 }
 
 }  // namespace mkb

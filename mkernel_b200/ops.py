@@ -30,6 +30,16 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _raw_stream_of(index: int):
+    """The current torch stream of device `index` as an address."""
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
 class _on_device:
     """Make `index` the current CUDA device for the duration of a call; free when it already is
     (the common case: one process per GPU), since these wrappers sit on latency-bound paths."""
@@ -153,20 +163,20 @@ class W4Weight:
     def __init__(self, N: int, K: int, group: int, dtype: torch.dtype, zero_points: bool, device,
                  form: str = "plain", head_dim: int = 0, rotary_dim: int = 0, rotated_heads: int = 0,
                  interleaved: bool = False):
-        _require(form in _W4_FORMS, f"form must be one of {sorted(_W4_FORMS)}")
+        if form not in _W4_FORMS:
+            _require(False, f"form must be one of {sorted(_W4_FORMS)}")
         _require(dtype in (torch.bfloat16, torch.float16), "4-bit weights have bfloat16 or float16 scales")
         _require(form == "rotary" or not (head_dim or rotary_dim or rotated_heads or interleaved),
                  "head_dim, rotary_dim, rotated_heads and interleaved belong to form 'rotary'")
-        self.shape, self.group, self.dtype, self.form = (int(N), int(K)), int(group), dtype, form
-        self.zero_points = bool(zero_points)
-        self.rotary_dim = int(rotary_dim)
-        self.view = _lib.W4View(None, int(N), int(K), self.group, _DTYPES[dtype], int(self.zero_points),
-                                _W4_FORMS[form], int(head_dim), int(rotary_dim), int(rotated_heads),
-                                int(bool(interleaved)))
+        self.shape, self.K, self.group, self.dtype, self.form = (N, K), K, group, dtype, form
+        self.n_out = N // 2 if form == "gate_up" else N
+        self.zero_points, self.rotary_dim = bool(zero_points), rotary_dim
+        self.view = _lib.W4View(None, N, K, group, _DTYPES[dtype], bool(zero_points), _W4_FORMS[form],
+                                head_dim, rotary_dim, rotated_heads, bool(interleaved))
         self.view_ref = ctypes.byref(self.view)
         nbytes = _lib.check(_lib.lib().mk_w4_bytes(self.view_ref))
         self.data = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        self.device = self.data.device
+        self.device, self.index = self.data.device, self.data.get_device()
         self.view.data = self.data.data_ptr()
 
     def dequantize(self, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -174,12 +184,13 @@ class W4Weight:
         ``w4_pack``, in ``out``'s type (by default a new tensor of this weight's type)."""
         if out is None:
             out = torch.empty(self.shape, dtype=self.dtype, device=self.device)
-        _require(out.device == self.device and out.dtype in _DTYPES and tuple(out.shape) == self.shape
-                 and out.stride(1) == 1 and out.stride(0) >= self.shape[1],
-                 f"out must be {self.shape} on {self.device}, bfloat16, float16 or float32, rows contiguous")
-        with _on_device(self.device):
-            _lib.check(_lib.lib().mk_w4_dequantize(self.view_ref, out.data_ptr(), out.stride(0),
-                                                   _DTYPES[out.dtype], _stream()))
+        (N, K), (ld, step) = self.shape, out.stride() if out.dim() == 2 else (0, 0)
+        if out.get_device() != self.index or out.dtype not in _DTYPES or out.shape != self.shape or \
+                (step != 1 and K > 1) or (ld < K and N > 1):
+            _require(False, f"out must be {self.shape} on {self.device}, bfloat16, float16 or float32, rows contiguous")
+        with _on_device(self.index):
+            _lib.check(_lib.lib().mk_w4_dequantize(self.view_ref, out.data_ptr(), ld if N > 1 else K,
+                                                   _DTYPES[out.dtype], _raw_stream_of(self.index)))
         return out
 
 
@@ -196,10 +207,12 @@ def w4_quantize(weight: torch.Tensor, group: int = 128, zero_points: bool = Fals
     _require(weight.stride(1) == 1 or weight.shape[1] == 1, "weight's rows must be contiguous")
     dtype = dtype or (weight.dtype if weight.dtype != torch.float32 else torch.bfloat16)
     N, K = weight.shape
+    ld = weight.stride(0) if N > 1 else K
+    _require(ld >= K, "weight's rows overlap")
     W = W4Weight(N, K, group, dtype, zero_points, weight.device, **form)
-    with _on_device(weight.device):
-        _lib.check(_lib.lib().mk_w4_quantize(W.view_ref, weight.data_ptr(), max(weight.stride(0), K),
-                                             _DTYPES[weight.dtype], _stream()))
+    with _on_device(W.index):
+        _lib.check(_lib.lib().mk_w4_quantize(W.view_ref, weight.data_ptr(), ld, _DTYPES[weight.dtype],
+                                             _raw_stream_of(W.index)))
     return W
 
 
@@ -222,68 +235,79 @@ def w4_pack(codes: torch.Tensor, scales: torch.Tensor, zero_points: torch.Tensor
              f"scales must be [N, ceil(K / group)] with a group of 32, 64 or 128 (K={K})")
     _require(zero_points is None or zero_points.shape == scales.shape, "zero_points must have the scales' shape")
     W = W4Weight(N, K, group, scales.dtype, zero_points is not None, codes.device, **form)
-    with _on_device(codes.device):
+    with _on_device(W.index):
         _lib.check(_lib.lib().mk_w4_pack(W.view_ref, codes.data_ptr(), scales.data_ptr(),
                                          zero_points.data_ptr() if zero_points is not None else None,
-                                         _stream()))
+                                         _raw_stream_of(W.index)))
     return W
 
 
-def _w4_operands(A: torch.Tensor, W: W4Weight, C: torch.Tensor, n_out: int) -> None:
-    _require(isinstance(W, W4Weight), "W must be a W4Weight (w4_quantize, w4_pack)")
-    dev, dtype = W.device, W.dtype
-    _require(A.device == dev and C.device == dev, f"A and C must be on the weights' device {dev}")
-    _require(A.dtype == dtype and C.dtype == dtype, f"A and C must be {dtype} like the weights' scales")
-    _require(A.dim() == 2 and A.shape[1] == W.shape[1], f"A must be [M, {W.shape[1]}]")
-    _require(C.dim() == 2 and C.shape[0] == A.shape[0] and C.shape[1] == n_out,
-             f"C must be [{A.shape[0]}, {n_out}]")
-    _require((A.stride(1) == 1 or A.shape[1] == 1) and (C.stride(1) == 1 or n_out == 1),
-             "rows of A and C must be contiguous")
-
-
-def _rows(t: torch.Tensor) -> int:
-    """Row stride of a matrix; a single row may have any."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _w4_launch(call, A: torch.Tensor, W: W4Weight, C: torch.Tensor, form: str, *more) -> None:
+    """Checks A [M, K] and C [M, outputs of W] and calls a product.  On the path of every token: each
+    property of a tensor is read once, and what a message needs only when there is one."""
+    if not isinstance(W, W4Weight) or W.form != form:
+        _require(False, f"W must be a W4Weight of form '{form}' (w4_quantize, w4_pack)")
+    a_shape, c_shape, a_stride, c_stride = A.shape, C.shape, A.stride(), C.stride()
+    index, dtype = W.index, W.dtype
+    if A.get_device() != index or C.get_device() != index:
+        _require(False, f"A and C must be on the weights' device cuda:{index}")
+    if A.dtype is not dtype or C.dtype is not dtype:
+        _require(False, f"A and C must be {dtype} like the weights' scales")
+    K, n_out = W.K, W.n_out
+    if len(a_shape) != 2 or a_shape[1] != K:
+        _require(False, f"A must be [M, {K}]")
+    M = a_shape[0]
+    if len(c_shape) != 2 or c_shape[0] != M or c_shape[1] != n_out:
+        _require(False, f"C must be [{M}, {n_out}]")
+    if (a_stride[1] != 1 and K != 1) or (c_stride[1] != 1 and n_out != 1):
+        _require(False, "rows of A and C must be contiguous")
+    lda, ldc = (a_stride[0], c_stride[0]) if M > 1 else (K, n_out)     # one row may have any stride
+    if M > 1 and ldc < n_out:
+        _require(False, "rows of C overlap")
+    if _current_device() != index:
+        with _on_device(index):
+            _lib.check(call(A.data_ptr(), lda, W.view_ref, C.data_ptr(), ldc, M, *more, _raw_stream_of(index)))
+        return
+    if call(A.data_ptr(), lda, W.view_ref, C.data_ptr(), ldc, M, *more, _raw_stream_of(index)) < 0:
+        _lib.check(-1)
 
 
 def w4_gemm(A: torch.Tensor, W: W4Weight, C: torch.Tensor) -> None:
     """C[M, N] = A[M, K] @ W^T with 4-bit weights: the single-token and small-batch form of
     ``gemm_bf16``.  A and C in the type of W's scales, any row strides; fp32 sums, rounded once."""
-    _w4_operands(A, W, C, W.shape[0])
-    with _on_device(W.device):
-        _lib.check(_lib.lib().mk_w4_gemm(A.data_ptr(), _rows(A), W.view_ref, C.data_ptr(), _rows(C),
-                                         A.shape[0], _stream()))
+    _w4_launch(_lib.lib().mk_w4_gemm, A, W, C, "plain")
 
 
 def w4_gemm_swiglu(A: torch.Tensor, W: W4Weight, H: torch.Tensor) -> None:
     """H[M, N/2] = silu(A @ G^T) * (A @ U^T), W of form "gate_up": the single-token form of
     ``ag_gemm_swiglu_launch``."""
-    _w4_operands(A, W, H, W.shape[0] // 2)
-    with _on_device(W.device):
-        _lib.check(_lib.lib().mk_w4_gemm_swiglu(A.data_ptr(), _rows(A), W.view_ref, H.data_ptr(),
-                                                _rows(H), A.shape[0], _stream()))
+    _w4_launch(_lib.lib().mk_w4_gemm_swiglu, A, W, H, "gate_up")
 
 
-def _rotary_operands(positions: torch.Tensor, inv_freq: torch.Tensor, rows: int, pairs: int, dev) -> None:
-    _require(positions.device == dev and inv_freq.device == dev, f"positions and inv_freq must be on {dev}")
-    _require(positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous() and
-             tuple(positions.shape) == (rows,), f"positions must be contiguous int32 or int64 [{rows}]")
-    _require(inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and inv_freq.dim() == 1 and
-             (pairs < 0 or inv_freq.shape[0] == pairs),
-             "inv_freq must be contiguous float32 [rotary_dim / 2]")
+def _rotary_operands(positions: torch.Tensor, inv_freq: torch.Tensor, rows: int, pairs: int, index: int) -> int:
+    """Checks the operands that say how far to turn; returns whether positions have 64 bits."""
+    if positions.get_device() != index or inv_freq.get_device() != index:
+        _require(False, f"positions and inv_freq must be on cuda:{index}")
+    wide = positions.dtype is torch.int64
+    shape = positions.shape
+    if not (wide or positions.dtype is torch.int32) or len(shape) != 1 or shape[0] != rows or \
+            (rows > 1 and positions.stride(0) != 1):
+        _require(False, f"positions must be contiguous int32 or int64 [{rows}]")
+    shape = inv_freq.shape
+    if inv_freq.dtype is not torch.float32 or len(shape) != 1 or (pairs >= 0 and shape[0] != pairs) or \
+            (shape[0] > 1 and inv_freq.stride(0) != 1):
+        _require(False, "inv_freq must be contiguous float32 [rotary_dim / 2]")
+    return wide
 
 
 def w4_gemm_rotary(A: torch.Tensor, W: W4Weight, C: torch.Tensor, positions: torch.Tensor,
                    inv_freq: torch.Tensor, scale: float = 1.0) -> None:
     """C[M, N] = A @ W^T, W of form "rotary": the query/key/value projection of M tokens with the
     rotated heads of row m turned by positions[m] before the rounding (see ``rotary``)."""
-    _w4_operands(A, W, C, W.shape[0])
-    _rotary_operands(positions, inv_freq, A.shape[0], W.rotary_dim // 2, W.device)
-    with _on_device(W.device):
-        _lib.check(_lib.lib().mk_w4_gemm_rotary(A.data_ptr(), _rows(A), W.view_ref, C.data_ptr(),
-                                                _rows(C), A.shape[0], positions.data_ptr(),
-                                                positions.dtype == torch.int64, inv_freq.data_ptr(),
-                                                scale, _stream()))
+    if not isinstance(W, W4Weight) or W.form != "rotary":
+        _require(False, "W must be a W4Weight of form 'rotary' (w4_quantize, w4_pack)")
+    wide = _rotary_operands(positions, inv_freq, A.shape[0] if A.dim() else 0, W.rotary_dim // 2, W.index)
+    _w4_launch(_lib.lib().mk_w4_gemm_rotary, A, W, C, "rotary", positions.data_ptr(), wide, inv_freq.data_ptr(), scale)
 
 
 def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -295,47 +319,39 @@ def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     it is X.  ``inverse`` turns back, which is the gradient: dX = rotary(dY, ..., inverse=True).
     Features contiguous, any row and head strides: the queries and keys of a projection
     [rows, (heads + ...) * head_dim] are a view of its output."""
-    Y = X if Y is None else Y
-    _require(isinstance(X, torch.Tensor) and X.is_cuda and X.dtype in _DTYPES and X.dim() == 3,
-             "X must be a CUDA tensor [rows, heads, head_dim] of bfloat16, float16 or float32")
-    _require(Y.device == X.device and Y.dtype == X.dtype and Y.shape == X.shape,
-             "Y must have X's device, type and shape")
-    rows, heads, dim = X.shape
-    _require(dim == 1 or (X.stride(2) == 1 and Y.stride(2) == 1), "features of X and Y must be contiguous")
-    _rotary_operands(positions, inv_freq, rows, -1, X.device)
-    if Y is not X:
-        _require(not _overlap(X, Y), "Y must be X or share no memory with it")
-    _require(_distinct(Y), "two elements of Y share memory")
-    with _on_device(X.device):
-        _lib.check(_lib.lib().mk_rotary(X.data_ptr(), X.stride(0), X.stride(1), Y.data_ptr(),
-                                        Y.stride(0), Y.stride(1), rows, heads, dim,
-                                        2 * inv_freq.shape[0], _DTYPES[X.dtype], positions.data_ptr(),
-                                        positions.dtype == torch.int64, inv_freq.data_ptr(), scale,
-                                        interleaved, inverse, _stream()))
+    if not isinstance(X, torch.Tensor) or not X.is_cuda or X.dtype not in _DTYPES or X.dim() != 3:
+        _require(False, "X must be a CUDA tensor [rows, heads, head_dim] of bfloat16, float16 or float32")
+    shape, xs, index = X.shape, X.stride(), X.get_device()
+    rows, heads, dim = shape
+    if Y is None or Y is X:
+        Y, ys = X, xs
+    else:
+        if Y.get_device() != index or Y.dtype is not X.dtype or Y.shape != shape:
+            _require(False, "Y must have X's device, type and shape")
+        ys = Y.stride()
+        if _overlap(X, xs, Y, ys, shape):
+            _require(False, "Y must be X or share no memory with it")
+    if dim > 1 and (xs[2] != 1 or ys[2] != 1):
+        _require(False, "features of X and Y must be contiguous")
+    # No two elements of Y at one address: one of the outer dimensions steps over all inside it.
+    if not ((heads < 2 or ys[1] >= dim) and (rows < 2 or ys[0] >= (heads - 1) * ys[1] + dim) or
+            (rows < 2 or ys[0] >= dim) and (heads < 2 or ys[1] >= (rows - 1) * ys[0] + dim)):
+        _require(False, "two elements of Y share memory")
+    wide = _rotary_operands(positions, inv_freq, rows, -1, index)
+    with _on_device(index):
+        _lib.check(_lib.lib().mk_rotary(X.data_ptr(), xs[0], xs[1], Y.data_ptr(), ys[0], ys[1], rows, heads, dim,
+                                        2 * inv_freq.shape[0], _DTYPES[X.dtype], positions.data_ptr(), wide,
+                                        inv_freq.data_ptr(), scale, interleaved, inverse, _raw_stream_of(index)))
     return Y
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    size = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
-    return t.data_ptr(), t.data_ptr() + size * t.element_size()
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    if a.numel() == 0:
+def _overlap(a: torch.Tensor, a_stride, b: torch.Tensor, b_stride, shape) -> bool:
+    """Whether the address ranges of two tensors of one shape and type meet."""
+    if 0 in shape:
         return False
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
-
-
-def _distinct(t: torch.Tensor) -> bool:
-    """No two elements of [rows, heads, dim] (features contiguous) at one address: one of the two
-    outer dimensions steps over everything inside it."""
-    if t.is_contiguous():
-        return True
-    (rows, heads, dim), (sr, sh, _) = t.shape, t.stride()
-    by_row = (heads < 2 or sh >= dim) and (rows < 2 or sr >= (heads - 1) * sh + dim)
-    by_head = (rows < 2 or sr >= dim) and (heads < 2 or sh >= (rows - 1) * sr + dim)
-    return by_row or by_head
+    a0, b0, size = a.data_ptr(), b.data_ptr(), a.element_size()
+    last = lambda strides: size * (1 + sum((n - 1) * s for n, s in zip(shape, strides)))
+    return a0 < b0 + last(b_stride) and b0 < a0 + last(a_stride)
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | None = None,
