@@ -11,113 +11,132 @@
 
 namespace mkb {
 
+// Division of an int below 2^31 by a fixed positive int, as a multiplication (Granlund and Montgomery).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  FastDiv() = default;
+  explicit FastDiv(int divisor) : d((uint32_t)divisor), shift(0) {
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 struct RotaryParams {
   const void* x;
   void* y;
   long long x_row, x_head, y_row, y_head;   // strides in elements
   long long rows;
   int heads, head_dim, rotary_dim;
-  int slots, turned;       // of a row; the first `turned` turn, the rest copy
-  int heads_each;          // heads that a thread walks
+  int turned;              // slots of a head that turn; the others copy
+  int rows_each;           // rows of a CTA
+  FastDiv slots, per_row;  // slots of a head; of a row
   float sign;
   RotaryArgs rotary;
 };
 
-constexpr int kRotaryThreads = 128;
-constexpr int kRotaryAhead = 4;   // heads whose loads a thread has in flight
+constexpr int kRotaryThreads = 256;
+constexpr int kRotaryAhead = 2;      // slots whose loads a thread has in flight
+constexpr int kRotaryAngles = 2048;  // of a CTA (16 KB of shared memory)
 
 template <typename T, int P> struct alignas(sizeof(T) * P) RotaryVec { T v[P]; };
 
-// A slot is P pairs of features: vector 0 and vector 1 of P elements each, which are the first and
-// second features of the pairs, or, interleaved, the pairs one after another.  A thread has a slot
-// of a row, takes its P angles once and walks heads_each heads; neighbouring threads have
-// neighbouring slots.  Angles cost P sines and cosines (in 64 bits up to the turn), so the more heads
-// share them the better, as long as there are enough threads to keep memory busy.
+// A slot is P pairs of features of a head: vector 0 and vector 1 of P elements each, which are the
+// first and second features of the pairs, or, interleaved, the pairs one after another.  A CTA has a few
+// whole rows.  Its threads ask for their first slots' features, then work out the rows' angles, each
+// once (sine and cosine, in 64 bits up to the turn, cost as much as turning several heads), and
+// find them in shared memory for every head.
 template <typename T, int P, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
   using Vec = RotaryVec<T, P>;
+  __shared__ __align__(16) float2 angles[kRotaryAngles];
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const unsigned long long e = (unsigned long long)blockIdx.x * kRotaryThreads + threadIdx.x;
-  const unsigned long long total = (unsigned long long)p.rows * p.slots;
-  if (e >= total) return;
-  long long row;
-  int slot;
-  if (total <= 0xffffffffu) {
-    row = (uint32_t)e / (uint32_t)p.slots;
-    slot = (int)((uint32_t)e % (uint32_t)p.slots);
-  } else {
-    row = (long long)(e / p.slots);
-    slot = (int)(e % p.slots);
-  }
-  const int h0 = blockIdx.y * p.heads_each;
-  const int heads = min(p.heads_each, p.heads - h0);
-  const T* x = static_cast<const T*>(p.x) + row * p.x_row + (long long)h0 * p.x_head;
-  T* y = static_cast<T*>(p.y) + row * p.y_row + (long long)h0 * p.y_head;
+  const long long row0 = (long long)blockIdx.x * p.rows_each;
+  const int rows = (int)min((long long)p.rows_each, p.rows - row0);
+  const uint32_t items = rows * p.per_row.d;
+  const int pairs = p.rotary_dim / 2;
 
-  if (slot >= p.turned) {   // features that are copied; the last vector may not exist
-    const int at = p.rotary_dim + (slot - p.turned) * 2 * P;
-    const bool two = at + P < p.head_dim;
-#pragma unroll kRotaryAhead
-    for (int h = 0; h < heads; ++h, x += p.x_head, y += p.y_head) {
-      *reinterpret_cast<Vec*>(y + at) = *reinterpret_cast<const Vec*>(x + at);
-      if (two) *reinterpret_cast<Vec*>(y + at + P) = *reinterpret_cast<const Vec*>(x + at + P);
-    }
-    return;
+  struct Item { const T* x; T* y; int a, b, angle; bool turns, second; };
+  auto item = [&](uint32_t e) {
+    const uint32_t r = p.per_row.div(e), in_row = e - r * p.per_row.d;
+    const uint32_t h = p.slots.div(in_row);
+    const int slot = (int)(in_row - h * p.slots.d);
+    Item i;
+    i.x = static_cast<const T*>(p.x) + (row0 + r) * p.x_row + h * p.x_head;
+    i.y = static_cast<T*>(p.y) + (row0 + r) * p.y_row + h * p.y_head;
+    i.turns = slot < p.turned;
+    i.a = !i.turns ? p.rotary_dim + (slot - p.turned) * 2 * P : INTERLEAVED ? slot * 2 * P : slot * P;
+    i.b = i.turns && !INTERLEAVED ? i.a + pairs : i.a + P;
+    i.second = i.b < p.head_dim;        // the last vector of a head's copied features may not exist
+    i.angle = (int)r * pairs + slot * P;
+    return i;
+  };
+  auto load = [&](uint32_t e, Vec& u, Vec& v) {
+    if (e >= items) return;
+    const Item i = item(e);
+    u = *reinterpret_cast<const Vec*>(i.x + i.a);
+    if (i.second) v = *reinterpret_cast<const Vec*>(i.x + i.b);
+  };
+
+  Vec u[kRotaryAhead], v[kRotaryAhead];
+#pragma unroll
+  for (int c = 0; c < kRotaryAhead; ++c) load(threadIdx.x + c * kRotaryThreads, u[c], v[c]);
+  for (int e = threadIdx.x; e < rows * pairs; e += kRotaryThreads) {
+    const int r = rows == 1 ? 0 : e / pairs;
+    float2 cs = rotary_cos_sin(rotary_position(p.rotary, row0 + r), __ldg(p.rotary.inv_freq + (e - r * pairs)),
+                               p.rotary.scale);
+    cs.y *= p.sign;
+    angles[e] = cs;
   }
-  const int a = INTERLEAVED ? slot * 2 * P : slot * P;
-  const int b = INTERLEAVED ? a + P : a + p.rotary_dim / 2;
-  float2 cs[P];
-  const long long position = rotary_position(p.rotary, row);
+  __syncthreads();
+  for (uint32_t e0 = threadIdx.x; e0 < items; e0 += kRotaryAhead * kRotaryThreads) {
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    cs[i] = rotary_cos_sin(position, __ldg(p.rotary.inv_freq + slot * P + i), p.rotary.scale);
-    cs[i].y *= p.sign;
-  }
-  for (int h = 0; h < heads; h += kRotaryAhead) {
-    Vec u[kRotaryAhead], v[kRotaryAhead];
-#pragma unroll
-    for (int i = 0; i < kRotaryAhead; ++i)
-      if (h + i < heads) {
-        u[i] = *reinterpret_cast<const Vec*>(x + i * p.x_head + a);
-        v[i] = *reinterpret_cast<const Vec*>(x + i * p.x_head + b);
-      }
-#pragma unroll
-    for (int i = 0; i < kRotaryAhead; ++i)
-      if (h + i < heads) {
+    for (int c = 0; c < kRotaryAhead; ++c) {
+      const uint32_t e = e0 + c * kRotaryThreads;
+      if (e >= items) break;
+      const Item i = item(e);
+      if (i.turns) {
 #pragma unroll
         for (int k = 0; k < P; ++k) {
           // pair k: elements k of both vectors, or elements 2 k and 2 k + 1 of the two in a row
-          T& first = INTERLEAVED ? (2 * k < P ? u[i].v[2 * k % P] : v[i].v[2 * k % P]) : u[i].v[k];
-          T& second = INTERLEAVED ? (2 * k + 1 < P ? u[i].v[(2 * k + 1) % P] : v[i].v[(2 * k + 1) % P]) : v[i].v[k];
-          const float2 r = rotary_turn((float)first, (float)second, cs[k]);
+          T& first = INTERLEAVED ? (2 * k < P ? u[c].v[2 * k % P] : v[c].v[2 * k % P]) : u[c].v[k];
+          T& second = INTERLEAVED ? (2 * k + 1 < P ? u[c].v[(2 * k + 1) % P] : v[c].v[(2 * k + 1) % P]) : v[c].v[k];
+          const float2 r = rotary_turn((float)first, (float)second, angles[i.angle + k]);
           first = (T)r.x;
           second = (T)r.y;
         }
-        *reinterpret_cast<Vec*>(y + i * p.y_head + a) = u[i];
-        *reinterpret_cast<Vec*>(y + i * p.y_head + b) = v[i];
       }
-    x += kRotaryAhead * p.x_head;
-    y += kRotaryAhead * p.y_head;
+      *reinterpret_cast<Vec*>(i.y + i.a) = u[c];
+      if (i.second) *reinterpret_cast<Vec*>(i.y + i.b) = v[c];
+      load(e + kRotaryAhead * kRotaryThreads, u[c], v[c]);
+    }
   }
 }
 
 template <typename T, int P>
 static int rotary_launch(RotaryParams& p, bool interleaved, bool in_place, int sms, cudaStream_t stream) {
   p.turned = p.rotary_dim / 2 / P;
-  p.slots = p.turned + (in_place ? 0 : (p.head_dim - p.rotary_dim + 2 * P - 1) / (2 * P));
-  // As many heads to a thread as leave 512 threads to an SM: 8192 rows of 40 heads of 128 share an angle
-  // among all 40, one token's are taken by a thread each.
-  const long long threads = p.rows * p.slots;
-  long long parts = (512LL * sms + threads - 1) / threads;
-  if (parts > p.heads) parts = p.heads;
-  p.heads_each = (int)((p.heads + parts - 1) / parts);
-  parts = (p.heads + p.heads_each - 1) / p.heads_each;
-  const long long blocks = (threads + kRotaryThreads - 1) / kRotaryThreads;
-  if (blocks > 0x7fffffffLL || parts > 65535)
-    return set_error(MK_ERR_INVALID, "mk_rotary: %lld rows of %d heads are too many", p.rows, p.heads);
+  const int slots = p.turned + (in_place ? 0 : (p.head_dim - p.rotary_dim + 2 * P - 1) / (2 * P));
+  const long long per_row = (long long)p.heads * slots;
+  if (per_row > 1 << 30 || p.rotary_dim / 2 > kRotaryAngles)
+    return set_error(MK_ERR_INVALID, "mk_rotary: heads of %d (%d turned) features, %d to a row, are too many", p.head_dim,
+                     p.rotary_dim, p.heads);
+  // Rows of a CTA: enough to give every thread its first slots, and so many that one wave of four CTAs to an
+  // SM has them all (8192 rows of 40 heads of 128: 54 us with a CTA to each row, whose latency comes
+  // back with every wave); their angles must fit shared memory.
+  long long rows_each = kRotaryAhead * kRotaryThreads / per_row;
+  const long long wave = (p.rows + 4 * sms - 1) / (4 * sms);
+  if (rows_each < wave) rows_each = wave;
+  if (rows_each > kRotaryAngles / (p.rotary_dim / 2)) rows_each = kRotaryAngles / (p.rotary_dim / 2);
+  if (rows_each < 1) rows_each = 1;
+  p.rows_each = (int)rows_each;
+  p.slots = FastDiv(slots);
+  p.per_row = FastDiv((int)per_row);
+  const long long blocks = (p.rows + rows_each - 1) / rows_each;
+  if (blocks > 0x7fffffffLL) return set_error(MK_ERR_INVALID, "mk_rotary: %lld rows are too many", p.rows);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks, (unsigned)parts, 1);
+  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
   cfg.blockDim = dim3(kRotaryThreads, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

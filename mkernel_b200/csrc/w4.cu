@@ -16,12 +16,11 @@ namespace mkb {
 // ------------------------------------------------------------------------------------------
 // laying the weights out
 // ------------------------------------------------------------------------------------------
-// The unit of all three kernels is what a lane of the product holds of one tile and quarter of a
-// block: 8 consecutive columns of a pair of rows, 8 bytes of codes.  Sixteen neighbouring threads
-// take a block's 128 columns, so rows are read and written in whole 256-byte pieces, a group
-// is reduced by shuffles, and nothing passes through shared memory.
+// The unit of all three kernels is a lane's 16 bytes of codes in the layout: of a pair of rows, columns
+// 8 t and 32 + 8 t and the seven behind each, in one half of a block; a chunk has as many units as a
+// CTA has threads.  A unit is read and written with 16-byte accesses, four neighbouring threads
+// covering whole sectors; a group is reduced by shuffles, and nothing passes through shared memory.
 constexpr int kW4PackThreads = 256;
-constexpr int kW4Units = kW4Strip / 2 * kW4Block / 8;   // of a chunk
 
 struct W4PackParams {
   W4Form form;
@@ -33,19 +32,22 @@ struct W4PackParams {
   // quantise
   const void* src;
   long long ld;
-  int vec;   // 16-byte accesses to whole units are aligned
+  int vec;   // 16-byte accesses to eight columns are aligned
 };
 
-// Unit u of a chunk: pair of rows, column of the block, and where its codes lie.
-struct W4Unit { int pair, col, offset; };
-__device__ __forceinline__ W4Unit w4_unit(int u) {
-  const int pair = u >> 4, hq = u >> 2 & 3, t = u & 3;
-  return {pair, hq * 32 + t * 8, (((hq >> 1) * 4 + (pair >> 3)) * 32 + (pair & 7) * 4 + t) * 16 + (hq & 1) * 8};
+struct W4Unit { int pair, col; };   // columns col and col + 32 of the block
+__device__ __forceinline__ W4Unit w4_unit() {
+  // threads: t fastest, then the half, then the pair
+  const int i = threadIdx.x;
+  return {i >> 3, (i >> 2 & 1) * 64 + (i & 3) * 8};
+}
+__device__ __forceinline__ int w4_unit_offset(const W4Unit& u) {
+  return (((u.col >> 6) * 4 + (u.pair >> 3)) * 32 + (u.pair & 7) * 4 + (u.col >> 3 & 3)) * 16;
 }
 
-// A unit's word of four codes each of the pair's rows, from bytes c (lowest: first column).
+// A word of the layout from four codes each of the pair's rows, a byte each, first column lowest: columns
+// 0, 1, 2, 3 go to bits 0, 16, 8, 24.
 __device__ __forceinline__ uint32_t w4_word(uint32_t first, uint32_t second) {
-  // columns 0, 1, 2, 3 go to bits 0, 16, 8, 24
   return __byte_perm(first, 0, 0x3120) | __byte_perm(second, 0, 0x3120) << 4;
 }
 
@@ -61,62 +63,63 @@ __device__ __forceinline__ uint16_t w4_offset_bits(int zero) {
 }
 
 template <typename T>
-__device__ __forceinline__ void w4_store_scales(const W4Form& f, uint8_t* chunk, const W4Unit& u, const uint16_t (&s)[2],
+__device__ __forceinline__ void w4_store_scales(const W4Form& f, uint8_t* chunk, int pair, int col, const uint16_t (&s)[2],
                                                 const int (&zero)[2]) {
-  uint8_t* p = chunk + w4_scale_offset(u.pair, u.col / f.group);
+  uint8_t* p = chunk + w4_scale_offset(pair, col / f.group);
   *reinterpret_cast<uint32_t*>(p) = s[0] | (uint32_t)s[1] << 16;
   if (f.zeros)
     *reinterpret_cast<uint32_t*>(p + kW4Block / f.group * 128) =
         w4_offset_bits<T>(zero[0]) | (uint32_t)w4_offset_bits<T>(zero[1]) << 16;
 }
 
-// Codes behind the matrix are 8 and their scales 0, whoever lays them out.
+// Codes behind the matrix are 8, their scales 0 and zero points 8, whoever lays them out.
 template <typename T>
 __global__ void __launch_bounds__(kW4PackThreads) w4_pack_kernel(W4PackParams p) {
   const W4Form& f = p.form;
-  const int strip = blockIdx.x / f.blocks, block = blockIdx.x % f.blocks;
-  uint8_t* chunk = p.data + (size_t)blockIdx.x * f.chunk_bytes;
+  const int strip = blockIdx.y, block = blockIdx.x;
+  uint8_t* chunk = p.data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
   const long long row_bytes = ((long long)f.K + 1) / 2, groups = ((long long)f.K + f.group - 1) / f.group;
-  for (int i = threadIdx.x; i < kW4Units; i += kW4PackThreads) {
-    const W4Unit u = w4_unit(i);
-    const long long k = (long long)block * kW4Block + u.col;
-    uint32_t nibbles[2];   // of 8 columns
+  const W4Unit u = w4_unit();
+  uint32_t words[4];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int col = u.col + 32 * q;
+    const long long k = (long long)block * kW4Block + col;
+    uint32_t low[2], high[2];
     uint16_t scale[2];
     int zero[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int n = w4_row(f, strip, u.pair, j);
-      nibbles[j] = 0x88888888u;
+      uint32_t v = 0x88888888u;   // nibbles of 8 columns
       scale[j] = 0;
       zero[j] = 8;
       if (n >= 0 && k < f.K) {
         const uint8_t* c = p.codes + n * row_bytes + k / 2;
-        uint32_t v = 0;
+        v = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v |= (k + 2 * e < f.K ? (uint32_t)__ldg(c + e) : 0x88u) << (8 * e);
         if (k + 8 > f.K) {
           const uint32_t mask = (1u << (4 * (int)(f.K - k))) - 1;
           v = (v & mask) | (0x88888888u & ~mask);
         }
-        nibbles[j] = v;
-        if (u.col % f.group == 0) {
+        if (col % f.group == 0) {
           scale[j] = __ldg(p.scales + n * groups + k / f.group);
           if (f.zeros) zero[j] = __ldg(p.zero_points + n * groups + k / f.group) & 15;
         }
       }
+      low[j] = __byte_perm(v & 0x0f0f, (v >> 4) & 0x0f0f, 0x5140);
+      high[j] = __byte_perm((v >> 16) & 0x0f0f, (v >> 20) & 0x0f0f, 0x5140);
     }
-    // columns 0, 1, 2, 3 of each four from nibbles to bytes
-    uint32_t low[2], high[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      low[j] = __byte_perm(nibbles[j] & 0x0f0f, (nibbles[j] >> 4) & 0x0f0f, 0x5140);
-      high[j] = __byte_perm((nibbles[j] >> 16) & 0x0f0f, (nibbles[j] >> 20) & 0x0f0f, 0x5140);
-    }
-    *reinterpret_cast<uint2*>(chunk + u.offset) = make_uint2(w4_word(low[0], low[1]), w4_word(high[0], high[1]));
-    if (u.col % f.group == 0) w4_store_scales<T>(f, chunk, u, scale, zero);
+    words[2 * q] = w4_word(low[0], low[1]);
+    words[2 * q + 1] = w4_word(high[0], high[1]);
+    if (col % f.group == 0) w4_store_scales<T>(f, chunk, u.pair, col, scale, zero);
   }
+  *reinterpret_cast<uint4*>(chunk + w4_unit_offset(u)) = make_uint4(words[0], words[1], words[2], words[3]);
 }
 
+// Eight columns of a source row, and the smallest and largest of them and 0 (symmetric: the largest
+// magnitude alone); NaN where there is one.  16-bit types two at a time.
 __device__ __forceinline__ float w4_max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -127,149 +130,241 @@ __device__ __forceinline__ float w4_min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+template <typename S> struct W4Source;
+template <> struct W4Source<float> {
+  float v[8];
+  __device__ __forceinline__ float operator[](int i) const { return v[i]; }
+  __device__ __forceinline__ void load(const float* p) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  __device__ __forceinline__ void load(const float* p, int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? __ldg(p + i) : 0.0f;
+  }
+  template <bool ZEROS> __device__ __forceinline__ void range(float& lo, float& hi) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (ZEROS) lo = w4_min_nan(lo, v[i]);
+      hi = w4_max_nan(hi, ZEROS ? v[i] : fabsf(v[i]));
+    }
+  }
+};
+template <typename S> struct W4Source16 {
+  uint32_t v[4];
+  __device__ __forceinline__ float operator[](int i) const {
+    const float2 two = W4Traits<S>::to_float2(v[i / 2]);
+    return i & 1 ? two.y : two.x;
+  }
+  __device__ __forceinline__ void load(const S* p) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  }
+  __device__ __forceinline__ void load(const S* p, int n) {
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = (2 * i < n ? (uint32_t)__ldg(e + 2 * i) : 0u) | (2 * i + 1 < n ? (uint32_t)__ldg(e + 2 * i + 1) << 16 : 0u);
+  }
+  template <bool ZEROS> __device__ __forceinline__ void range(float& lo, float& hi) const {
+    uint32_t least = 0, most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (ZEROS) least = W4Traits<S>::min2(least, v[i]);
+      most = W4Traits<S>::max2(most, ZEROS ? v[i] : v[i] & 0x7fff7fffu);
+    }
+    const float2 a = W4Traits<S>::to_float2(least), b = W4Traits<S>::to_float2(most);
+    if (ZEROS) lo = w4_min_nan(lo, w4_min_nan(a.x, a.y));
+    hi = w4_max_nan(hi, w4_max_nan(b.x, b.y));
+  }
+};
+template <> struct W4Source<__nv_bfloat16> : W4Source16<__nv_bfloat16> {};
+template <> struct W4Source<__half> : W4Source16<__half> {};
 
-// w / s rounded to fp32, given r = 1 / s.  For w and s of 16 bits a quotient that is not half way between
-// two whole numbers is much further from there than fp32's last place, and one that is, is exact: one
-// correction of w r by its remainder (Markstein's last step) rounds the same way as the division.
-__device__ __forceinline__ float w4_quotient(float w, float s, float r) {
+// w / d rounded to fp32, given r within a few units of 1 / d: a correction by the remainder, which the
+// fused multiply-add gives exactly (Markstein).
+__device__ __forceinline__ float w4_quotient(float w, float d, float r) {
   const float q = w * r;
-  return __fmaf_rn(__fmaf_rn(-q, s, w), r, q);
+  return __fmaf_rn(__fmaf_rn(-q, d, w), r, q);
 }
 
 // Quantiser: reads the matrix once and writes the chunk.  Memory bounds it (2 or 4 bytes in, 0.53 out a
-// weight), arithmetic closely behind: hence the quotient above and the rounding by an addition.
+// weight), instructions closely behind.  Hence no division in the common case: the rounded quotient
+// of two 16-bit values is far from half way between whole numbers (2^-12 of it) unless it is exactly
+// there, and then w4_quotient is exact too, so both go the same way.  Nor a clamp below: the
+// quotient of the largest magnitude is within 2^-8 of 7, that of hi - lo of 15.  Both need a scale that
+// is no subnormal; for others, and for fp32 weights, it is divided and clamped as the definition says.
 template <typename T, typename S, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParams p) {
   const W4Form& f = p.form;
-  const int strip = blockIdx.x / f.blocks, block = blockIdx.x % f.blocks;
-  uint8_t* chunk = p.data + (size_t)blockIdx.x * f.chunk_bytes;
-#pragma unroll 1
-  for (int c = threadIdx.x; c < kW4Units; c += kW4PackThreads) {
-    const W4Unit u = w4_unit(c);
-    const int k = block * kW4Block + u.col;
-    const bool whole = p.vec && k + 8 <= f.K;
-    float w[2][8];
-    bool row[2];
+  const int strip = blockIdx.y, block = blockIdx.x;
+  uint8_t* chunk = p.data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
+  const W4Unit u = w4_unit();
+  const int k0 = block * kW4Block + u.col;
+  W4Source<S> w[2][2];
+  bool row[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int n = w4_row(f, strip, u.pair, j);
-      row[j] = n >= 0;
-      const S* src = static_cast<const S*>(p.src) + (long long)(n < 0 ? 0 : n) * p.ld + k;
-      if (row[j] && whole) {
-        constexpr int kPer = 16 / sizeof(S);
+  for (int j = 0; j < 2; ++j) {
+    const int n = w4_row(f, strip, u.pair, j);
+    row[j] = n >= 0;
+    const S* src = static_cast<const S*>(p.src) + (long long)(n < 0 ? 0 : n) * p.ld + k0;
 #pragma unroll
-        for (int e = 0; e < 8; e += kPer) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + e));
-          const S* x = reinterpret_cast<const S*>(&v);
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) w[j][e + i] = (float)x[i];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[j][e] = row[j] && k + e < f.K ? (float)__ldg(src + e) : 0.0f;
-      }
+    for (int q = 0; q < 2; ++q) {
+      const int k = k0 + 32 * q;
+      if (row[j] && p.vec && k + 8 <= f.K) w[j][q].load(src + 32 * q);
+      else w[j][q].load(src + 32 * q, row[j] ? f.K - k : 0);
     }
-    uint16_t scale_bits[2];
-    int zeros[2];
-    uint32_t low[2], high[2];
+  }
+  uint32_t words[4];
+  uint16_t scale_bits[2];
+  int zeros[2];
+  constexpr int kPasses = GROUP == 32 ? 2 : 1;   // groups that a unit meets
+  uint32_t codes[2][2][2];                       // row, q, first or second four columns; a byte each
+#pragma unroll
+  for (int pass = 0; pass < kPasses; ++pass) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      float lo = 0.0f, hi = 0.0f;   // symmetric: hi is the largest magnitude
+      float lo = 0.0f, hi = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (ZEROS) lo = w4_min_nan(lo, w[j][e]);
-        hi = w4_max_nan(hi, ZEROS ? w[j][e] : fabsf(w[j][e]));
-      }
+      for (int q = 0; q < 2; ++q)
+        if (kPasses == 1 || q == pass) w[j][q].template range<ZEROS>(lo, hi);
 #pragma unroll
-      for (int d = 1; d < GROUP / 8; d *= 2) {
+      for (int d = 1; d < (GROUP == 128 ? 8 : 4); d *= 2) {
         if (ZEROS) lo = w4_min_nan(lo, __shfl_xor_sync(~0u, lo, d));
         hi = w4_max_nan(hi, __shfl_xor_sync(~0u, hi, d));
       }
-      float range = ZEROS ? __fdiv_rn(hi - lo, 15.0f) : __fdiv_rn(hi, 7.0f);
-      if (!isfinite(hi) || !isfinite(lo)) range = __int_as_float(0x7fc00000);
+      const float span = ZEROS ? hi - lo : hi;
+      // Markstein's division by a constant is the division, but for subnormal results
+      const float n = ZEROS ? 15.0f : 7.0f;
+      float range = span < 0x1p-100f ? __fdiv_rn(span, n) : w4_quotient(span, n, 1.0f / n);
+      if (!(span <= 3.402823466e38f)) range = __int_as_float(0x7fc00000);   // an infinity or NaN in the group
       const T scale_t = W4Traits<T>::from_float(range);
       scale_bits[j] = *reinterpret_cast<const uint16_t*>(&scale_t);
       const float scale = W4Traits<T>::to_float(scale_bits[j]);
       const float divisor = scale == 0.0f ? 1.0f : scale;
-      zeros[j] = 8;
-      if (ZEROS && row[j] && k < f.K) zeros[j] = (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, divisor)), 0.0f), 15.0f);
-      // fp32 weights, and scales whose remainders could be lost among the subnormals, are divided
-      if (sizeof(S) == 2 && divisor >= 0x1p-90f && divisor <= 0x1p90f) {
-        const float inverse = __fdiv_rn(1.0f, divisor);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[j][e] = w4_quotient(w[j][e], divisor, inverse);
-      } else {
-#pragma unroll 1
-        for (int e = 0; e < 8; ++e) {
-          // one division at a time, in a loop that keeps w in registers
-          float q = __fdiv_rn(w[j][0], divisor);
-#pragma unroll
-          for (int i = 0; i < 7; ++i) w[j][i] = w[j][i + 1];
-          w[j][7] = q;
-        }
-      }
+      const bool plain = sizeof(S) == 2 && scale >= (sizeof(T) == 2 && W4Traits<T>::kUnit == 0x1p-9f ? 0x1p-14f : 0x1p-90f) &&
+                         scale <= 0x1p90f;
       // quotient + 1.5 2^23 is the rounded quotient in the low bits (ties to even)
       constexpr float kRound = 12582912.0f;
-      const float least = kRound - zeros[j], most = kRound + (15 - zeros[j]);
-      uint32_t b[8];
+      zeros[j] = 8;
+      if (plain) {
+        float inverse;
+        asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(divisor));
+        if (ZEROS) zeros[j] = (int)(__float_as_uint(w4_quotient(-lo, divisor, inverse) + kRound) & 15);
+        const float most = kRound + (15 - zeros[j]);
+        const uint32_t add = zeros[j] * 0x01010101u;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(fminf(fmaxf(w[j][e] + kRound, least), most));
-      // low bytes, each a two's complement number of -15..15: plus the zero point, none carries
-      const uint32_t add = zeros[j] * 0x01010101u;
-      low[j] = __vadd4(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410), add);
-      high[j] = __vadd4(__byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410), add);
-      if (!row[j] || k + 8 > f.K) {   // behind the matrix: as pack leaves it
-        const int n = row[j] ? max(0, f.K - k) : 0;
-        const uint32_t keep_low = n >= 4 ? ~0u : (1u << (8 * n)) - 1;
-        const uint32_t keep_high = n >= 8 ? ~0u : n <= 4 ? 0u : (1u << (8 * (n - 4))) - 1;
-        low[j] = (low[j] & keep_low) | (0x08080808u & ~keep_low);
-        high[j] = (high[j] & keep_high) | (0x08080808u & ~keep_high);
+        for (int q = 0; q < 2; ++q) {
+          if (kPasses == 2 && q != pass) continue;
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            uint32_t b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float x = w4_quotient(w[j][q][e + i], divisor, inverse) + kRound;
+              b[i] = __float_as_uint(ZEROS ? fminf(x, most) : x);
+            }
+            // the low bytes are -15..15: their low nibbles plus the zero point, modulo 16
+            const uint32_t v = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+            codes[j][q][e / 4] = ZEROS ? ((v & 0x0f0f0f0fu) + add) & 0x0f0f0f0fu : (v & 0x0f0f0f0fu) ^ 0x08080808u;
+          }
+        }
+      } else {
+        if (ZEROS) zeros[j] = (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, divisor)), 0.0f), 15.0f);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          if (kPasses == 2 && q != pass) continue;
+          codes[j][q][0] = codes[j][q][1] = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float c = fminf(fmaxf(rintf(__fdiv_rn(w[j][q][e], divisor)) + zeros[j], 0.0f), 15.0f);
+            codes[j][q][e / 4] |= (uint32_t)(int)c << (8 * (e % 4));
+          }
+        }
       }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (kPasses == 2 && q != pass) continue;
+        const int n = row[j] ? f.K - k0 - 32 * q : 0;
+        if (n < 8) {   // behind the matrix: as pack leaves it
+          const uint32_t keep0 = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+          const uint32_t keep1 = n <= 4 ? 0u : (1u << (8 * (n - 4))) - 1;
+          codes[j][q][0] = (codes[j][q][0] & keep0) | (0x08080808u & ~keep0);
+          codes[j][q][1] = (codes[j][q][1] & keep1) | (0x08080808u & ~keep1);
+        }
+      }
+      if (!row[j] || k0 - u.col % GROUP + (kPasses == 2 ? 32 * pass : 0) >= f.K) zeros[j] = 8;
     }
-    *reinterpret_cast<uint2*>(chunk + u.offset) = make_uint2(w4_word(low[0], low[1]), w4_word(high[0], high[1]));
-    if (u.col % GROUP == 0) w4_store_scales<T>(f, chunk, u, scale_bits, zeros);
+    const int col = u.col + (kPasses == 2 ? 32 * pass : 0);
+    if (col % GROUP == 0) w4_store_scales<T>(f, chunk, u.pair, col, scale_bits, zeros);
   }
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) words[2 * q + e] = w4_word(codes[0][q][e], codes[1][q][e]);
+  *reinterpret_cast<uint4*>(chunk + w4_unit_offset(u)) = make_uint4(words[0], words[1], words[2], words[3]);
+}
+
+__device__ __forceinline__ uint32_t w4_round2(float a, float b, __nv_bfloat16) { return ptx::pack_bf16x2(a, b); }
+__device__ __forceinline__ uint32_t w4_round2(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // The matrix back from its layout, 8 consecutive columns of a row as one 16-byte store (two for fp32).
+// code - zero times scale is exact in fp32 (5 bits times at most 11), so it is rounded once.
 template <typename T, typename O>
 __global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f, const uint8_t* data, O* out,
                                                                        long long ld, int vec) {
-  const int strip = blockIdx.x / f.blocks, block = blockIdx.x % f.blocks;
-  const uint8_t* chunk = data + (size_t)blockIdx.x * f.chunk_bytes;
+  const int strip = blockIdx.y, block = blockIdx.x;
+  const uint8_t* chunk = data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
+  const W4Unit u = w4_unit();
+  const int n0 = w4_row(f, strip, u.pair, 0), n1 = w4_row(f, strip, u.pair, 1);
+  const uint4 code = __ldg(reinterpret_cast<const uint4*>(chunk + w4_unit_offset(u)));
+  const uint32_t words[4] = {code.x, code.y, code.z, code.w};
 #pragma unroll
-  for (int c = 0; c < kW4Units / kW4PackThreads; ++c) {
-    const W4Unit u = w4_unit(c * kW4PackThreads + threadIdx.x);
-    const long long k = (long long)block * kW4Block + u.col;
-    if (k >= f.K) continue;
-    const uint2 code = __ldg(reinterpret_cast<const uint2*>(chunk + u.offset));
-    const uint8_t* sp = chunk + w4_scale_offset(u.pair, u.col / f.group);
-    const float2 scale = W4Traits<T>::to_float2(__ldg(reinterpret_cast<const uint32_t*>(sp)));
-    float2 off = make_float2(-8.0f, -8.0f);
+  for (int q = 0; q < 2; ++q) {
+    const int col = u.col + 32 * q, k = block * kW4Block + col;
+    if (k >= f.K) break;
+    const uint8_t* sp = chunk + w4_scale_offset(u.pair, col / f.group);
+    float2 scale = W4Traits<T>::to_float2(__ldg(reinterpret_cast<const uint32_t*>(sp)));
+    uint32_t off0 = W4Traits<T>::kMinusEight, off1 = off0;
     if (f.zeros) {
-      off = W4Traits<T>::to_float2(__ldg(reinterpret_cast<const uint32_t*>(sp + kW4Block / f.group * 128)));
-      off = make_float2(off.x / W4Traits<T>::kUnit, off.y / W4Traits<T>::kUnit);
+      const uint32_t both = __ldg(reinterpret_cast<const uint32_t*>(sp + kW4Block / f.group * 128));
+      off0 = __byte_perm(both, 0, 0x1010);
+      off1 = __byte_perm(both, 0, 0x3232);
+    }
+    float v[2][8];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      uint32_t a[4];   // row of the pair: i % 2; columns 2 (i / 2) and the next
+      w4_decode<T>(words[2 * q + s], off0, off1, a);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 two = W4Traits<T>::to_float2(W4Traits<T>::fma2(a[i], W4Traits<T>::kBack, 0x80008000u));
+        const float by = i & 1 ? scale.y : scale.x;
+        v[i & 1][4 * s + 2 * (i >> 1)] = two.x * by;
+        v[i & 1][4 * s + 2 * (i >> 1) + 1] = two.y * by;
+      }
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int n = w4_row(f, strip, u.pair, j);
+      const int n = j ? n1 : n0;
       if (n < 0) continue;
-      alignas(16) O v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        // columns 0, 1, 2, 3 are bits 0, 16, 8, 24
-        const uint32_t q = ((e & 4 ? code.y : code.x) >> (4 * j + 16 * (e & 1) + 4 * (e & 2))) & 15;
-        v[e] = (O)(((float)q + (j ? off.y : off.x)) * (j ? scale.y : scale.x));   // to the nearest, ties to even
-      }
       O* dst = out + (long long)n * ld + k;
       if (vec && k + 8 <= f.K) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(O) / 2; ++i)
-          reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(v)[i];
+        if constexpr (sizeof(O) == 4) {
+          reinterpret_cast<float4*>(dst)[0] = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
+          reinterpret_cast<float4*>(dst)[1] = make_float4(v[j][4], v[j][5], v[j][6], v[j][7]);
+        } else {
+          *reinterpret_cast<uint4*>(dst) =
+              make_uint4(w4_round2(v[j][0], v[j][1], O()), w4_round2(v[j][2], v[j][3], O()),
+                         w4_round2(v[j][4], v[j][5], O()), w4_round2(v[j][6], v[j][7], O()));
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (k + e < f.K) dst[e] = v[e];
+          if (k + e < f.K) dst[e] = (O)v[j][e];
       }
     }
   }
@@ -623,8 +718,8 @@ static int w4_check(const mk_w4* w, const char* what, bool need_data) {
                        w->N / w->head_dim);
   }
   const W4Form f = w4_form(*w);
-  if ((long long)f.strips * f.blocks > 0x7fffffffLL)
-    return set_error(MK_ERR_INVALID, "%s: %d x %d is too large", what, w->N, w->K);
+  if (f.strips > 65535)
+    return set_error(MK_ERR_INVALID, "%s: N=%d is above %d", what, w->N, 65535 * kW4Strip);
   if (need_data && (!w->data || (reinterpret_cast<uintptr_t>(w->data) & 15) != 0))
     return set_error(MK_ERR_INVALID, "%s: packed weights must be a 16-byte aligned device buffer", what);
   return MK_OK;
@@ -762,7 +857,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
 }
 
 template <typename T, typename S>
-static int w4_quantize_group(const W4PackParams& p, unsigned grid, cudaStream_t s) {
+static int w4_quantize_group(const W4PackParams& p, dim3 grid, cudaStream_t s) {
   const bool z = p.form.zeros;
   auto kern = p.form.group == 32   ? (z ? w4_quantize_kernel<T, S, 32, true> : w4_quantize_kernel<T, S, 32, false>)
               : p.form.group == 64 ? (z ? w4_quantize_kernel<T, S, 64, true> : w4_quantize_kernel<T, S, 64, false>)
@@ -773,7 +868,7 @@ static int w4_quantize_group(const W4PackParams& p, unsigned grid, cudaStream_t 
 }
 
 template <typename T>
-static int w4_quantize_launch(const W4PackParams& p, int src_dtype, unsigned grid, cudaStream_t s) {
+static int w4_quantize_launch(const W4PackParams& p, int src_dtype, dim3 grid, cudaStream_t s) {
   if (src_dtype == MK_BF16) return w4_quantize_group<T, __nv_bfloat16>(p, grid, s);
   if (src_dtype == MK_FP16) return w4_quantize_group<T, __half>(p, grid, s);
   return w4_quantize_group<T, float>(p, grid, s);
@@ -781,7 +876,7 @@ static int w4_quantize_launch(const W4PackParams& p, int src_dtype, unsigned gri
 
 template <typename T>
 static int w4_dequantize_launch(const W4Form& f, const uint8_t* data, void* out, long long ld, int dtype, int vec,
-                                unsigned grid, cudaStream_t s) {
+                                dim3 grid, cudaStream_t s) {
   if (dtype == MK_BF16)
     w4_dequantize_kernel<T><<<grid, kW4PackThreads, 0, s>>>(f, data, static_cast<__nv_bfloat16*>(out), ld, vec);
   else if (dtype == MK_FP16)
@@ -824,7 +919,7 @@ int mk_w4_pack(const mk_w4* w, const uint8_t* codes, const void* scales, const u
   p.codes = codes;
   p.scales = static_cast<const uint16_t*>(scales);
   p.zero_points = zero_points;
-  const unsigned grid = (unsigned)(p.form.strips * p.form.blocks);
+  const dim3 grid(p.form.blocks, p.form.strips, 1);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (w->dtype == MK_BF16) w4_pack_kernel<__nv_bfloat16><<<grid, kW4PackThreads, 0, s>>>(p);
   else w4_pack_kernel<__half><<<grid, kW4PackThreads, 0, s>>>(p);
@@ -851,7 +946,7 @@ int mk_w4_quantize(const mk_w4* w, const void* src, long long ld, int src_dtype,
   p.src = src;
   p.ld = ld;
   p.vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && ld * size % 16 == 0;
-  const unsigned grid = (unsigned)(p.form.strips * p.form.blocks);
+  const dim3 grid(p.form.blocks, p.form.strips, 1);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return w->dtype == MK_BF16 ? w4_quantize_launch<__nv_bfloat16>(p, src_dtype, grid, s)
                              : w4_quantize_launch<__half>(p, src_dtype, grid, s);
@@ -871,7 +966,7 @@ int mk_w4_dequantize(const mk_w4* w, void* out, long long ld, int out_dtype, voi
   if (rc != MK_OK) return rc;
   const W4Form f = w4_form(*w);
   const int vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ld * size % 16 == 0;
-  const unsigned grid = (unsigned)(f.strips * f.blocks);
+  const dim3 grid(f.blocks, f.strips, 1);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uint8_t* data = static_cast<const uint8_t*>(w->data);
   return w->dtype == MK_BF16 ? w4_dequantize_launch<__nv_bfloat16>(f, data, out, ld, out_dtype, vec, grid, s)

@@ -76,11 +76,22 @@ template <> struct W4Traits<__nv_bfloat16> {
   static constexpr uint32_t kHigh = 0x7d007d00u;      // 2^123: in bits 4..7, where it is 16 times as much
   static constexpr uint32_t kMinusEight = 0xbe00be00u;   // -8 kUnit
   static constexpr float kUnit = 0x1p-6f;
+  static constexpr uint32_t kBack = 0x42804280u;      // 1 / kUnit, twice
   static __device__ __forceinline__ float to_float(uint32_t bits) { return __uint_as_float(bits << 16); }
   static __device__ __forceinline__ float2 to_float2(uint32_t two) {
     return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
   }
   static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
   static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
     asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
@@ -92,6 +103,7 @@ template <> struct W4Traits<__half> {
   static constexpr uint32_t kHigh = 0x68006800u;      // 2^11
   static constexpr uint32_t kMinusEight = 0xa400a400u;
   static constexpr float kUnit = 0x1p-9f;
+  static constexpr uint32_t kBack = 0x60006000u;
   static __device__ __forceinline__ float to_float(uint32_t bits) {
     return __half2float(__ushort_as_half((unsigned short)bits));
   }
@@ -99,6 +111,16 @@ template <> struct W4Traits<__half> {
     return __half22float2(*reinterpret_cast<const __half2*>(&two));
   }
   static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
   static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
