@@ -21,7 +21,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libmkernel_b200.so"
 DIAG_LIB = PKG / "libmkernel_b200_diag.so"
-SOURCES = ["ops.cu", "w4.cu", "rotary.cu", "transport.cpp"]
+SOURCES = ["ops.cu", "w4.cu", "w4_tile.cu", "rotary.cu", "transport.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

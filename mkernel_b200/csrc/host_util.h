@@ -15,6 +15,9 @@ int device_sm_count(int* out);
 // The "pdl" option: launch with programmatic stream serialization.
 bool option_pdl();
 
+// The "wait_limit_ms" option in nanoseconds.
+unsigned long long option_wait_limit_ns();
+
 // Looks up a driver API symbol through the runtime.  Returns MK_OK or MK_ERR_CUDA.
 int driver_entry(const char* symbol, void** fn);
 

@@ -176,6 +176,11 @@ bool option_pdl() {
   return g_opt.pdl != 0;
 }
 
+unsigned long long option_wait_limit_ns() {
+  std::lock_guard<std::mutex> g(g_opt_mu);
+  return (unsigned long long)g_opt.wait_limit_ms * 1000000ull;
+}
+
 static int make_plan(const Options& o, int op, int rank, int world, int M, int N, int K,
                      int b_layout, int num_sms, Plan* out, int epilogue = EPI_NONE) {
   if (op < OP_GEMM || op > OP_AR) return set_error(MK_ERR_INVALID, "unknown op %d", op);

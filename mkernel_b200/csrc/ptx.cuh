@@ -242,6 +242,11 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t cluster_addr) {
                : "memory");
   return v;
 }
+__device__ __forceinline__ float ld_cluster_f1(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
 // Arrive on an mbarrier that may live in the peer CTA (cluster address).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
@@ -344,6 +349,76 @@ __device__ __forceinline__ void umma_kblock(uint32_t d_tmem, uint32_t a_lo, uint
           "r"(accumulate), "r"(commit_a), "r"(commit_b), "r"(do_commit ? 1u : 0u)
         : "memory");
   }
+}
+// MMAs of 16-bit operands whose A operand lies in tensor memory, N = 2 or 4 of them along K (8 columns of A,
+// 32 bytes of B each), by the elected lane of a converged warp.  `accumulate` = 0 makes the first one
+// overwrite the accumulator.
+template <int N>
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t desc_hi,
+                                        uint32_t idesc, uint32_t accumulate) {
+  static_assert(N == 2 || N == 4, "");
+  asm volatile(
+      "{\n\t.reg .pred pe, pa, pm;\n\t.reg .b64 db;\n\t.reg .b32 ra, rb;\n\t"
+      "elect.sync _|pe, 0xffffffff;\n\t"
+      "setp.ne.and.b32 pm, %6, 0, pe;\n\t"
+      "setp.ne.b32 pa, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, pa;\n\t"
+      "setp.eq.b32 pa, 0, 0;\n\t"
+      "add.u32 ra, %1, 8;\n\t"
+      "add.u32 rb, %2, 2;\n\t"
+      "mov.b64 db, {rb, %3};\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %4, pa;\n\t"
+      "add.u32 ra, ra, 8;\n\t"
+      "add.u32 rb, rb, 2;\n\t"
+      "mov.b64 db, {rb, %3};\n\t"
+      "@pm tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %4, pa;\n\t"
+      "add.u32 ra, ra, 8;\n\t"
+      "add.u32 rb, rb, 2;\n\t"
+      "mov.b64 db, {rb, %3};\n\t"
+      "@pm tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %4, pa;\n\t"
+      "}\n"
+      ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate), "r"(N == 4 ? 1u : 0u)
+      : "memory");
+}
+// 16 lanes x N / 4 times 8 columns: thread (g, t) = (lane / 4, lane % 4) holds, of each eight columns,
+// columns 2 t and 2 t + 1 of lanes g and g + 8.
+__device__ __forceinline__ void tmem_st_16x256(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_16x256(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// 32 lanes x 16 consecutive fp32 columns.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// The mbarrier counts one arrival when all copies that this thread has started so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+// 8-byte asynchronous copy of which `bytes` (0..8) are read and the rest zeroed.
+__device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // The commit that publishes a finished accumulator, by the elected lane of a converged warp.
 template <int CG>

@@ -8,8 +8,7 @@
 #include "../../include/mkernel_b200.h"
 #include "host_util.h"
 #include "ptx.cuh"
-#include "rotary.cuh"
-#include "w4_layout.cuh"
+#include "w4_product.cuh"
 
 namespace mkb {
 
@@ -373,47 +372,6 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f,
 // ------------------------------------------------------------------------------------------
 // the product for few tokens
 // ------------------------------------------------------------------------------------------
-enum W4Epilogue : int { W4_EPI_NONE = 0, W4_EPI_SWIGLU = 1, W4_EPI_ROTARY = 2 };
-
-struct W4Params {
-  W4Form form;
-  const uint8_t* data;
-  const void* A;
-  long long lda;
-  void* C;
-  long long ldc;
-  int M;
-  int vec;        // rows of A are 16-byte aligned and K is a multiple of 8
-  int stage_bytes;
-  int split;      // CTAs of a cluster, which share a strip along K
-  int epilogue;
-  RotaryArgs rotary;
-};
-
-// C's entries of one pair of rows and one token.
-template <typename T>
-__device__ __forceinline__ void w4_epilogue(const W4Params& p, int strip, int pair, int token, float2 v) {
-  const W4Form& f = p.form;
-  const int n0 = w4_row(f, strip, pair, 0);
-  if (n0 < 0) return;
-  T* row = static_cast<T*>(p.C) + (long long)token * p.ldc;
-  if (p.epilogue == W4_EPI_SWIGLU) {
-    // silu in fp32; for a gate below -88 the exponential is inf and the quotient -0, as it should be
-    row[n0] = W4Traits<T>::from_float(v.x / (1.0f + __expf(-v.x)) * v.y);
-    return;
-  }
-  const int n1 = w4_row(f, strip, pair, 1);
-  if (p.epilogue == W4_EPI_ROTARY) {
-    const int half = f.head_dim / 2;
-    const int index = strip * (kW4Strip / 2) + pair, head = index / half, i = index % half;
-    if (head < f.rotated_heads && i < f.rotary_dim / 2)
-      v = rotary_turn(v.x, v.y, rotary_cos_sin(rotary_position(p.rotary, token),
-                                               __ldg(p.rotary.inv_freq + i), p.rotary.scale));
-  }
-  row[n0] = W4Traits<T>::from_float(v.x);
-  if (n1 >= 0) row[n1] = W4Traits<T>::from_float(v.y);
-}
-
 // d = a b (fresh) or d += a b.
 template <typename T>
 __device__ __forceinline__ void w4_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool fresh) {
@@ -725,34 +683,6 @@ static int w4_check(const mk_w4* w, const char* what, bool need_data) {
   return MK_OK;
 }
 
-template <typename K>
-static int w4_launch(K kern, dim3 grid, int threads, int smem, int cluster, cudaStream_t stream,
-                     const W4Params& p) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (cluster > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = cluster;
-    attr[n].val.clusterDim.y = 1;
-    attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (option_pdl()) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  MKB_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
-  return MK_OK;
-}
-
 // How the few-token product is cut.  All choices follow from how many CTAs there are to fill the SMs;
 // figures are microseconds, 1 token, bf16, group 128, medians of graph replays.
 struct W4StreamPlan { int nt, tiles, warps, split, stage_bytes; long long token_tiles, ctas; };
@@ -845,6 +775,10 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.vec = (reinterpret_cast<uintptr_t>(A) & 15) == 0 && lda % 8 == 0 && w->K % 8 == 0;
   p.epilogue = epilogue;
   p.rotary = rotary;
+  p.wait_limit_ns = option_wait_limit_ns();
+  // Up to 16 tokens the stream kernel is bound by memory as it should be; every 16 more cost it another
+  // pass over the weights.
+  if (M > 16) return w4_tile_launch(p, w->dtype, sms, static_cast<cudaStream_t>(stream));
   const W4StreamPlan pl = w4_stream_plan(p.form, M, sms);
   p.stage_bytes = pl.stage_bytes;
   p.split = pl.split;

@@ -1,0 +1,87 @@
+// What the two kernels of the 4-bit products share: their parameters, what is done with a finished
+// pair of sums, and the launch.
+#pragma once
+#include <cuda_runtime.h>
+
+#include "host_util.h"
+#include "ptx.cuh"
+#include "rotary.cuh"
+#include "w4_layout.cuh"
+
+namespace mkb {
+
+enum W4Epilogue : int { W4_EPI_NONE = 0, W4_EPI_SWIGLU = 1, W4_EPI_ROTARY = 2 };
+
+struct W4Params {
+  W4Form form;
+  const uint8_t* data;
+  const void* A;
+  long long lda;
+  void* C;
+  long long ldc;
+  int M;
+  int vec;             // rows of A start on whole copies (16 bytes in the stream kernel, 8 in the tile kernel)
+  int stage_bytes;     // of a shared-memory ring
+  int split;           // CTAs of a cluster, which share a strip along K
+  int token_tiles;     // tile kernel
+  uint64_t wait_limit_ns;
+  int epilogue;
+  RotaryArgs rotary;
+};
+
+// C's entries of one pair of rows and one token.
+template <typename T>
+__device__ __forceinline__ void w4_epilogue(const W4Params& p, int strip, int pair, int token, float2 v) {
+  const W4Form& f = p.form;
+  const int n0 = w4_row(f, strip, pair, 0);
+  if (n0 < 0) return;
+  T* row = static_cast<T*>(p.C) + (long long)token * p.ldc;
+  if (p.epilogue == W4_EPI_SWIGLU) {
+    // silu in fp32; for a gate below -88 the exponential is inf and the quotient -0, as it should be
+    row[n0] = W4Traits<T>::from_float(v.x / (1.0f + __expf(-v.x)) * v.y);
+    return;
+  }
+  const int n1 = w4_row(f, strip, pair, 1);
+  if (p.epilogue == W4_EPI_ROTARY) {
+    const int half = f.head_dim / 2;
+    const int index = strip * (kW4Strip / 2) + pair, head = index / half, i = index % half;
+    if (head < f.rotated_heads && i < f.rotary_dim / 2)
+      v = rotary_turn(v.x, v.y, rotary_cos_sin(rotary_position(p.rotary, token),
+                                               __ldg(p.rotary.inv_freq + i), p.rotary.scale));
+  }
+  row[n0] = W4Traits<T>::from_float(v.x);
+  if (n1 >= 0) row[n1] = W4Traits<T>::from_float(v.y);
+}
+
+template <typename K>
+inline int w4_launch(K kern, dim3 grid, int threads, int smem, int cluster, cudaStream_t stream,
+                     const W4Params& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (option_pdl()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  MKB_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+  return MK_OK;
+}
+
+// The product for more tokens than the stream kernel takes (w4_tile.cu).
+int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream);
+
+}  // namespace mkb

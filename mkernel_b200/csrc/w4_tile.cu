@@ -1,0 +1,420 @@
+// The product with 4-bit weights for more than a few tokens, on the 5th-generation tensor cores.
+//
+// A CTA computes 128 rows of the matrix (two strips) for up to 2 TH tokens, D = W A^T with the weights as
+// the 128-row operand.  That operand never exists in shared memory: the lanes that decode the codes
+// write whole numbers (code - zero, times a power of two) into tensor memory, in the 16x256b form
+// whose lanes are the layout's lanes, and the MMA takes its A operand from there.  So shared memory
+// carries only the packed codes and the tokens.
+//
+// One step is one group of columns.  The sums of a group are exact products added in fp32 by the tensor
+// core; the threads that own the accumulator's lanes (a lane is a row of the matrix) read it, multiply
+// it by the row's scale in fp32 and add it to registers, while the tensor core works on the next
+// group in the other accumulator.  No weight is rounded to be multiplied.
+//
+// Warps 0..7 decode and rescale (quadrant warp % 4 of the lanes; of a step, warp / 4 decides which half of
+// the decoding and which half of the tokens), warp 8 issues the MMAs, warps 9..11 copy a ring of
+// stages (a block of 128 columns: codes of two strips, tokens in the 128-byte swizzle).
+//
+// What bounds it, at 128 tokens to a CTA: 128 x 128 x 128 MMAs take about 510 cycles of the tensor pipe,
+// decoding and rescaling 8 warps about 350 of each scheduler's, and the copies 40 KB of L2 traffic,
+// about 640 cycles at 64 bytes a cycle.
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "../../include/mkernel_b200.h"
+#include "w4_product.cuh"
+
+namespace mkb {
+
+constexpr int kTileRows = 2 * kW4Strip;
+constexpr int kTileCompute = 8;                    // warps
+constexpr int kTileLoaders = 3;
+constexpr int kTileThreads = (kTileCompute + 1 + kTileLoaders) * 32;
+constexpr int kTileMaxStages = 8;
+constexpr int kTileControl = 1024;                 // bytes before the ring
+constexpr int kTilePitch = kTileRows + 4;          // floats of a token's sums
+
+__host__ __device__ constexpr int w4_tile_stages(int tokens) { return tokens <= 64 ? 8 : tokens <= 96 ? 6 : 5; }
+
+struct TileWait {
+  volatile uint32_t* abort;   // shared: some wait of this CTA has run out
+  uint64_t limit_ns;
+};
+
+// False when the wait has run out, here or elsewhere in the CTA.
+__device__ __noinline__ bool w4_slow_wait(const TileWait& c, uint32_t bar, uint32_t parity) {
+  uint64_t t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    if ((it & 127u) == 0u) {
+      if (*c.abort != 0u) return false;
+      uint64_t now;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > c.limit_ns) {
+        *c.abort = 1u;
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool w4_wait(const TileWait& c, uint32_t bar, uint32_t parity) {
+  return ptx::mbar_try_wait(bar, parity) || w4_slow_wait(c, bar, parity);
+}
+// The same for a whole warp that goes on, or gives up, together.
+__device__ __forceinline__ bool w4_wait_warp(const TileWait& c, uint32_t bar, uint32_t parity) {
+  return __all_sync(~0u, w4_wait(c, bar, parity));
+}
+
+template <typename T, int TH, int GROUP>
+__global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_constant__ W4Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  constexpr int kTokens = 2 * TH;
+  constexpr int kStages = w4_tile_stages(kTokens);
+  constexpr int kSteps = kW4Block / GROUP;          // of a block
+  constexpr uint32_t kCols = 2 * kTokens + GROUP <= 256 ? 256 : 512;
+  constexpr int kXHalf = kTokens * 128;             // bytes of 64 columns of the tokens
+
+  const W4Form& f = p.form;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* const base_ptr = smem_raw + (base - raw);
+  // control words: full[8] empty[8] a_full[2] d_full[2] | tensor memory address, abort flag
+  auto full = [&](int s) { return base + 8u * s; };
+  auto empty = [&](int s) { return base + 64u + 8u * s; };
+  auto a_full = [&](int i) { return base + 128u + 8u * i; };
+  auto d_full = [&](int i) { return base + 144u + 8u * i; };
+  volatile uint32_t* const s_tmem = reinterpret_cast<volatile uint32_t*>(base_ptr + 192);
+  volatile uint32_t* const s_abort = s_tmem + 1;
+  const uint32_t ring = base + kTileControl;
+  uint8_t* const ring_ptr = base_ptr + kTileControl;
+
+  const int rank = blockIdx.x % p.split;
+  const int unit = blockIdx.x / p.split;
+  const int row_tile = unit / p.token_tiles, token0 = unit % p.token_tiles * kTokens;
+  const int blocks = (f.blocks - rank + p.split - 1) / p.split;     // rank, rank + split, ...
+  const int strip0 = 2 * row_tile;
+  const bool two = strip0 + 1 < f.strips;
+
+  if (warp == kTileCompute) {
+    ptx::tmem_alloc(base + 192, kCols);
+    ptx::tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(full(s), kTileLoaders * 32);
+      ptx::mbar_init(empty(s), kTileCompute + 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(a_full(i), kTileCompute);
+      ptx::mbar_init(d_full(i), 1);
+    }
+    *s_abort = 0u;
+    ptx::fence_mbar_init();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  const uint32_t tmem_a = tmem + 2 * kTokens;
+  const TileWait wc{s_abort, p.wait_limit_ns};
+
+  const size_t strip_bytes = (size_t)f.blocks * f.chunk_bytes;
+  const uint8_t* const data = p.data + (size_t)strip0 * strip_bytes + (size_t)rank * f.chunk_bytes;
+  if (warp > kTileCompute) {
+    // what is read first may be asked into L2 before the kernel ahead has finished
+    const int lt = threadIdx.x - (kTileCompute + 1) * 32;
+    for (int b = 0; b < kStages && b < blocks; ++b)
+      for (int o = lt * 128; o < f.chunk_bytes; o += kTileLoaders * 32 * 128)
+        for (int i = 0; i <= (int)two; ++i)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(data + i * strip_bytes + (size_t)b * p.split * f.chunk_bytes + o));
+  }
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+
+  float acc[TH];
+  if (warp < kTileCompute) {
+    // ---------------- decode, rescale ----------------
+    const int quad = warp & 3, sub = warp >> 2, g = lane >> 2;
+    const int strip = quad >> 1, tile0 = (quad & 1) * 2;
+    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+    const int x_bytes = kTokens * 256;
+    const int codes_at = x_bytes + strip * f.chunk_bytes;
+    // scale of the accumulator's lane, in 16-bit units behind the codes
+    const int row = (quad & 1) * 32 + lane;
+    const int scale_at = codes_at + kW4CodeBytes + ((row & 7) * 8 + (row >> 4) * 2 + ((row >> 3) & 1)) * 2;
+    const int offset_at = codes_at + kW4CodeBytes + kSteps * 128 + g * 16;
+#pragma unroll
+    for (int i = 0; i < TH; ++i) acc[i] = 0.0f;
+    float scale = 0.0f;
+    bool ok = true;
+    auto rescale = [&](int step, float by) {
+      if (!w4_wait_warp(wc, d_full(step & 1), (step >> 1) & 1)) return false;
+      ptx::tc_fence_after();
+      const uint32_t at = tmem + lane_base + (step & 1) * kTokens + sub * TH;
+      if constexpr (TH % 32 == 0) {
+#pragma unroll
+        for (int c = 0; c < TH; c += 32) {
+          float d[2][16];
+          ptx::tmem_ld_32x16(at + c, d[0]);
+          ptx::tmem_ld_32x16(at + c + 16, d[1]);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[c + i] = fmaf(by, d[i / 16][i % 16], acc[c + i]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < TH; c += 16) {
+          float d[16];
+          ptx::tmem_ld_32x16(at + c, d);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(by, d[i], acc[c + i]);
+        }
+      }
+      return true;
+    };
+    int step = 0;
+    for (int b = 0; ok && b < blocks; ++b) {
+      const int s = b % kStages;
+      if (!w4_wait_warp(wc, full(s), (b / kStages) & 1)) { ok = false; break; }
+      const uint8_t* stage = ring_ptr + s * p.stage_bytes;
+#pragma unroll
+      for (int gi = 0; gi < kSteps; ++gi, ++step) {
+        // The other user of this operand buffer, two steps back, has finished: its sums have been read.
+        const uint32_t a_at = tmem_a + lane_base + (step & 1) * (GROUP / 2);
+        auto offsets = [&](int tile, uint32_t& off0, uint32_t& off1) {
+          off0 = off1 = W4Traits<T>::kMinusEight;
+          if (f.zeros) {
+            const uint32_t both = *reinterpret_cast<const uint32_t*>(stage + offset_at + gi * 128 + tile * 4);
+            off0 = __byte_perm(both, 0, 0x1010);
+            off1 = __byte_perm(both, 0, 0x3232);
+          }
+        };
+        auto decode = [&](uint32_t word, uint32_t off0, uint32_t off1, uint32_t* r) {
+          uint32_t a[4];
+          w4_decode<T>(word, off0, off1, a);
+          r[0] = a[0]; r[1] = a[2]; r[2] = a[1]; r[3] = a[3];
+        };
+        if constexpr (GROUP == 32) {
+          const int tile = tile0 + sub;
+          const uint2 c = *reinterpret_cast<const uint2*>(stage + codes_at + (((gi >> 1) * 4 + tile) * 32 + lane) * 16 + (gi & 1) * 8);
+          uint32_t off0, off1, r[8];
+          offsets(tile, off0, off1);
+          decode(c.x, off0, off1, r);
+          decode(c.y, off0, off1, r + 4);
+          ptx::tmem_st_16x256(a_at + ((uint32_t)(sub * 16) << 16), r);
+        } else {
+          // a half of the block: the step itself, or this warp's part of it
+          const int half = GROUP == 64 ? gi : sub;
+#pragma unroll
+          for (int i = 0; i < (GROUP == 64 ? 1 : 2); ++i) {
+            const int in_quad = GROUP == 64 ? sub : i, tile = tile0 + in_quad;
+            const uint4 c = *reinterpret_cast<const uint4*>(stage + codes_at + ((half * 4 + tile) * 32 + lane) * 16);
+            uint32_t off0, off1, r[16];
+            offsets(tile, off0, off1);
+            decode(c.x, off0, off1, r);
+            decode(c.y, off0, off1, r + 4);
+            decode(c.z, off0, off1, r + 8);
+            decode(c.w, off0, off1, r + 12);
+            ptx::tmem_st_16x256(a_at + ((uint32_t)(in_quad * 16) << 16) + (GROUP == 128 ? half * 32 : 0), r);
+          }
+        }
+        const float next =
+            W4Traits<T>::to_float(*reinterpret_cast<const uint16_t*>(stage + scale_at + gi * 128));
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive(a_full(step & 1));
+          if (gi == kSteps - 1) ptx::mbar_arrive(empty(s));
+        }
+        if (step > 0 && !rescale(step - 1, scale)) { ok = false; break; }
+        scale = next;
+      }
+    }
+    if (ok && step > 0) ok = rescale(step - 1, scale);
+    if (!ok) {
+#pragma unroll
+      for (int i = 0; i < TH; ++i) acc[i] = __int_as_float(0x7fc00000);
+    }
+    ptx::tc_fence_before();
+  } else if (warp == kTileCompute) {
+    // ---------------- MMA issue: the whole warp, one lane elected inside the statement ----------------
+    constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t idesc = (1u << 4) | (kType << 7) | (kType << 10) | ((kTokens >> 3) << 17) | ((128u >> 4) << 24);
+    const uint32_t desc_hi = static_cast<uint32_t>(ptx::make_smem_desc_sw128(0, 16, 1024) >> 32);
+    int step = 0;
+    bool ok = true;
+    for (int b = 0; ok && b < blocks; ++b) {
+      const int s = b % kStages;
+      ok = w4_wait_warp(wc, full(s), (b / kStages) & 1);
+      if (!ok) break;
+      ptx::fence_proxy_async();   // the tokens were written by ordinary (asynchronous) copies
+      const uint32_t x = ring + s * p.stage_bytes;
+      const uint32_t b_lo = static_cast<uint32_t>(ptx::make_smem_desc_sw128(x, 16, 1024));
+#pragma unroll
+      for (int gi = 0; gi < kSteps; ++gi, ++step) {
+        ok = w4_wait_warp(wc, a_full(step & 1), (step >> 1) & 1);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + (step & 1) * kTokens, a = tmem_a + (step & 1) * (GROUP / 2);
+        if constexpr (GROUP == 128) {
+          ptx::umma_ts<4>(d, a, b_lo, desc_hi, idesc, 0);
+          ptx::umma_ts<4>(d, a + 32, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
+        } else if constexpr (GROUP == 64) {
+          ptx::umma_ts<4>(d, a, b_lo + gi * (kXHalf >> 4), desc_hi, idesc, 0);
+        } else {
+          ptx::umma_ts<2>(d, a, b_lo + (gi >> 1) * (kXHalf >> 4) + (gi & 1) * 4, desc_hi, idesc, 0);
+        }
+        ptx::umma_commit_elect<1>(d_full(step & 1), 0);
+      }
+      if (ok) ptx::umma_commit_elect<1>(empty(s), 0);
+    }
+  } else {
+    // ---------------- copies ----------------
+    const int lt = threadIdx.x - (kTileCompute + 1) * 32, lw = lt >> 5;
+    constexpr int kLoadThreads = kTileLoaders * 32;
+    const int pieces = f.chunk_bytes / 16 * (two ? 2 : 1);
+    // Lane = 4 columns of a token (columns 32 q + 8 t + 4 s of the block), which lie at position
+    // 32 q + 16 s + 4 t: the order in which the decoded codes reach tensor memory.
+    const int q = lane >> 3, t = lane >> 1 & 3, sx = lane & 1;
+    const uint32_t x_unit = (q & 1) * 4 + sx * 2 + (t >> 1), x_low = (q >> 1) * kXHalf + (t & 1) * 8;
+    for (int b = 0; b < blocks; ++b) {
+      const int s = b % kStages;
+      if (b >= kStages && !w4_wait(wc, empty(s), (b / kStages - 1) & 1)) break;
+      const uint32_t stage = ring + s * p.stage_bytes;
+      const uint8_t* chunk = data + (size_t)b * p.split * f.chunk_bytes;
+      const uint32_t codes = stage + kTokens * 256;
+      for (int i = lt; i < pieces; i += kLoadThreads) {
+        const int o = i * 16;
+        const uint8_t* from = o < f.chunk_bytes ? chunk + o : chunk + strip_bytes + (o - f.chunk_bytes);
+        ptx::cp_async_16(codes + o, from);
+      }
+      const long long k = (long long)(rank + b * p.split) * kW4Block + lane * 4;
+      const long long left = (f.K - k) * 2;
+      const int bytes = left >= 8 ? 8 : left > 0 ? (int)left : 0;
+      const uint16_t* A = static_cast<const uint16_t*>(p.A);
+      if (p.vec) {
+#pragma unroll 4
+        for (int m = lw; m < kTokens; m += kTileLoaders) {
+          const int n = token0 + m < p.M ? bytes : 0;
+          ptx::cp_async_8(stage + x_low + m * 128 + ((x_unit ^ (m & 7)) << 4),
+                          n > 0 ? A + (long long)(token0 + m) * p.lda + k : A, n);
+        }
+        ptx::cp_async_arrive(full(s));
+      } else {
+        // rows that no 8-byte access can start on
+#pragma unroll 4
+        for (int m = lw; m < kTokens; m += kTileLoaders) {
+          uint32_t e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            e[i] = token0 + m < p.M && 2 * i < bytes ? __ldg(A + (long long)(token0 + m) * p.lda + k + i) : 0u;
+          *reinterpret_cast<uint2*>(ring_ptr + s * p.stage_bytes + x_low + m * 128 + ((x_unit ^ (m & 7)) << 4)) =
+              make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
+        }
+        ptx::cp_async_commit();
+        ptx::cp_async_wait<0>();
+        ptx::mbar_arrive(full(s));
+      }
+    }
+    ptx::cp_async_commit();
+    ptx::cp_async_wait<0>();
+  }
+  // a wait that ran out leaves MMAs that may still read the ring
+  if (*s_abort != 0u) __nanosleep(50000);
+  __syncthreads();
+  if (warp == kTileCompute) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, kCols);
+  }
+
+  // The sums, token by token, over the ring; the CTAs of a cluster then share the tokens.
+  float* const red = reinterpret_cast<float*>(ring_ptr);
+  if (warp < kTileCompute) {
+    const int quad = warp & 3, sub = warp >> 2;
+#pragma unroll
+    for (int i = 0; i < TH; ++i) red[(sub * TH + i) * kTilePitch + quad * 32 + lane] = acc[i] * (1.0f / W4Traits<T>::kUnit);
+  }
+  if (p.split > 1) ptx::cluster_sync_all();
+  else __syncthreads();
+  const int tokens = min(kTokens, p.M - token0);
+  for (int e = rank * kTileThreads + threadIdx.x; e < tokens * kW4Strip; e += p.split * kTileThreads) {
+    const int token = e / kW4Strip, pair = e % kW4Strip;     // 32 pairs of each strip
+    if (pair >= kW4Strip / 2 && !two) continue;
+    const int r = (pair >> 5) * kW4Strip + (pair >> 3 & 3) * 16 + (pair & 7);
+    const uint32_t at = ring + (token * kTilePitch + r) * 4;
+    float2 v = make_float2(0.0f, 0.0f);
+    for (int c = 0; c < p.split; ++c) {
+      const uint32_t a = p.split > 1 ? ptx::map_to_cta(at, c) : at;
+      v.x += ptx::ld_cluster_f1(a);
+      v.y += ptx::ld_cluster_f1(a + 32);
+    }
+    w4_epilogue<T>(p, strip0 + (pair >> 5), pair & 31, token0 + token, v);
+  }
+  if (p.split > 1) ptx::cluster_sync_all();   // nobody leaves while its shared memory is read
+}
+
+template <typename T, int TH, int GROUP>
+static int w4_tile_kernel_launch(const W4Params& p, unsigned grid, cudaStream_t stream) {
+  constexpr int kStages = w4_tile_stages(2 * TH);
+  const int ring = kStages * p.stage_bytes, sums = 2 * TH * kTilePitch * 4;
+  const int smem = 1024 + kTileControl + (ring > sums ? ring : sums);
+  auto kern = w4_tile_kernel<T, TH, GROUP>;
+  static bool attr_set[64];
+  int dev = 0;
+  MKB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    MKB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  return w4_launch(kern, dim3(grid, 1, 1), kTileThreads, smem, p.split, stream, p);
+}
+
+template <typename T, int TH>
+static int w4_tile_group(const W4Params& p, unsigned grid, cudaStream_t stream) {
+  if (p.form.group == 32) return w4_tile_kernel_launch<T, TH, 32>(p, grid, stream);
+  if (p.form.group == 64) return w4_tile_kernel_launch<T, TH, 64>(p, grid, stream);
+  return w4_tile_kernel_launch<T, TH, 128>(p, grid, stream);
+}
+
+template <typename T>
+static int w4_tile_tokens(const W4Params& p, int tokens, unsigned grid, cudaStream_t stream) {
+  switch (tokens) {
+    case 32: return w4_tile_group<T, 16>(p, grid, stream);
+    case 64: return w4_tile_group<T, 32>(p, grid, stream);
+    case 96: return w4_tile_group<T, 48>(p, grid, stream);
+    default: return w4_tile_group<T, 64>(p, grid, stream);
+  }
+}
+
+int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
+  const W4Form& f = p.form;
+  const long long row_tiles = (f.strips + 1) / 2;
+  // Tokens to a CTA and CTAs to a cluster along K: whichever finishes first by a rough count of cycles,
+  // 330 or 5 a token for a block, 4000 to start and end, 1500 more for a cluster.
+  int tokens = 128;
+  long long best = -1;
+  for (int t = 32; t <= 128; t += 32)
+    for (int split = 1; split <= 8 && split <= f.blocks; split *= 2) {
+      const long long units = row_tiles * ((p.M + t - 1) / t) * split;
+      const long long waves = (units + sms - 1) / sms;
+      if (split > 1 && waves > 1) continue;
+      const long long cost = waves * ((long long)((f.blocks + split - 1) / split) * (5 * t < 330 ? 330 : 5 * t) + 4000) +
+                             (split > 1 ? 1500 : 0);
+      if (best < 0 || cost < best) { best = cost; tokens = t; p.split = split; }
+    }
+  p.token_tiles = (p.M + tokens - 1) / tokens;
+  p.stage_bytes = (tokens * 256 + 2 * f.chunk_bytes + 1023) / 1024 * 1024;
+  p.vec = (reinterpret_cast<uintptr_t>(p.A) & 7) == 0 && p.lda % 4 == 0;
+  const long long grid = row_tiles * p.token_tiles * p.split;
+  if (grid > 0x7fffffffLL) return set_error(MK_ERR_INVALID, "4-bit product: M=%d, N=%d is too large", p.M, f.N);
+  return dtype == MK_BF16 ? w4_tile_tokens<__nv_bfloat16>(p, tokens, (unsigned)grid, stream)
+                          : w4_tile_tokens<__half>(p, tokens, (unsigned)grid, stream);
+}
+
+}  // namespace mkb
