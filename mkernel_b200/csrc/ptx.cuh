@@ -160,9 +160,16 @@ __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
-// ---------------------------------------------------------------- TMA: untiled bulk store
+// ---------------------------------------------------------------- TMA: untiled bulk copies
+// global (this GPU's memory) -> this CTA's shared memory, completion on an mbarrier of this CTA.
+// Addresses and size are multiples of 16.
+__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
 // shared -> global (the destination may be a mapped peer GPU address); completion is tracked by
-// the issuing thread's bulk async-group.  No load of this kind is used anywhere.
+// the issuing thread's bulk async-group.
 __device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes) {
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
                "r"(src), "r"(bytes)
@@ -242,9 +249,10 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t cluster_addr) {
                : "memory");
   return v;
 }
-__device__ __forceinline__ float ld_cluster_f1(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr) : "memory");
   return v;
 }
 // Arrive on an mbarrier that may live in the peer CTA (cluster address).
@@ -411,14 +419,6 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float (&v)[16]) {
       : "memory");
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-// The mbarrier counts one arrival when all copies that this thread has started so far have landed.
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-// 8-byte asynchronous copy of which `bytes` (0..8) are read and the rest zeroed.
-__device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // The commit that publishes a finished accumulator, by the elected lane of a converged warp.
 template <int CG>

@@ -15,10 +15,11 @@ namespace mkb {
 // ------------------------------------------------------------------------------------------
 // laying the weights out
 // ------------------------------------------------------------------------------------------
-// The unit of all three kernels is a lane's 16 bytes of codes in the layout: of a pair of rows, columns
-// 8 t and 32 + 8 t and the seven behind each, in one half of a block; a chunk has as many units as a
-// CTA has threads.  A unit is read and written with 16-byte accesses, four neighbouring threads
-// covering whole sectors; a group is reduced by shuffles, and nothing passes through shared memory.
+// The unit of all three kernels is 16 consecutive columns of a pair of rows: one word of the layout for
+// each of four lanes.  Four neighbouring threads have the 64 columns of a half, and after exchanging
+// words (w4_transpose) each has the 16 bytes of one lane.  A chunk has as many units as a CTA has
+// threads, a unit is read and written with 16-byte accesses, a group is reduced by shuffles, and
+// nothing passes through shared memory.
 constexpr int kW4PackThreads = 256;
 
 struct W4PackParams {
@@ -34,14 +35,28 @@ struct W4PackParams {
   int vec;   // 16-byte accesses to eight columns are aligned
 };
 
-struct W4Unit { int pair, col; };   // columns col and col + 32 of the block
-__device__ __forceinline__ W4Unit w4_unit() {
-  // threads: t fastest, then the half, then the pair
-  const int i = threadIdx.x;
-  return {i >> 3, (i >> 2 & 1) * 64 + (i & 3) * 8};
-}
+struct W4Unit { int pair, col; };   // columns col .. col + 15 of the block
+__device__ __forceinline__ W4Unit w4_unit() { return {(int)threadIdx.x >> 3, ((int)threadIdx.x & 7) * 16}; }
+// Place of the lane that the unit's thread has after the exchange: t = thread % 4.
 __device__ __forceinline__ int w4_unit_offset(const W4Unit& u) {
-  return (((u.col >> 6) * 4 + (u.pair >> 3)) * 32 + (u.pair & 7) * 4 + (u.col >> 3 & 3)) * 16;
+  return (((u.col >> 6) * 4 + (u.pair >> 3)) * 32 + (u.pair & 7) * 4 + (u.col >> 4 & 3)) * 16;
+}
+
+// Word i of thread j for word j of thread i, among four neighbouring threads.
+__device__ __forceinline__ void w4_transpose(uint32_t (&w)[4]) {
+  const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const uint32_t other = __shfl_xor_sync(~0u, odd ? w[i] : w[i + 1], 1);
+    if (odd) w[i] = other;
+    else w[i + 1] = other;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t other = __shfl_xor_sync(~0u, upper ? w[i] : w[i + 2], 2);
+    if (upper) w[i] = other;
+    else w[i + 2] = other;
+  }
 }
 
 // A word of the layout from four codes each of the pair's rows, a byte each, first column lowest: columns
@@ -79,20 +94,17 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_pack_kernel(W4PackParams p)
   uint8_t* chunk = p.data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
   const long long row_bytes = ((long long)f.K + 1) / 2, groups = ((long long)f.K + f.group - 1) / f.group;
   const W4Unit u = w4_unit();
-  uint32_t words[4];
+  const long long k0 = (long long)block * kW4Block + u.col;
+  uint32_t bytes[2][4];   // row, four columns; a byte each
+  uint16_t scale[2] = {0, 0};
+  int zero[2] = {8, 8};
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int col = u.col + 32 * q;
-    const long long k = (long long)block * kW4Block + col;
-    uint32_t low[2], high[2];
-    uint16_t scale[2];
-    int zero[2];
+  for (int j = 0; j < 2; ++j) {
+    const int n = w4_row(f, strip, u.pair, j);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int n = w4_row(f, strip, u.pair, j);
+    for (int h = 0; h < 2; ++h) {
+      const long long k = k0 + 8 * h;
       uint32_t v = 0x88888888u;   // nibbles of 8 columns
-      scale[j] = 0;
-      zero[j] = 8;
       if (n >= 0 && k < f.K) {
         const uint8_t* c = p.codes + n * row_bytes + k / 2;
         v = 0;
@@ -102,19 +114,21 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_pack_kernel(W4PackParams p)
           const uint32_t mask = (1u << (4 * (int)(f.K - k))) - 1;
           v = (v & mask) | (0x88888888u & ~mask);
         }
-        if (col % f.group == 0) {
-          scale[j] = __ldg(p.scales + n * groups + k / f.group);
-          if (f.zeros) zero[j] = __ldg(p.zero_points + n * groups + k / f.group) & 15;
-        }
       }
-      low[j] = __byte_perm(v & 0x0f0f, (v >> 4) & 0x0f0f, 0x5140);
-      high[j] = __byte_perm((v >> 16) & 0x0f0f, (v >> 20) & 0x0f0f, 0x5140);
+      bytes[j][2 * h] = __byte_perm(v & 0x0f0f, (v >> 4) & 0x0f0f, 0x5140);
+      bytes[j][2 * h + 1] = __byte_perm((v >> 16) & 0x0f0f, (v >> 20) & 0x0f0f, 0x5140);
     }
-    words[2 * q] = w4_word(low[0], low[1]);
-    words[2 * q + 1] = w4_word(high[0], high[1]);
-    if (col % f.group == 0) w4_store_scales<T>(f, chunk, u.pair, col, scale, zero);
+    if (u.col % f.group == 0 && n >= 0 && k0 < f.K) {
+      scale[j] = __ldg(p.scales + n * groups + k0 / f.group);
+      if (f.zeros) zero[j] = __ldg(p.zero_points + n * groups + k0 / f.group) & 15;
+    }
   }
+  uint32_t words[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) words[i] = w4_word(bytes[0][i], bytes[1][i]);
+  w4_transpose(words);
   *reinterpret_cast<uint4*>(chunk + w4_unit_offset(u)) = make_uint4(words[0], words[1], words[2], words[3]);
+  if (u.col % f.group == 0) w4_store_scales<T>(f, chunk, u.pair, u.col, scale, zero);
 }
 
 // Eight columns of a source row, and the smallest and largest of them and 0 (symmetric: the largest
@@ -200,7 +214,7 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParam
   uint8_t* chunk = p.data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
   const W4Unit u = w4_unit();
   const int k0 = block * kW4Block + u.col;
-  W4Source<S> w[2][2];
+  W4Source<S> w[2][2];   // row, eight columns
   bool row[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -208,106 +222,85 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParam
     row[j] = n >= 0;
     const S* src = static_cast<const S*>(p.src) + (long long)(n < 0 ? 0 : n) * p.ld + k0;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int k = k0 + 32 * q;
-      if (row[j] && p.vec && k + 8 <= f.K) w[j][q].load(src + 32 * q);
-      else w[j][q].load(src + 32 * q, row[j] ? f.K - k : 0);
+    for (int h = 0; h < 2; ++h) {
+      const int k = k0 + 8 * h;
+      if (row[j] && p.vec && k + 8 <= f.K) w[j][h].load(src + 8 * h);
+      else w[j][h].load(src + 8 * h, row[j] ? f.K - k : 0);
     }
   }
-  uint32_t words[4];
   uint16_t scale_bits[2];
   int zeros[2];
-  constexpr int kPasses = GROUP == 32 ? 2 : 1;   // groups that a unit meets
-  uint32_t codes[2][2][2];                       // row, q, first or second four columns; a byte each
+  uint32_t codes[2][4];   // row, four columns; a byte each
 #pragma unroll
-  for (int pass = 0; pass < kPasses; ++pass) {
+  for (int j = 0; j < 2; ++j) {
+    float lo = 0.0f, hi = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float lo = 0.0f, hi = 0.0f;
+    for (int h = 0; h < 2; ++h) w[j][h].template range<ZEROS>(lo, hi);
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-        if (kPasses == 1 || q == pass) w[j][q].template range<ZEROS>(lo, hi);
-#pragma unroll
-      for (int d = 1; d < (GROUP == 128 ? 8 : 4); d *= 2) {
-        if (ZEROS) lo = w4_min_nan(lo, __shfl_xor_sync(~0u, lo, d));
-        hi = w4_max_nan(hi, __shfl_xor_sync(~0u, hi, d));
-      }
-      const float span = ZEROS ? hi - lo : hi;
-      // Markstein's division by a constant is the division, but for subnormal results
-      const float n = ZEROS ? 15.0f : 7.0f;
-      float range = span < 0x1p-100f ? __fdiv_rn(span, n) : w4_quotient(span, n, 1.0f / n);
-      if (!(span <= 3.402823466e38f)) range = __int_as_float(0x7fc00000);   // an infinity or NaN in the group
-      const T scale_t = W4Traits<T>::from_float(range);
-      scale_bits[j] = *reinterpret_cast<const uint16_t*>(&scale_t);
-      const float scale = W4Traits<T>::to_float(scale_bits[j]);
-      const float divisor = scale == 0.0f ? 1.0f : scale;
-      const bool plain = sizeof(S) == 2 && scale >= (sizeof(T) == 2 && W4Traits<T>::kUnit == 0x1p-9f ? 0x1p-14f : 0x1p-90f) &&
-                         scale <= 0x1p90f;
+    for (int d = 1; d < GROUP / 16; d *= 2) {
+      if (ZEROS) lo = w4_min_nan(lo, __shfl_xor_sync(~0u, lo, d));
+      hi = w4_max_nan(hi, __shfl_xor_sync(~0u, hi, d));
+    }
+    const float span = ZEROS ? hi - lo : hi;
+    // Markstein's division by a constant is the division, but for subnormal results
+    const float n = ZEROS ? 15.0f : 7.0f;
+    float range = span < 0x1p-100f ? __fdiv_rn(span, n) : w4_quotient(span, n, 1.0f / n);
+    if (!(span <= 3.402823466e38f)) range = __int_as_float(0x7fc00000);   // an infinity or NaN in the group
+    const T scale_t = W4Traits<T>::from_float(range);
+    scale_bits[j] = *reinterpret_cast<const uint16_t*>(&scale_t);
+    const float scale = W4Traits<T>::to_float(scale_bits[j]);
+    const float divisor = scale == 0.0f ? 1.0f : scale;
+    const float least = std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-90f;
+    zeros[j] = 8;
+    if (sizeof(S) == 2 && scale >= least && scale <= 0x1p90f) {
       // quotient + 1.5 2^23 is the rounded quotient in the low bits (ties to even)
       constexpr float kRound = 12582912.0f;
-      zeros[j] = 8;
-      if (plain) {
-        float inverse;
-        asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(divisor));
-        if (ZEROS) zeros[j] = (int)(__float_as_uint(w4_quotient(-lo, divisor, inverse) + kRound) & 15);
-        const float most = kRound + (15 - zeros[j]);
-        const uint32_t add = zeros[j] * 0x01010101u;
+      float inverse;
+      asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(divisor));
+      if (ZEROS) zeros[j] = (int)(__float_as_uint(w4_quotient(-lo, divisor, inverse) + kRound) & 15);
+      const float most = kRound + (15 - zeros[j]);
+      const uint32_t add = zeros[j] * 0x01010101u;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          if (kPasses == 2 && q != pass) continue;
+      for (int e = 0; e < 4; ++e) {
+        uint32_t b[4];
 #pragma unroll
-          for (int e = 0; e < 8; e += 4) {
-            uint32_t b[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float x = w4_quotient(w[j][q][e + i], divisor, inverse) + kRound;
-              b[i] = __float_as_uint(ZEROS ? fminf(x, most) : x);
-            }
-            // the low bytes are -15..15: their low nibbles plus the zero point, modulo 16
-            const uint32_t v = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-            codes[j][q][e / 4] = ZEROS ? ((v & 0x0f0f0f0fu) + add) & 0x0f0f0f0fu : (v & 0x0f0f0f0fu) ^ 0x08080808u;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const float x = w4_quotient(w[j][e / 2][e % 2 * 4 + i], divisor, inverse) + kRound;
+          b[i] = __float_as_uint(ZEROS ? fminf(x, most) : x);
         }
-      } else {
-        if (ZEROS) zeros[j] = (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, divisor)), 0.0f), 15.0f);
+        // the low bytes are -15..15: their low nibbles plus the zero point, modulo 16
+        const uint32_t v = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+        codes[j][e] = ZEROS ? ((v & 0x0f0f0f0fu) + add) & 0x0f0f0f0fu : (v & 0x0f0f0f0fu) ^ 0x08080808u;
+      }
+    } else {
+      if (ZEROS) zeros[j] = (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, divisor)), 0.0f), 15.0f);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          if (kPasses == 2 && q != pass) continue;
-          codes[j][q][0] = codes[j][q][1] = 0;
+      for (int e = 0; e < 4; ++e) {
+        codes[j][e] = 0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float c = fminf(fmaxf(rintf(__fdiv_rn(w[j][q][e], divisor)) + zeros[j], 0.0f), 15.0f);
-            codes[j][q][e / 4] |= (uint32_t)(int)c << (8 * (e % 4));
-          }
+        for (int i = 0; i < 4; ++i) {
+          const float c = fminf(fmaxf(rintf(__fdiv_rn(w[j][e / 2][e % 2 * 4 + i], divisor)) + zeros[j], 0.0f), 15.0f);
+          codes[j][e] |= (uint32_t)(int)c << (8 * i);
         }
       }
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        if (kPasses == 2 && q != pass) continue;
-        const int n = row[j] ? f.K - k0 - 32 * q : 0;
-        if (n < 8) {   // behind the matrix: as pack leaves it
-          const uint32_t keep0 = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
-          const uint32_t keep1 = n <= 4 ? 0u : (1u << (8 * (n - 4))) - 1;
-          codes[j][q][0] = (codes[j][q][0] & keep0) | (0x08080808u & ~keep0);
-          codes[j][q][1] = (codes[j][q][1] & keep1) | (0x08080808u & ~keep1);
-        }
-      }
-      if (!row[j] || k0 - u.col % GROUP + (kPasses == 2 ? 32 * pass : 0) >= f.K) zeros[j] = 8;
     }
-    const int col = u.col + (kPasses == 2 ? 32 * pass : 0);
-    if (col % GROUP == 0) w4_store_scales<T>(f, chunk, u.pair, col, scale_bits, zeros);
+    const int have = row[j] ? f.K - k0 : 0;
+    if (have < 16) {   // behind the matrix: as pack leaves it
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int m = have - 4 * e;
+        const uint32_t keep = m >= 4 ? ~0u : m <= 0 ? 0u : (1u << (8 * m)) - 1;
+        codes[j][e] = (codes[j][e] & keep) | (0x08080808u & ~keep);
+      }
+    }
+    if (!row[j] || k0 - u.col % GROUP >= f.K) zeros[j] = 8;
   }
+  if (u.col % GROUP == 0) w4_store_scales<T>(f, chunk, u.pair, u.col, scale_bits, zeros);
+  uint32_t words[4];
 #pragma unroll
-  for (int q = 0; q < 2; ++q)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) words[2 * q + e] = w4_word(codes[0][q][e], codes[1][q][e]);
+  for (int i = 0; i < 4; ++i) words[i] = w4_word(codes[0][i], codes[1][i]);
+  w4_transpose(words);
   *reinterpret_cast<uint4*>(chunk + w4_unit_offset(u)) = make_uint4(words[0], words[1], words[2], words[3]);
-}
-
-__device__ __forceinline__ uint32_t w4_round2(float a, float b, __nv_bfloat16) { return ptx::pack_bf16x2(a, b); }
-__device__ __forceinline__ uint32_t w4_round2(float a, float b, __half) {
-  const __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // The matrix back from its layout, 8 consecutive columns of a row as one 16-byte store (two for fp32).
@@ -318,52 +311,53 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f,
   const int strip = blockIdx.y, block = blockIdx.x;
   const uint8_t* chunk = data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
   const W4Unit u = w4_unit();
-  const int n0 = w4_row(f, strip, u.pair, 0), n1 = w4_row(f, strip, u.pair, 1);
   const uint4 code = __ldg(reinterpret_cast<const uint4*>(chunk + w4_unit_offset(u)));
-  const uint32_t words[4] = {code.x, code.y, code.z, code.w};
+  uint32_t words[4] = {code.x, code.y, code.z, code.w};
+  w4_transpose(words);
+  const int k0 = block * kW4Block + u.col;
+  if (k0 >= f.K) return;
+  const uint8_t* sp = chunk + w4_scale_offset(u.pair, u.col / f.group);
+  const float2 scale = W4Traits<T>::to_float2(__ldg(reinterpret_cast<const uint32_t*>(sp)));
+  uint32_t off0 = W4Traits<T>::kMinusEight, off1 = off0;
+  if (f.zeros) {
+    const uint32_t both = __ldg(reinterpret_cast<const uint32_t*>(sp + kW4Block / f.group * 128));
+    off0 = __byte_perm(both, 0, 0x1010);
+    off1 = __byte_perm(both, 0, 0x3232);
+  }
+  float v[2][16];
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int col = u.col + 32 * q, k = block * kW4Block + col;
-    if (k >= f.K) break;
-    const uint8_t* sp = chunk + w4_scale_offset(u.pair, col / f.group);
-    float2 scale = W4Traits<T>::to_float2(__ldg(reinterpret_cast<const uint32_t*>(sp)));
-    uint32_t off0 = W4Traits<T>::kMinusEight, off1 = off0;
-    if (f.zeros) {
-      const uint32_t both = __ldg(reinterpret_cast<const uint32_t*>(sp + kW4Block / f.group * 128));
-      off0 = __byte_perm(both, 0, 0x1010);
-      off1 = __byte_perm(both, 0, 0x3232);
+  for (int e = 0; e < 4; ++e) {
+    uint32_t a[4];   // row of the pair: i % 2; columns 2 (i / 2) and the next
+    w4_decode<T>(words[e], off0, off1, a);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 two = W4Traits<T>::to_float2(W4Traits<T>::fma2(a[i], W4Traits<T>::kBack, 0x80008000u));
+      const float by = i & 1 ? scale.y : scale.x;
+      v[i & 1][4 * e + 2 * (i >> 1)] = two.x * by;
+      v[i & 1][4 * e + 2 * (i >> 1) + 1] = two.y * by;
     }
-    float v[2][8];
+  }
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      uint32_t a[4];   // row of the pair: i % 2; columns 2 (i / 2) and the next
-      w4_decode<T>(words[2 * q + s], off0, off1, a);
+  for (int j = 0; j < 2; ++j) {
+    const int n = w4_row(f, strip, u.pair, j);
+    if (n < 0) continue;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 two = W4Traits<T>::to_float2(W4Traits<T>::fma2(a[i], W4Traits<T>::kBack, 0x80008000u));
-        const float by = i & 1 ? scale.y : scale.x;
-        v[i & 1][4 * s + 2 * (i >> 1)] = two.x * by;
-        v[i & 1][4 * s + 2 * (i >> 1) + 1] = two.y * by;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int n = j ? n1 : n0;
-      if (n < 0) continue;
+    for (int h = 0; h < 16; h += 8) {
+      const int k = k0 + h;
       O* dst = out + (long long)n * ld + k;
       if (vec && k + 8 <= f.K) {
         if constexpr (sizeof(O) == 4) {
-          reinterpret_cast<float4*>(dst)[0] = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
-          reinterpret_cast<float4*>(dst)[1] = make_float4(v[j][4], v[j][5], v[j][6], v[j][7]);
+          reinterpret_cast<float4*>(dst)[0] = make_float4(v[j][h], v[j][h + 1], v[j][h + 2], v[j][h + 3]);
+          reinterpret_cast<float4*>(dst)[1] = make_float4(v[j][h + 4], v[j][h + 5], v[j][h + 6], v[j][h + 7]);
         } else {
           *reinterpret_cast<uint4*>(dst) =
-              make_uint4(w4_round2(v[j][0], v[j][1], O()), w4_round2(v[j][2], v[j][3], O()),
-                         w4_round2(v[j][4], v[j][5], O()), w4_round2(v[j][6], v[j][7], O()));
+              make_uint4(w4_round2(v[j][h], v[j][h + 1], O()), w4_round2(v[j][h + 2], v[j][h + 3], O()),
+                         w4_round2(v[j][h + 4], v[j][h + 5], O()), w4_round2(v[j][h + 6], v[j][h + 7], O()));
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (k + e < f.K) dst[e] = (O)v[j][e];
+          if (k + e < f.K) dst[e] = (O)v[j][h + e];
       }
     }
   }
@@ -412,19 +406,16 @@ __host__ __device__ constexpr int w4_stage_bytes(int chunk, int tiles, int token
   return chunk - (4 - tiles) * 1024 + tokens * 256;
 }
 
-// Place of 8 activations (quarter hq of the block, lane t) of a token behind the chunk.  Odd tokens swap
-// quarters, so that the two tokens that eight lanes read at once lie in different banks.
-__device__ __forceinline__ int w4_x_slot(int token, int hq, int t) {
-  return token * 256 + ((hq ^ (token & 1)) * 64) + t * 16;
-}
+// Place of 16 columns (slot of the block) of a token behind the chunk.  Neighbouring tokens swap slots, so
+// that the four tokens whose columns a half-warp reads at once lie in different banks.
+__device__ __forceinline__ int w4_x_slot(int token, int slot) { return token * 256 + (slot ^ (token & 3)) * 32; }
 
 // Starts the copies of TILES tiles of a chunk (`chunk`: the address of the first, plus this lane's
 // 16 bytes; `tail`: that of the chunk's scales) and of the activations of block `block` into a stage.
-// x: column 8 t of this lane's token (g of each eight).
+// x: column 8 t of this lane's token (g of each eight); x_to: where its columns 8 t and 32 + 8 t go.
 template <int NT, int TILES, int TAIL>
 __device__ __forceinline__ void w4_fill(const W4Params& p, const uint8_t* chunk, const uint8_t* tail,
-                                        int block, int token0, const uint16_t* const (&x)[NT], const bool (&have)[NT], int x_even,
-                                        int x_odd, uint32_t stage, uint8_t* stage_ptr, int lane) {
+                                        int block, int token0, const uint16_t* const (&x)[NT], const bool (&have)[NT], const int (&x_to)[2], uint32_t stage, uint8_t* stage_ptr, int lane) {
   const uint32_t dst = stage + lane * 16;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
@@ -441,7 +432,7 @@ __device__ __forceinline__ void w4_fill(const W4Params& p, const uint8_t* chunk,
         const uint16_t* from = x[n] + k0;
 #pragma unroll
         for (int hq = 0; hq < 4; ++hq)
-          ptx::cp_async_16(stage + ((hq & 1) ? x_odd : x_even) + n * 2048 + hq * 64, from + hq * 32);
+          ptx::cp_async_16(stage + x_to[hq & 1] + n * 2048 + (hq >> 1) * 128, from + hq * 32);
       }
   } else {
     // The last block of K, and rows that no 16-byte access can start on: lanes take consecutive
@@ -462,7 +453,7 @@ __device__ __forceinline__ void w4_fill(const W4Params& p, const uint8_t* chunk,
         if (m0 + m < tokens)
 #pragma unroll
           for (int hq = 0; hq < 4; ++hq)
-            *reinterpret_cast<uint16_t*>(stage_ptr + TILES * 1024 + TAIL + w4_x_slot(m0 + m, hq, 0) + lane * 2) = v[m][hq];
+            *reinterpret_cast<uint16_t*>(stage_ptr + TILES * 1024 + TAIL + w4_x_slot(m0 + m, hq * 2 + (lane >> 4)) + (lane & 15) * 2) = v[m][hq];
     }
   }
 }
@@ -524,11 +515,12 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
     x[n] = static_cast<const uint16_t*>(p.A) + (long long)(token0 + (have[n] ? n * 8 + g : 0)) * p.lda + 8 * t;
   }
   const int gx = min(g, last);
-  const int x_even = kCodes + kTail + w4_x_slot(gx, 0, t), x_odd = kCodes + kTail + w4_x_slot(gx, 1, t) - 64;
+  const int x_to[2] = {kCodes + kTail + w4_x_slot(gx, t >> 1) + (t & 1) * 16,
+                       kCodes + kTail + w4_x_slot(gx, 2 + (t >> 1)) + (t & 1) * 16};
 #pragma unroll
   for (int i = 0; i < kW4Stages; ++i) {
     if (first + i * step < f.blocks)
-      w4_fill<NT, TILES, kTail>(p, chunk, tail, first + i * step, token0, x, have, x_even, x_odd,
+      w4_fill<NT, TILES, kTail>(p, chunk, tail, first + i * step, token0, x, have, x_to,
                                 ring + i * p.stage_bytes, ring_ptr + i * p.stage_bytes, lane);
     chunk += chunk_step;
     tail += chunk_step;
@@ -550,7 +542,9 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
     const uint8_t* base = ring_ptr + at;
     const uint8_t* base_codes = base + lane * 16;
     const uint8_t* base_scales = base + kCodes + g * 16 + tile0 * 4;
-    const uint8_t* base_x[2] = {base + x_even, base + x_odd};
+    const uint8_t* base_x[4];   // this lane's 4 columns of the first four 16
+#pragma unroll
+    for (int i = 0; i < 4; ++i) base_x[i] = base + kCodes + kTail + w4_x_slot(gx, i) + t * 8;
     float part[TILES][NT][4];
     uint32_t off[TILES][2];
 #pragma unroll
@@ -561,11 +555,13 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
 #pragma unroll
       for (int q = 0; q < 2; ++q) {          // 32 columns at a time
         const int hq = h * 2 + q, gi = hq * 32 / GROUP;
-        uint4 xv[NT];
+        uint2 xv[2][NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          // past the last token of a second eight: any finite address of the stage (see above)
-          xv[n] = *reinterpret_cast<const uint4*>(base_x[q] + (n * 8 + g <= last ? n * 2048 : 0) + hq * 64);
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            // past the last token of a second eight: another token of the stage (see above)
+            xv[s][n] = *reinterpret_cast<const uint2*>(base_x[q * 2 + s] + (n * 8 + g <= last ? n * 2048 : 0) + h * 128);
         const bool fresh = hq * 32 % GROUP == 0;
         if (ZEROS && fresh) {
           uint32_t both[TILES];
@@ -587,7 +583,7 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
                          ZEROS ? off[r][1] : W4Traits<T>::kMinusEight, a);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-              w4_mma<T>(part[r][n], a, s ? xv[n].z : xv[n].x, s ? xv[n].w : xv[n].y, fresh && s == 0);
+              w4_mma<T>(part[r][n], a, xv[s][n].x, xv[s][n].y, fresh && s == 0);
           }
         }
         if ((hq + 1) * 32 % GROUP == 0) {
@@ -610,7 +606,7 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
     __syncwarp();
     const int ahead = block + kW4Stages * step;
     if (ahead < f.blocks)
-      w4_fill<NT, TILES, kTail>(p, chunk, tail, ahead, token0, x, have, x_even, x_odd, ring + at, ring_ptr + at,
+      w4_fill<NT, TILES, kTail>(p, chunk, tail, ahead, token0, x, have, x_to, ring + at, ring_ptr + at,
                                 lane);
     chunk += chunk_step;
     tail += chunk_step;
@@ -775,6 +771,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.vec = (reinterpret_cast<uintptr_t>(A) & 15) == 0 && lda % 8 == 0 && w->K % 8 == 0;
   p.epilogue = epilogue;
   p.rotary = rotary;
+  p.wide = (reinterpret_cast<uintptr_t>(C) & 7) == 0 && ldc % 4 == 0 && (form != MK_W4_GATE_UP || w->N / 2 % 4 == 0);
   p.wait_limit_ns = option_wait_limit_ns();
   // Up to 16 tokens the stream kernel is bound by memory as it should be; every 16 more cost it another
   // pass over the weights.

@@ -7,13 +7,14 @@
 // Codes are stored in the order in which the lanes of a warp need them as the A operand of the
 // 16x8x16 matrix instruction: [half of 64 columns][tile of 16 rows][lane][16 bytes], so a lane
 // loads its operands of four such instructions with one 16-byte access.  Lane (g = lane / 4,
-// t = lane % 4) holds rows g and g + 8 of the tile; word j of its 16 bytes holds columns
-// 32 (j / 2) + 8 t + 4 (j % 2) + {0, 1, 2, 3} of the half.  Which column of the instruction a
-// matrix column lands on does not matter to a dot product as long as both operands agree; this
-// order gives a lane 8 consecutive columns (16 bytes of the other operand) and keeps every
-// instruction inside a group of 32.  Nibble i + 4 e of the word is operand register i (row
-// g + 8 (i % 2), column pair i / 2), element e: (word >> 4 i) & 0x000f000f is the register's two
-// codes in the low bits of its two halves.
+// t = lane % 4) holds rows g and g + 8 of the tile; word v of its 16 bytes holds columns
+// 16 v + 4 t + {0, 1, 2, 3} of the half.  Which column of the instruction a matrix column lands on
+// does not matter to a dot product as long as both operands agree; with this order a lane needs four
+// consecutive columns (8 bytes) of the other operand for an instruction, an instruction stays inside 16
+// consecutive columns, and the same words written to tensor memory as 16x256b (whose lanes are the
+// same lanes) put the columns there in their natural order.  Nibble i + 4 e of the word is operand
+// register i (row g + 8 (i % 2), column pair i / 2), element e: (word >> 4 i) & 0x000f000f is the
+// register's two codes in the low bits of its two halves.
 // Scales and offsets of a group: [g][tile][2], 16 bits each, so that a lane takes the eight that
 // belong to its rows with one 16-byte access.  An offset is -zero point * kUnit (see W4Traits).
 //

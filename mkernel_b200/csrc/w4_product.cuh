@@ -20,14 +20,24 @@ struct W4Params {
   void* C;
   long long ldc;
   int M;
-  int vec;             // rows of A start on whole copies (16 bytes in the stream kernel, 8 in the tile kernel)
+  int vec;             // rows of A start on 16 bytes (and, in the stream kernel, K is a multiple of 8)
   int stage_bytes;     // of a shared-memory ring
   int split;           // CTAs of a cluster, which share a strip along K
   int token_tiles;     // tile kernel
+  int wide;            // C takes 8-byte stores at every fourth column
   uint64_t wait_limit_ns;
   int epilogue;
   RotaryArgs rotary;
 };
+
+// silu(gate) up in fp32; for a gate below -88 the exponential is inf and the quotient -0, as it should be.
+__device__ __forceinline__ float w4_silu_mul(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
+
+__device__ __forceinline__ uint32_t w4_round2(float a, float b, __nv_bfloat16) { return ptx::pack_bf16x2(a, b); }
+__device__ __forceinline__ uint32_t w4_round2(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 
 // C's entries of one pair of rows and one token.
 template <typename T>
@@ -37,8 +47,7 @@ __device__ __forceinline__ void w4_epilogue(const W4Params& p, int strip, int pa
   if (n0 < 0) return;
   T* row = static_cast<T*>(p.C) + (long long)token * p.ldc;
   if (p.epilogue == W4_EPI_SWIGLU) {
-    // silu in fp32; for a gate below -88 the exponential is inf and the quotient -0, as it should be
-    row[n0] = W4Traits<T>::from_float(v.x / (1.0f + __expf(-v.x)) * v.y);
+    row[n0] = W4Traits<T>::from_float(w4_silu_mul(v.x, v.y));
     return;
   }
   const int n1 = w4_row(f, strip, pair, 1);
@@ -53,9 +62,32 @@ __device__ __forceinline__ void w4_epilogue(const W4Params& p, int strip, int pa
   if (n1 >= 0) row[n1] = W4Traits<T>::from_float(v.y);
 }
 
-template <typename K>
-inline int w4_launch(K kern, dim3 grid, int threads, int smem, int cluster, cudaStream_t stream,
-                     const W4Params& p) {
+// The same of four consecutive pairs (pair a multiple of 4).  first[i], second[i]: their two sums.
+template <typename T>
+__device__ __forceinline__ void w4_epilogue4(const W4Params& p, int strip, int pair, int token, float4 first, float4 second) {
+  const W4Form& f = p.form;
+  const float a[4] = {first.x, first.y, first.z, first.w}, b[4] = {second.x, second.y, second.z, second.w};
+  // the two forms whose outputs of four pairs are neighbours
+  if (p.wide && p.epilogue != W4_EPI_ROTARY) {
+    T* row = static_cast<T*>(p.C) + (long long)token * p.ldc;
+    float v[4];
+    const bool glu = p.epilogue == W4_EPI_SWIGLU;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = glu ? w4_silu_mul(a[i], b[i]) : a[i];
+    const int n0 = w4_row(f, strip, pair, 0), n1 = glu ? -1 : w4_row(f, strip, pair, 1);
+    const int n_out = glu ? f.N / 2 : f.N;
+    if (n0 >= 0 && n0 + 4 <= n_out && (n1 >= 0 || glu) && n1 + 4 <= n_out) {
+      *reinterpret_cast<uint2*>(row + n0) = make_uint2(w4_round2(v[0], v[1], T()), w4_round2(v[2], v[3], T()));
+      if (!glu) *reinterpret_cast<uint2*>(row + n1) = make_uint2(w4_round2(b[0], b[1], T()), w4_round2(b[2], b[3], T()));
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w4_epilogue<T>(p, strip, pair + i, token, make_float2(a[i], b[i]));
+}
+
+template <typename K, typename... Args>
+inline int w4_launch(K kern, dim3 grid, int threads, int smem, int cluster, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads, 1, 1);
@@ -77,7 +109,7 @@ inline int w4_launch(K kern, dim3 grid, int threads, int smem, int cluster, cuda
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  MKB_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+  MKB_CUDA(cudaLaunchKernelEx(&cfg, kern, args...));
   return MK_OK;
 }
 

@@ -12,12 +12,14 @@
 // group in the other accumulator.  No weight is rounded to be multiplied.
 //
 // Warps 0..7 decode and rescale (quadrant warp % 4 of the lanes; of a step, warp / 4 decides which half of
-// the decoding and which half of the tokens), warp 8 issues the MMAs, warps 9..11 copy a ring of
-// stages (a block of 128 columns: codes of two strips, tokens in the 128-byte swizzle).
+// the decoding and which half of the tokens), warp 8 issues the MMAs, a thread of warp 9 (warps
+// 9..11 where rows are not aligned) copies a ring of stages (a block of 128 columns: codes of two strips,
+// tokens in the 128-byte swizzle).
 //
 // What bounds it, at 128 tokens to a CTA: 128 x 128 x 128 MMAs take about 510 cycles of the tensor pipe,
 // decoding and rescaling 8 warps about 350 of each scheduler's, and the copies 40 KB of L2 traffic,
 // about 640 cycles at 64 bytes a cycle.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -31,7 +33,6 @@ constexpr int kTileRows = 2 * kW4Strip;
 constexpr int kTileCompute = 8;                    // warps
 constexpr int kTileLoaders = 3;
 constexpr int kTileThreads = (kTileCompute + 1 + kTileLoaders) * 32;
-constexpr int kTileMaxStages = 8;
 constexpr int kTileControl = 1024;                 // bytes before the ring
 constexpr int kTilePitch = kTileRows + 4;          // floats of a token's sums
 
@@ -69,7 +70,8 @@ __device__ __forceinline__ bool w4_wait_warp(const TileWait& c, uint32_t bar, ui
 }
 
 template <typename T, int TH, int GROUP>
-__global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_constant__ W4Params p) {
+__global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_constant__ W4Params p,
+                                                                 const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int kTokens = 2 * TH;
   constexpr int kStages = w4_tile_stages(kTokens);
@@ -105,7 +107,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(full(s), kTileLoaders * 32);
+      ptx::mbar_init(full(s), p.vec ? 1 : kTileLoaders * 32);
       ptx::mbar_init(empty(s), kTileCompute + 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -253,7 +255,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
       const int s = b % kStages;
       ok = w4_wait_warp(wc, full(s), (b / kStages) & 1);
       if (!ok) break;
-      ptx::fence_proxy_async();   // the tokens were written by ordinary (asynchronous) copies
+      if (!p.vec) ptx::fence_proxy_async();   // the tokens were written by ordinary stores
       const uint32_t x = ring + s * p.stage_bytes;
       const uint32_t b_lo = static_cast<uint32_t>(ptx::make_smem_desc_sw128(x, 16, 1024));
 #pragma unroll
@@ -274,53 +276,53 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
       }
       if (ok) ptx::umma_commit_elect<1>(empty(s), 0);
     }
+  } else if (p.vec) {
+    // ---------------- copies: one thread, tokens by tensor copies, codes by plain ones ----------------
+    if (warp == kTileCompute + 1 && lane == 0) {
+      const uint32_t tx = kTokens * 256 + f.chunk_bytes * (two ? 2 : 1);
+      for (int b = 0; b < blocks; ++b) {
+        const int s = b % kStages;
+        if (b >= kStages && !w4_wait(wc, empty(s), (b / kStages - 1) & 1)) break;
+        const uint32_t stage = ring + s * p.stage_bytes;
+        const uint8_t* chunk = data + (size_t)b * p.split * f.chunk_bytes;
+        const int k = (rank + b * p.split) * kW4Block;
+        ptx::mbar_expect_tx(full(s), tx);
+        ptx::bulk_g2s(stage + kTokens * 256, chunk, f.chunk_bytes, full(s));
+        if (two) ptx::bulk_g2s(stage + kTokens * 256 + f.chunk_bytes, chunk + strip_bytes, f.chunk_bytes, full(s));
+        ptx::tma_load_2d(stage, &map, full(s), k, token0);
+        ptx::tma_load_2d(stage + kXHalf, &map, full(s), k + 64, token0);
+      }
+    }
   } else {
-    // ---------------- copies ----------------
+    // ---------------- copies where rows of tokens start on no 16 bytes ----------------
     const int lt = threadIdx.x - (kTileCompute + 1) * 32, lw = lt >> 5;
-    constexpr int kLoadThreads = kTileLoaders * 32;
     const int pieces = f.chunk_bytes / 16 * (two ? 2 : 1);
-    // Lane = 4 columns of a token (columns 32 q + 8 t + 4 s of the block), which lie at position
-    // 32 q + 16 s + 4 t: the order in which the decoded codes reach tensor memory.
-    const int q = lane >> 3, t = lane >> 1 & 3, sx = lane & 1;
-    const uint32_t x_unit = (q & 1) * 4 + sx * 2 + (t >> 1), x_low = (q >> 1) * kXHalf + (t & 1) * 8;
+    // lane = 4 columns of a token, in the 128-byte swizzle
+    const uint32_t unit = lane >> 1 & 7, low = (lane >> 4) * kXHalf + (lane & 1) * 8;
+    const uint16_t* A = static_cast<const uint16_t*>(p.A);
     for (int b = 0; b < blocks; ++b) {
       const int s = b % kStages;
       if (b >= kStages && !w4_wait(wc, empty(s), (b / kStages - 1) & 1)) break;
       const uint32_t stage = ring + s * p.stage_bytes;
       const uint8_t* chunk = data + (size_t)b * p.split * f.chunk_bytes;
-      const uint32_t codes = stage + kTokens * 256;
-      for (int i = lt; i < pieces; i += kLoadThreads) {
+      for (int i = lt; i < pieces; i += kTileLoaders * 32) {
         const int o = i * 16;
-        const uint8_t* from = o < f.chunk_bytes ? chunk + o : chunk + strip_bytes + (o - f.chunk_bytes);
-        ptx::cp_async_16(codes + o, from);
+        ptx::cp_async_16(stage + kTokens * 256 + o,
+                         o < f.chunk_bytes ? chunk + o : chunk + strip_bytes + (o - f.chunk_bytes));
       }
       const long long k = (long long)(rank + b * p.split) * kW4Block + lane * 4;
-      const long long left = (f.K - k) * 2;
-      const int bytes = left >= 8 ? 8 : left > 0 ? (int)left : 0;
-      const uint16_t* A = static_cast<const uint16_t*>(p.A);
-      if (p.vec) {
 #pragma unroll 4
-        for (int m = lw; m < kTokens; m += kTileLoaders) {
-          const int n = token0 + m < p.M ? bytes : 0;
-          ptx::cp_async_8(stage + x_low + m * 128 + ((x_unit ^ (m & 7)) << 4),
-                          n > 0 ? A + (long long)(token0 + m) * p.lda + k : A, n);
-        }
-        ptx::cp_async_arrive(full(s));
-      } else {
-        // rows that no 8-byte access can start on
-#pragma unroll 4
-        for (int m = lw; m < kTokens; m += kTileLoaders) {
-          uint32_t e[4];
+      for (int m = lw; m < kTokens; m += kTileLoaders) {
+        uint32_t e[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            e[i] = token0 + m < p.M && 2 * i < bytes ? __ldg(A + (long long)(token0 + m) * p.lda + k + i) : 0u;
-          *reinterpret_cast<uint2*>(ring_ptr + s * p.stage_bytes + x_low + m * 128 + ((x_unit ^ (m & 7)) << 4)) =
-              make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
-        }
-        ptx::cp_async_commit();
-        ptx::cp_async_wait<0>();
-        ptx::mbar_arrive(full(s));
+        for (int i = 0; i < 4; ++i)
+          e[i] = token0 + m < p.M && k + i < f.K ? __ldg(A + (long long)(token0 + m) * p.lda + k + i) : 0u;
+        *reinterpret_cast<uint2*>(ring_ptr + s * p.stage_bytes + low + m * 128 + ((unit ^ (m & 7)) << 4)) =
+            make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
       }
+      ptx::cp_async_commit();
+      ptx::cp_async_wait<0>();
+      ptx::mbar_arrive(full(s));
     }
     ptx::cp_async_commit();
     ptx::cp_async_wait<0>();
@@ -342,25 +344,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   }
   if (p.split > 1) ptx::cluster_sync_all();
   else __syncthreads();
-  const int tokens = min(kTokens, p.M - token0);
-  for (int e = rank * kTileThreads + threadIdx.x; e < tokens * kW4Strip; e += p.split * kTileThreads) {
-    const int token = e / kW4Strip, pair = e % kW4Strip;     // 32 pairs of each strip
-    if (pair >= kW4Strip / 2 && !two) continue;
-    const int r = (pair >> 5) * kW4Strip + (pair >> 3 & 3) * 16 + (pair & 7);
+  // Four pairs of a token at a time: rows r .. r + 3 and r + 8 .. r + 11 of a tile.
+  const int items = min(kTokens, p.M - token0) * (two ? 16 : 8);
+  for (int e = rank * kTileThreads + threadIdx.x; e < items; e += p.split * kTileThreads) {
+    const int token = two ? e >> 4 : e >> 3, quad = two ? e & 15 : e & 7;   // 8 quads of each strip
+    const int r = (quad >> 3) * kW4Strip + (quad >> 1 & 3) * 16 + (quad & 1) * 4;
     const uint32_t at = ring + (token * kTilePitch + r) * 4;
-    float2 v = make_float2(0.0f, 0.0f);
+    float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
     for (int c = 0; c < p.split; ++c) {
       const uint32_t a = p.split > 1 ? ptx::map_to_cta(at, c) : at;
-      v.x += ptx::ld_cluster_f1(a);
-      v.y += ptx::ld_cluster_f1(a + 32);
+      const float4 x = ptx::ld_cluster_f4(a), y = ptx::ld_cluster_f4(a + 32);
+      u.x += x.x; u.y += x.y; u.z += x.z; u.w += x.w;
+      v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
     }
-    w4_epilogue<T>(p, strip0 + (pair >> 5), pair & 31, token0 + token, v);
+    w4_epilogue4<T>(p, strip0 + (quad >> 3), (quad & 7) * 4, token0 + token, u, v);
   }
   if (p.split > 1) ptx::cluster_sync_all();   // nobody leaves while its shared memory is read
 }
 
 template <typename T, int TH, int GROUP>
-static int w4_tile_kernel_launch(const W4Params& p, unsigned grid, cudaStream_t stream) {
+static int w4_tile_kernel_launch(const W4Params& p, const CUtensorMap& map, unsigned grid, cudaStream_t stream) {
   constexpr int kStages = w4_tile_stages(2 * TH);
   const int ring = kStages * p.stage_bytes, sums = 2 * TH * kTilePitch * 4;
   const int smem = 1024 + kTileControl + (ring > sums ? ring : sums);
@@ -372,24 +375,48 @@ static int w4_tile_kernel_launch(const W4Params& p, unsigned grid, cudaStream_t 
     MKB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  return w4_launch(kern, dim3(grid, 1, 1), kTileThreads, smem, p.split, stream, p);
+  return w4_launch(kern, dim3(grid, 1, 1), kTileThreads, smem, p.split, stream, p, map);
 }
 
 template <typename T, int TH>
-static int w4_tile_group(const W4Params& p, unsigned grid, cudaStream_t stream) {
-  if (p.form.group == 32) return w4_tile_kernel_launch<T, TH, 32>(p, grid, stream);
-  if (p.form.group == 64) return w4_tile_kernel_launch<T, TH, 64>(p, grid, stream);
-  return w4_tile_kernel_launch<T, TH, 128>(p, grid, stream);
+static int w4_tile_group(const W4Params& p, const CUtensorMap& map, unsigned grid, cudaStream_t stream) {
+  if (p.form.group == 32) return w4_tile_kernel_launch<T, TH, 32>(p, map, grid, stream);
+  if (p.form.group == 64) return w4_tile_kernel_launch<T, TH, 64>(p, map, grid, stream);
+  return w4_tile_kernel_launch<T, TH, 128>(p, map, grid, stream);
 }
 
 template <typename T>
-static int w4_tile_tokens(const W4Params& p, int tokens, unsigned grid, cudaStream_t stream) {
+static int w4_tile_tokens(const W4Params& p, const CUtensorMap& map, int tokens, unsigned grid, cudaStream_t stream) {
   switch (tokens) {
-    case 32: return w4_tile_group<T, 16>(p, grid, stream);
-    case 64: return w4_tile_group<T, 32>(p, grid, stream);
-    case 96: return w4_tile_group<T, 48>(p, grid, stream);
-    default: return w4_tile_group<T, 64>(p, grid, stream);
+    case 32: return w4_tile_group<T, 16>(p, map, grid, stream);
+    case 64: return w4_tile_group<T, 32>(p, map, grid, stream);
+    case 96: return w4_tile_group<T, 48>(p, map, grid, stream);
+    default: return w4_tile_group<T, 64>(p, map, grid, stream);
   }
+}
+
+// Tokens as a tensor map: boxes of 64 columns (128 bytes, swizzled) of a CTA's tokens; columns behind K and
+// rows behind M read as zeros.
+static int w4_tile_map(CUtensorMap* map, const W4Params& p, int dtype, int tokens) {
+  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  if (!encode) {
+    void* fn = nullptr;
+    const int rc = driver_entry("cuTensorMapEncodeTiled", &fn);
+    if (rc != MK_OK) return rc;
+    encode = reinterpret_cast<Encode>(fn);
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)p.form.K, (cuuint64_t)p.M};
+  const cuuint64_t strides[1] = {(cuuint64_t)p.lda * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)tokens}, ones[2] = {1, 1};
+  const CUresult r =
+      encode(map, dtype == MK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(p.A), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(MK_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return MK_OK;
 }
 
 int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
@@ -410,11 +437,16 @@ int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
     }
   p.token_tiles = (p.M + tokens - 1) / tokens;
   p.stage_bytes = (tokens * 256 + 2 * f.chunk_bytes + 1023) / 1024 * 1024;
-  p.vec = (reinterpret_cast<uintptr_t>(p.A) & 7) == 0 && p.lda % 4 == 0;
+  p.vec = (reinterpret_cast<uintptr_t>(p.A) & 15) == 0 && p.lda % 8 == 0;
+  CUtensorMap map = {};
+  if (p.vec) {
+    const int rc = w4_tile_map(&map, p, dtype, tokens);
+    if (rc != MK_OK) return rc;
+  }
   const long long grid = row_tiles * p.token_tiles * p.split;
   if (grid > 0x7fffffffLL) return set_error(MK_ERR_INVALID, "4-bit product: M=%d, N=%d is too large", p.M, f.N);
-  return dtype == MK_BF16 ? w4_tile_tokens<__nv_bfloat16>(p, tokens, (unsigned)grid, stream)
-                          : w4_tile_tokens<__half>(p, tokens, (unsigned)grid, stream);
+  return dtype == MK_BF16 ? w4_tile_tokens<__nv_bfloat16>(p, map, tokens, (unsigned)grid, stream)
+                          : w4_tile_tokens<__half>(p, map, tokens, (unsigned)grid, stream);
 }
 
 }  // namespace mkb
