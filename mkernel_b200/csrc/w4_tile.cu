@@ -1,6 +1,6 @@
 // The product with 4-bit weights for more than a few tokens, on the 5th-generation tensor cores.
 //
-// A CTA computes 128 rows of the matrix (two strips) for up to 2 TH tokens, D = W A^T with the weights as
+// A CTA computes 128 rows of the matrix (two strips) for up to 128 tokens, D = W A^T with the weights as
 // the 128-row operand.  That operand never exists in shared memory: the lanes that decode the codes
 // write whole numbers (code - zero, times a power of two) into tensor memory, in the 16x256b form
 // whose lanes are the layout's lanes, and the MMA takes its A operand from there.  So shared memory
@@ -8,17 +8,19 @@
 //
 // One step is one group of columns.  The sums of a group are exact products added in fp32 by the tensor
 // core; the threads that own the accumulator's lanes (a lane is a row of the matrix) read it, multiply
-// it by the row's scale in fp32 and add it to registers, while the tensor core works on the next
-// group in the other accumulator.  No weight is rounded to be multiplied.
+// it by the row's scale in fp32 and add it to registers.  No weight is rounded to be multiplied.
 //
-// Warps 0..7 decode and rescale (quadrant warp % 4 of the lanes; of a step, warp / 4 decides which half of
-// the decoding and which half of the tokens), warp 8 issues the MMAs, a thread of warp 9 (warps
-// 9..11 where rows are not aligned) copies a ring of stages (a block of 128 columns: codes of two strips,
+// A step is little work and a long way: decoding, a barrier, the tensor core, a barrier, reading,
+// rescaling are about 900 cycles one after another for eight warps that share it, when 310 would keep
+// memory busy.  Hence 16 warps and several steps under way: up to 64 tokens, two sets of eight warps
+// take turns at the steps (each with sums of its own, added at the end); for more, whose sums would not
+// fit its registers, all 16 share every step.  Decoders run ahead of the rescaling by the operand
+// buffers that tensor memory has room for beside the accumulators.
+//
+// Warps 0..15 decode and rescale (quadrant warp % 4 of the lanes; of a step, the other bits decide which part
+// of the decoding and which of the tokens), warps 16 and 17 issue the MMAs, a thread of warp 18 (warps 18
+// and 19 where rows are not aligned) copies a ring of stages (a block of 128 columns: codes of two strips,
 // tokens in the 128-byte swizzle).
-//
-// What bounds it, at 128 tokens to a CTA: 128 x 128 x 128 MMAs take about 510 cycles of the tensor pipe,
-// decoding and rescaling 8 warps about 350 of each scheduler's, and the copies 40 KB of L2 traffic,
-// about 640 cycles at 64 bytes a cycle.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -30,13 +32,18 @@
 namespace mkb {
 
 constexpr int kTileRows = 2 * kW4Strip;
-constexpr int kTileCompute = 8;                    // warps
-constexpr int kTileLoaders = 3;
-constexpr int kTileThreads = (kTileCompute + 1 + kTileLoaders) * 32;
+constexpr int kTileCompute = 16;                   // warps
+constexpr int kTileIssue = 2;
+constexpr int kTileLoaders = 2;
+constexpr int kTileThreads = (kTileCompute + kTileIssue + kTileLoaders) * 32;
 constexpr int kTileControl = 1024;                 // bytes before the ring
 constexpr int kTilePitch = kTileRows + 4;          // floats of a token's sums
 
 __host__ __device__ constexpr int w4_tile_stages(int tokens) { return tokens <= 64 ? 8 : tokens <= 96 ? 6 : 5; }
+
+// Accumulators (of `tokens` columns) and operand buffers (of at most 64) that share tensor memory's 512.
+__host__ __device__ constexpr int w4_tile_sums(int tokens) { return tokens == 128 ? 2 : tokens == 96 ? 3 : 4; }
+__host__ __device__ constexpr int w4_tile_operands(int tokens) { return tokens == 96 ? 3 : 4; }
 
 struct TileWait {
   volatile uint32_t* abort;   // shared: some wait of this CTA has run out
@@ -69,14 +76,19 @@ __device__ __forceinline__ bool w4_wait_warp(const TileWait& c, uint32_t bar, ui
   return __all_sync(~0u, w4_wait(c, bar, parity));
 }
 
-template <typename T, int TH, int GROUP>
+template <typename T, int TOKENS, int GROUP>
 __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_constant__ W4Params p,
                                                                  const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t smem_raw[];
-  constexpr int kTokens = 2 * TH;
+  constexpr int kTokens = TOKENS;
+  constexpr int kSets = TOKENS <= 64 ? 2 : 1;       // of warps, that take turns at the steps
+  constexpr int kSubs = kSets == 2 ? 2 : 4;         // warps of a set on a quadrant
+  constexpr int TH = TOKENS / kSubs;                // sums of a thread
   constexpr int kStages = w4_tile_stages(kTokens);
   constexpr int kSteps = kW4Block / GROUP;          // of a block
-  constexpr uint32_t kCols = 2 * kTokens + GROUP <= 256 ? 256 : 512;
+  constexpr int kSums = w4_tile_sums(kTokens), kOperands = w4_tile_operands(kTokens);
+  constexpr uint32_t kUsed = kSums * kTokens + kOperands * (GROUP / 2), kCols = kUsed <= 256 ? 256 : 512;
+  static_assert(kUsed <= 512, "tensor memory has 512 columns");
   constexpr int kXHalf = kTokens * 128;             // bytes of 64 columns of the tokens
 
   const W4Form& f = p.form;
@@ -84,12 +96,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* const base_ptr = smem_raw + (base - raw);
-  // control words: full[8] empty[8] a_full[2] d_full[2] | tensor memory address, abort flag
+  // control words: full[8] empty[8] a_full[4] d_full[4] d_free[4] | tensor memory address, abort flag
   auto full = [&](int s) { return base + 8u * s; };
   auto empty = [&](int s) { return base + 64u + 8u * s; };
   auto a_full = [&](int i) { return base + 128u + 8u * i; };
-  auto d_full = [&](int i) { return base + 144u + 8u * i; };
-  volatile uint32_t* const s_tmem = reinterpret_cast<volatile uint32_t*>(base_ptr + 192);
+  auto d_full = [&](int i) { return base + 160u + 8u * i; };
+  auto d_free = [&](int i) { return base + 192u + 8u * i; };
+  volatile uint32_t* const s_tmem = reinterpret_cast<volatile uint32_t*>(base_ptr + 224);
   volatile uint32_t* const s_abort = s_tmem + 1;
   const uint32_t ring = base + kTileControl;
   uint8_t* const ring_ptr = base_ptr + kTileControl;
@@ -102,17 +115,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   const bool two = strip0 + 1 < f.strips;
 
   if (warp == kTileCompute) {
-    ptx::tmem_alloc(base + 192, kCols);
+    ptx::tmem_alloc(base + 224, kCols);
     ptx::tmem_relinquish();
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       ptx::mbar_init(full(s), p.vec ? 1 : kTileLoaders * 32);
-      ptx::mbar_init(empty(s), kTileCompute + 1);
+      // the warps that decode from it, and the issuing warps that multiply by it
+      ptx::mbar_init(empty(s), GROUP == 128 ? kTileCompute / kSets + 1 : kTileCompute + kTileIssue);
     }
-    for (int i = 0; i < 2; ++i) {
-      ptx::mbar_init(a_full(i), kTileCompute);
+    for (int i = 0; i < kOperands; ++i) ptx::mbar_init(a_full(i), kTileCompute / kSets);
+    for (int i = 0; i < kSums; ++i) {
       ptx::mbar_init(d_full(i), 1);
+      ptx::mbar_init(d_free(i), kTileCompute / kSets);
     }
     *s_abort = 0u;
     ptx::fence_mbar_init();
@@ -121,14 +136,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  const uint32_t tmem_a = tmem + 2 * kTokens;
+  const uint32_t tmem_a = tmem + kSums * kTokens;
   const TileWait wc{s_abort, p.wait_limit_ns};
 
   const size_t strip_bytes = (size_t)f.blocks * f.chunk_bytes;
   const uint8_t* const data = p.data + (size_t)strip0 * strip_bytes + (size_t)rank * f.chunk_bytes;
-  if (warp > kTileCompute) {
+  if (warp >= kTileCompute + kTileIssue) {
     // what is read first may be asked into L2 before the kernel ahead has finished
-    const int lt = threadIdx.x - (kTileCompute + 1) * 32;
+    const int lt = threadIdx.x - (kTileCompute + kTileIssue) * 32;
     for (int b = 0; b < kStages && b < blocks; ++b)
       for (int o = lt * 128; o < f.chunk_bytes; o += kTileLoaders * 32 * 128)
         for (int i = 0; i <= (int)two; ++i)
@@ -140,130 +155,151 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   float acc[TH];
   if (warp < kTileCompute) {
     // ---------------- decode, rescale ----------------
-    const int quad = warp & 3, sub = warp >> 2, g = lane >> 2;
+    const int set = kSets == 2 ? warp >> 3 : 0, quad = warp & 3, g = lane >> 2;
+    const int sub = kSets == 2 ? (warp >> 2) & 1 : warp >> 2;
     const int strip = quad >> 1, tile0 = (quad & 1) * 2;
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const int x_bytes = kTokens * 256;
-    const int codes_at = x_bytes + strip * f.chunk_bytes;
+    const int codes_at = kTokens * 256 + strip * f.chunk_bytes;
     // scale of the accumulator's lane, in 16-bit units behind the codes
     const int row = (quad & 1) * 32 + lane;
     const int scale_at = codes_at + kW4CodeBytes + ((row & 7) * 8 + (row >> 4) * 2 + ((row >> 3) & 1)) * 2;
     const int offset_at = codes_at + kW4CodeBytes + kSteps * 128 + g * 16;
 #pragma unroll
     for (int i = 0; i < TH; ++i) acc[i] = 0.0f;
-    float scale = 0.0f;
-    bool ok = true;
-    auto rescale = [&](int step, float by) {
-      if (!w4_wait_warp(wc, d_full(step & 1), (step >> 1) & 1)) return false;
-      ptx::tc_fence_after();
-      const uint32_t at = tmem + lane_base + (step & 1) * kTokens + sub * TH;
-      if constexpr (TH % 32 == 0) {
+    // The parts of a step that a warp decodes: the quadrant's two tiles, the GROUP columns, cut into kSubs.
+    // kWords words of a lane's four in kUnits tiles, 8 columns of tensor memory a word.
+    constexpr int kUnits = GROUP == 128 && kSubs == 2 ? 2 : 1;
+    constexpr int kWords = (GROUP == 32 ? 2 : 4) / (GROUP < 128 && kSubs == 4 ? 2 : 1);
+    const int my_tile = kUnits == 2 ? 0 : sub & 1;
+    const int my_half = GROUP == 128 ? (kSubs == 4 ? sub >> 1 : sub) : 0;      // of the step
+    const int my_word = GROUP < 128 && kSubs == 4 ? (sub >> 1) * kWords : 0;   // of the step's part of a lane's words
+    auto load_codes = [&](const uint8_t* stage, int gi, uint32_t (&c)[kUnits][kWords]) {
 #pragma unroll
-        for (int c = 0; c < TH; c += 32) {
-          float d[2][16];
-          ptx::tmem_ld_32x16(at + c, d[0]);
-          ptx::tmem_ld_32x16(at + c + 16, d[1]);
-          ptx::tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) acc[c + i] = fmaf(by, d[i / 16][i % 16], acc[c + i]);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < TH; c += 16) {
-          float d[16];
-          ptx::tmem_ld_32x16(at + c, d);
-          ptx::tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(by, d[i], acc[c + i]);
+      for (int i = 0; i < kUnits; ++i) {
+        const int half = GROUP == 128 ? my_half : GROUP == 64 ? gi : gi >> 1;
+        const int word = (GROUP == 32 ? (gi & 1) * 2 : 0) + my_word;
+        const uint8_t* from = stage + codes_at + ((half * 4 + tile0 + my_tile + i) * 32 + lane) * 16 + word * 4;
+        if constexpr (kWords == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(from);
+          c[i][0] = v.x; c[i][1] = v.y; c[i][2] = v.z; c[i][3] = v.w;
+        } else if constexpr (kWords == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(from);
+          c[i][0] = v.x; c[i][1] = v.y;
+        } else {
+          c[i][0] = *reinterpret_cast<const uint32_t*>(from);
         }
       }
+    };
+
+    constexpr int kAhead = kOperands / kSets - 1;   // steps that a set decodes before one is rescaled
+    float scale[kAhead + 1];                        // of this step and the last ones
+#pragma unroll
+    for (int i = 0; i <= kAhead; ++i) scale[i] = 0.0f;
+    bool ok = true;
+    int sums = set;                                 // accumulator of the step that is rescaled next
+    uint32_t parity = 0;
+    constexpr int kBatch = TH % 16 == 0 ? 16 : 8;
+    auto rescale = [&](float by) {
+      if (!w4_wait_warp(wc, d_full(sums), parity)) return false;
+      ptx::tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < TH; c += kBatch) {
+        float d[kBatch];
+        ptx::tmem_ld<kBatch>(tmem + lane_base + sums * kTokens + sub * TH + c, d);
+        ptx::tmem_ld_wait();
+        if (c + kBatch == TH) {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (kOperands > kSums && lane == 0) ptx::mbar_arrive(d_free(sums));
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) acc[c + i] = fmaf(by, d[i], acc[c + i]);
+      }
+      sums += kSets;
+      if (sums >= kSums) { sums -= kSums; parity ^= 1; }
       return true;
     };
-    int step = 0;
-    for (int b = 0; ok && b < blocks; ++b) {
+    int operand = set, step = 0;                    // steps of this set
+    // one step in two blocks, one in a block's two, two in its four; or every one
+    for (int b = GROUP == 128 ? set : 0; ok && b < blocks; b += GROUP == 128 ? kSets : 1) {
       const int s = b % kStages;
       if (!w4_wait_warp(wc, full(s), (b / kStages) & 1)) { ok = false; break; }
       const uint8_t* stage = ring_ptr + s * p.stage_bytes;
+      constexpr int kMine = GROUP == 128 ? 1 : kSteps / kSets;
 #pragma unroll
-      for (int gi = 0; gi < kSteps; ++gi, ++step) {
-        // The other user of this operand buffer, two steps back, has finished: its sums have been read.
-        const uint32_t a_at = tmem_a + lane_base + (step & 1) * (GROUP / 2);
-        auto offsets = [&](int tile, uint32_t& off0, uint32_t& off1) {
-          off0 = off1 = W4Traits<T>::kMinusEight;
+      for (int j = 0; j < kMine; ++j, ++step) {
+        const int gi = GROUP == 128 ? 0 : j * kSets + set;
+        const uint32_t a_at = tmem_a + lane_base + operand * (GROUP / 2);
+        uint32_t codes[kUnits][kWords];
+        load_codes(stage, gi, codes);
+#pragma unroll
+        for (int i = kAhead; i > 0; --i) scale[i] = scale[i - 1];
+        const uint16_t scale_bits = *reinterpret_cast<const uint16_t*>(stage + scale_at + gi * 128);
+        // The last step that used this operand buffer has been rescaled, so the tensor core has left it.
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          uint32_t off0 = W4Traits<T>::kMinusEight, off1 = off0;
           if (f.zeros) {
-            const uint32_t both = *reinterpret_cast<const uint32_t*>(stage + offset_at + gi * 128 + tile * 4);
+            const uint32_t both = *reinterpret_cast<const uint32_t*>(stage + offset_at + gi * 128 + (tile0 + my_tile + i) * 4);
             off0 = __byte_perm(both, 0, 0x1010);
             off1 = __byte_perm(both, 0, 0x3232);
           }
-        };
-        auto decode = [&](uint32_t word, uint32_t off0, uint32_t off1, uint32_t* r) {
-          uint32_t a[4];
-          w4_decode<T>(word, off0, off1, a);
-          r[0] = a[0]; r[1] = a[2]; r[2] = a[1]; r[3] = a[3];
-        };
-        if constexpr (GROUP == 32) {
-          const int tile = tile0 + sub;
-          const uint2 c = *reinterpret_cast<const uint2*>(stage + codes_at + (((gi >> 1) * 4 + tile) * 32 + lane) * 16 + (gi & 1) * 8);
-          uint32_t off0, off1, r[8];
-          offsets(tile, off0, off1);
-          decode(c.x, off0, off1, r);
-          decode(c.y, off0, off1, r + 4);
-          ptx::tmem_st_16x256(a_at + ((uint32_t)(sub * 16) << 16), r);
-        } else {
-          // a half of the block: the step itself, or this warp's part of it
-          const int half = GROUP == 64 ? gi : sub;
+          uint32_t r[kWords * 4];
 #pragma unroll
-          for (int i = 0; i < (GROUP == 64 ? 1 : 2); ++i) {
-            const int in_quad = GROUP == 64 ? sub : i, tile = tile0 + in_quad;
-            const uint4 c = *reinterpret_cast<const uint4*>(stage + codes_at + ((half * 4 + tile) * 32 + lane) * 16);
-            uint32_t off0, off1, r[16];
-            offsets(tile, off0, off1);
-            decode(c.x, off0, off1, r);
-            decode(c.y, off0, off1, r + 4);
-            decode(c.z, off0, off1, r + 8);
-            decode(c.w, off0, off1, r + 12);
-            ptx::tmem_st_16x256(a_at + ((uint32_t)(in_quad * 16) << 16) + (GROUP == 128 ? half * 32 : 0), r);
+          for (int w = 0; w < kWords; ++w) {
+            uint32_t a[4];
+            w4_decode<T>(codes[i][w], off0, off1, a);
+            r[4 * w] = a[0]; r[4 * w + 1] = a[2]; r[4 * w + 2] = a[1]; r[4 * w + 3] = a[3];
           }
+          ptx::tmem_st_16x256(a_at + ((uint32_t)((my_tile + i) * 16) << 16) + my_half * 32 + my_word * 8, r);
         }
-        const float next =
-            W4Traits<T>::to_float(*reinterpret_cast<const uint16_t*>(stage + scale_at + gi * 128));
+        scale[0] = W4Traits<T>::to_float(scale_bits);
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          ptx::mbar_arrive(a_full(step & 1));
-          if (gi == kSteps - 1) ptx::mbar_arrive(empty(s));
+          ptx::mbar_arrive(a_full(operand));
+          if (j == kMine - 1) ptx::mbar_arrive(empty(s));
         }
-        if (step > 0 && !rescale(step - 1, scale)) { ok = false; break; }
-        scale = next;
+        operand += kSets;
+        if (operand >= kOperands) operand -= kOperands;
+        if (step >= kAhead && !rescale(scale[kAhead])) { ok = false; break; }
       }
     }
-    if (ok && step > 0) ok = rescale(step - 1, scale);
+#pragma unroll
+    for (int i = kAhead - 1; i >= 0; --i)
+      if (ok && step > i) ok = rescale(scale[i]);
     if (!ok) {
 #pragma unroll
       for (int i = 0; i < TH; ++i) acc[i] = __int_as_float(0x7fc00000);
     }
     ptx::tc_fence_before();
-  } else if (warp == kTileCompute) {
+  } else if (warp < kTileCompute + kTileIssue) {
     // ---------------- MMA issue: the whole warp, one lane elected inside the statement ----------------
+    // Two warps take turns at the steps: one would be the slowest part of the pipeline (a wait is 150
+    // cycles, the instructions of a step 260, its commits 120).  They need not wait for the tokens: who
+    // decoded the step has.
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t idesc = (1u << 4) | (kType << 7) | (kType << 10) | ((kTokens >> 3) << 17) | ((128u >> 4) << 24);
     const uint32_t desc_hi = static_cast<uint32_t>(ptx::make_smem_desc_sw128(0, 16, 1024) >> 32);
-    int step = 0;
-    bool ok = true;
-    for (int b = 0; ok && b < blocks; ++b) {
+    const int me = warp - kTileCompute;
+    int operand = me, sums = me;
+    uint32_t a_parity = 0, free_parity = 1;   // a fresh barrier has "completed" the phase before its first
+    constexpr int kMine = GROUP == 128 ? 1 : kSteps / kTileIssue;
+    for (int b = GROUP == 128 ? me : 0; b < blocks; b += GROUP == 128 ? kTileIssue : 1) {
       const int s = b % kStages;
-      ok = w4_wait_warp(wc, full(s), (b / kStages) & 1);
-      if (!ok) break;
-      if (!p.vec) ptx::fence_proxy_async();   // the tokens were written by ordinary stores
-      const uint32_t x = ring + s * p.stage_bytes;
-      const uint32_t b_lo = static_cast<uint32_t>(ptx::make_smem_desc_sw128(x, 16, 1024));
+      const uint32_t b_lo = static_cast<uint32_t>(ptx::make_smem_desc_sw128(ring + s * p.stage_bytes, 16, 1024));
+      bool ok = true;
 #pragma unroll
-      for (int gi = 0; gi < kSteps; ++gi, ++step) {
-        ok = w4_wait_warp(wc, a_full(step & 1), (step >> 1) & 1);
+      for (int j = 0; j < kMine; ++j) {
+        const int gi = GROUP == 128 ? 0 : j * kTileIssue + me;
+        ok = w4_wait_warp(wc, a_full(operand), a_parity);
+        // Decoders that run no further ahead than there are accumulators have emptied this one.
+        if (kOperands > kSums) ok = ok && w4_wait_warp(wc, d_free(sums), free_parity);
         if (!ok) break;
+        if (!p.vec) ptx::fence_proxy_async();   // the tokens were written by ordinary stores
         ptx::tc_fence_after();
-        const uint32_t d = tmem + (step & 1) * kTokens, a = tmem_a + (step & 1) * (GROUP / 2);
+        const uint32_t d = tmem + sums * kTokens, a = tmem_a + operand * (GROUP / 2);
         if constexpr (GROUP == 128) {
           ptx::umma_ts<4>(d, a, b_lo, desc_hi, idesc, 0);
           ptx::umma_ts<4>(d, a + 32, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
@@ -272,13 +308,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
         } else {
           ptx::umma_ts<2>(d, a, b_lo + (gi >> 1) * (kXHalf >> 4) + (gi & 1) * 4, desc_hi, idesc, 0);
         }
-        ptx::umma_commit_elect<1>(d_full(step & 1), 0);
+        ptx::umma_commit_elect<1>(d_full(sums), 0);
+        operand += kTileIssue;
+        if (operand >= kOperands) { operand -= kOperands; a_parity ^= 1; }
+        sums += kTileIssue;
+        if (sums >= kSums) { sums -= kSums; free_parity ^= 1; }
       }
-      if (ok) ptx::umma_commit_elect<1>(empty(s), 0);
+      if (!ok) break;
+      ptx::umma_commit_elect<1>(empty(s), 0);
     }
   } else if (p.vec) {
     // ---------------- copies: one thread, tokens by tensor copies, codes by plain ones ----------------
-    if (warp == kTileCompute + 1 && lane == 0) {
+    if (warp == kTileCompute + kTileIssue && lane == 0) {
       const uint32_t tx = kTokens * 256 + f.chunk_bytes * (two ? 2 : 1);
       for (int b = 0; b < blocks; ++b) {
         const int s = b % kStages;
@@ -295,7 +336,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
     }
   } else {
     // ---------------- copies where rows of tokens start on no 16 bytes ----------------
-    const int lt = threadIdx.x - (kTileCompute + 1) * 32, lw = lt >> 5;
+    const int lt = threadIdx.x - (kTileCompute + kTileIssue) * 32, lw = lt >> 5;
     const int pieces = f.chunk_bytes / 16 * (two ? 2 : 1);
     // lane = 4 columns of a token, in the 128-byte swizzle
     const uint32_t unit = lane >> 1 & 7, low = (lane >> 4) * kXHalf + (lane & 1) * 8;
@@ -338,9 +379,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   // The sums, token by token, over the ring; the CTAs of a cluster then share the tokens.
   float* const red = reinterpret_cast<float*>(ring_ptr);
   if (warp < kTileCompute) {
-    const int quad = warp & 3, sub = warp >> 2;
+    const int set = kSets == 2 ? warp >> 3 : 0, quad = warp & 3, sub = kSets == 2 ? (warp >> 2) & 1 : warp >> 2;
 #pragma unroll
-    for (int i = 0; i < TH; ++i) red[(sub * TH + i) * kTilePitch + quad * 32 + lane] = acc[i] * (1.0f / W4Traits<T>::kUnit);
+    for (int i = 0; i < TH; ++i) red[((set * kTokens) + sub * TH + i) * kTilePitch + quad * 32 + lane] = acc[i] * (1.0f / W4Traits<T>::kUnit);
   }
   if (p.split > 1) ptx::cluster_sync_all();
   else __syncthreads();
@@ -352,22 +393,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
     const uint32_t at = ring + (token * kTilePitch + r) * 4;
     float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
     for (int c = 0; c < p.split; ++c) {
-      const uint32_t a = p.split > 1 ? ptx::map_to_cta(at, c) : at;
-      const float4 x = ptx::ld_cluster_f4(a), y = ptx::ld_cluster_f4(a + 32);
-      u.x += x.x; u.y += x.y; u.z += x.z; u.w += x.w;
-      v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+#pragma unroll
+      for (int set = 0; set < kSets; ++set) {
+        const uint32_t own = at + set * kTokens * kTilePitch * 4;
+        const uint32_t a = p.split > 1 ? ptx::map_to_cta(own, c) : own;
+        const float4 x = ptx::ld_cluster_f4(a), y = ptx::ld_cluster_f4(a + 32);
+        u.x += x.x; u.y += x.y; u.z += x.z; u.w += x.w;
+        v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+      }
     }
     w4_epilogue4<T>(p, strip0 + (quad >> 3), (quad & 7) * 4, token0 + token, u, v);
   }
   if (p.split > 1) ptx::cluster_sync_all();   // nobody leaves while its shared memory is read
 }
 
-template <typename T, int TH, int GROUP>
+template <typename T, int TOKENS, int GROUP>
 static int w4_tile_kernel_launch(const W4Params& p, const CUtensorMap& map, unsigned grid, cudaStream_t stream) {
-  constexpr int kStages = w4_tile_stages(2 * TH);
-  const int ring = kStages * p.stage_bytes, sums = 2 * TH * kTilePitch * 4;
+  constexpr int kStages = w4_tile_stages(TOKENS);
+  const int ring = kStages * p.stage_bytes, sums = (TOKENS <= 64 ? 2 : 1) * TOKENS * kTilePitch * 4;
   const int smem = 1024 + kTileControl + (ring > sums ? ring : sums);
-  auto kern = w4_tile_kernel<T, TH, GROUP>;
+  auto kern = w4_tile_kernel<T, TOKENS, GROUP>;
   static bool attr_set[64];
   int dev = 0;
   MKB_CUDA(cudaGetDevice(&dev));
@@ -378,20 +423,20 @@ static int w4_tile_kernel_launch(const W4Params& p, const CUtensorMap& map, unsi
   return w4_launch(kern, dim3(grid, 1, 1), kTileThreads, smem, p.split, stream, p, map);
 }
 
-template <typename T, int TH>
+template <typename T, int TOKENS>
 static int w4_tile_group(const W4Params& p, const CUtensorMap& map, unsigned grid, cudaStream_t stream) {
-  if (p.form.group == 32) return w4_tile_kernel_launch<T, TH, 32>(p, map, grid, stream);
-  if (p.form.group == 64) return w4_tile_kernel_launch<T, TH, 64>(p, map, grid, stream);
-  return w4_tile_kernel_launch<T, TH, 128>(p, map, grid, stream);
+  if (p.form.group == 32) return w4_tile_kernel_launch<T, TOKENS, 32>(p, map, grid, stream);
+  if (p.form.group == 64) return w4_tile_kernel_launch<T, TOKENS, 64>(p, map, grid, stream);
+  return w4_tile_kernel_launch<T, TOKENS, 128>(p, map, grid, stream);
 }
 
 template <typename T>
 static int w4_tile_tokens(const W4Params& p, const CUtensorMap& map, int tokens, unsigned grid, cudaStream_t stream) {
   switch (tokens) {
-    case 32: return w4_tile_group<T, 16>(p, map, grid, stream);
-    case 64: return w4_tile_group<T, 32>(p, map, grid, stream);
-    case 96: return w4_tile_group<T, 48>(p, map, grid, stream);
-    default: return w4_tile_group<T, 64>(p, map, grid, stream);
+    case 32: return w4_tile_group<T, 32>(p, map, grid, stream);
+    case 64: return w4_tile_group<T, 64>(p, map, grid, stream);
+    case 96: return w4_tile_group<T, 96>(p, map, grid, stream);
+    default: return w4_tile_group<T, 128>(p, map, grid, stream);
   }
 }
 
