@@ -142,4 +142,73 @@ __device__ __forceinline__ void w4_decode(uint32_t word, uint32_t off0, uint32_t
   a[3] = W::fma2(next & 0x00f000f0u, W::kHigh, off1);
 }
 
+// The same as the weights themselves, rounded to T: (code - zero) * scale.  sc0, sc1: the scales of rows g and
+// g + 8, each twice; off0, off1: their zero points as the layout holds them.  With `rest`, what the rounding
+// left: the two together are the weight exactly (4 bits times at most 11 are 15, the two parts have
+// at least 16).
+template <typename T>
+struct W4Round;
+template <>
+struct W4Round<__nv_bfloat16> {
+  uint32_t off0, off1, sc0, sc1;
+  __device__ __forceinline__ W4Round(uint32_t o0, uint32_t o1, uint32_t s0, uint32_t s1) : off0(o0), off1(o1) {
+    // a power of two: bf16 has room for it in the exponent
+    sc0 = mul2(s0, W4Traits<__nv_bfloat16>::kBack);
+    sc1 = mul2(s1, W4Traits<__nv_bfloat16>::kBack);
+  }
+  static __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  template <bool REST>
+  __device__ __forceinline__ void get(uint32_t word, uint32_t (&a)[4], uint32_t (&rest)[4]) const {
+    uint32_t v[4];
+    w4_decode<__nv_bfloat16>(word, off0, off1, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t sc = i & 1 ? sc1 : sc0;
+      a[i] = mul2(v[i], sc);
+      if (REST) rest[i] = W4Traits<__nv_bfloat16>::fma2(v[i], sc, a[i] ^ 0x80008000u);
+    }
+  }
+};
+template <>
+struct W4Round<__half> {
+  // fp16 has not, so the code is made whole another way: in the low bits of 1024 (or, 16 times as much, four
+  // bits up), less 1024 (64) and the zero point.
+  uint32_t less0, less1, sc0, sc1;
+  __device__ __forceinline__ W4Round(uint32_t o0, uint32_t o1, uint32_t s0, uint32_t s1) : sc0(s0), sc1(s1) {
+    less0 = W4Traits<__half>::fma2(o0, W4Traits<__half>::kBack, 0xe400e400u);   // -zero - 1024
+    less1 = W4Traits<__half>::fma2(o1, W4Traits<__half>::kBack, 0xd400d400u);   // -zero - 64
+  }
+  static __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t low(uint32_t word, uint32_t less) {
+    uint32_t v, r;
+    asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(v) : "r"(word), "n"(0x64006400));
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(less));
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t high(uint32_t word, uint32_t less) {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xea;" : "=r"(v) : "r"(word), "n"(0x64006400));
+    return W4Traits<__half>::fma2(v, 0x2c002c00u, less);   // times 1/16
+  }
+  template <bool REST>
+  __device__ __forceinline__ void get(uint32_t word, uint32_t (&a)[4], uint32_t (&rest)[4]) const {
+    const uint32_t next = word >> 8;
+    const uint32_t v[4] = {low(word, less0), high(word, less1), low(next, less0), high(next, less1)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t sc = i & 1 ? sc1 : sc0;
+      a[i] = mul2(v[i], sc);
+      if (REST) rest[i] = W4Traits<__half>::fma2(v[i], sc, a[i] ^ 0x80008000u);
+    }
+  }
+};
+
 }  // namespace mkb

@@ -1,29 +1,28 @@
 // The product with 4-bit weights for more than a few tokens, on the 5th-generation tensor cores.
 //
-// A CTA computes 128 rows of the matrix (two strips) for up to 128 tokens, D = W A^T with the weights as
+// A CTA computes 128 rows of the matrix (two strips) for up to 256 tokens, D = W A^T with the weights as
 // the 128-row operand.  That operand never exists in shared memory: the lanes that decode the codes
-// write whole numbers (code - zero, times a power of two) into tensor memory, in the 16x256b form
-// whose lanes are the layout's lanes, and the MMA takes its A operand from there.  So shared memory
-// carries only the packed codes and the tokens.
+// write the weights into tensor memory, in the 16x256b form whose lanes are the layout's lanes, and the
+// MMA takes its A operand from there.  So shared memory carries only the packed codes and the tokens.
 //
-// One step is one group of columns.  The sums of a group are exact products added in fp32 by the tensor
-// core; the threads that own the accumulator's lanes (a lane is a row of the matrix) read it, multiply
-// it by the row's scale in fp32 and add it to registers.  No weight is rounded to be multiplied.
+// Here a weight is rounded to the 16-bit type before it is multiplied, (code - zero) * scale, exactly as
+// mk_w4_dequantize gives it, and D stays in tensor memory from the first column to the last.  The
+// few-token kernel rounds nothing; to do the same here the sums of every group must leave the tensor core to
+// be scaled in fp32, which was built first and costs a tour through registers and two waits a group
+// (256 tokens of 8192 x 8192 in groups of 64: 59 us that way, 34 this).  What the rounding adds is
+// smaller than the output's own (relative to the result 1.4e-3 in bf16, where that is 1.7e-3).  In the
+// SwiGLU form two such sums are multiplied and it would be larger (2.1e-3), so there what the rounding left
+// (REST) is multiplied as well, and nothing is lost.
 //
-// A step is little work and a long way: decoding, a barrier, the tensor core, a barrier, reading,
-// rescaling are about 900 cycles one after another for eight warps that share it, when 310 would keep
-// memory busy.  Hence 16 warps and several steps under way: up to 64 tokens, two sets of eight warps
-// take turns at the steps (each with sums of its own, added at the end); for more, whose sums would not
-// fit its registers, all 16 share every step.  Decoders run ahead of the rescaling by the operand
-// buffers that tensor memory has room for beside the accumulators.
-//
-// Warps 0..15 decode and rescale (quadrant warp % 4 of the lanes; of a step, the other bits decide which part
-// of the decoding and which of the tokens), warps 16 and 17 issue the MMAs, a thread of warp 18 (warps 18
-// and 19 where rows are not aligned) copies a ring of stages (a block of 128 columns: codes of two strips,
-// tokens in the 128-byte swizzle).
+// Warps 0..7 decode (quadrant warp % 4 of the lanes, half warp / 4 of a block's 128 columns) and at the end
+// read the sums, warp 8 issues the MMAs, a thread of warp 9 (warps 9..11 where rows are not aligned)
+// copies a ring of stages (a block: codes of two strips, tokens in the 128-byte swizzle).  Decoders
+// run ahead of the tensor core by the operand buffers that tensor memory has room for.  Up to 64 tokens
+// two CTAs share an SM, which hides their starts, ends and waits behind one another.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cstdlib>
 #include <type_traits>
 
 #include "../../include/mkernel_b200.h"
@@ -32,18 +31,21 @@
 namespace mkb {
 
 constexpr int kTileRows = 2 * kW4Strip;
-constexpr int kTileCompute = 16;                   // warps
-constexpr int kTileIssue = 2;
-constexpr int kTileLoaders = 2;
-constexpr int kTileThreads = (kTileCompute + kTileIssue + kTileLoaders) * 32;
+constexpr int kTileCompute = 8;                    // warps
+constexpr int kTileLoaders = 3;
+constexpr int kTileThreads = (kTileCompute + 1 + kTileLoaders) * 32;
 constexpr int kTileControl = 1024;                 // bytes before the ring
 constexpr int kTilePitch = kTileRows + 4;          // floats of a token's sums
 
-__host__ __device__ constexpr int w4_tile_stages(int tokens) { return tokens <= 64 ? 8 : tokens <= 96 ? 6 : 5; }
-
-// Accumulators (of `tokens` columns) and operand buffers (of at most 64) that share tensor memory's 512.
-__host__ __device__ constexpr int w4_tile_sums(int tokens) { return tokens == 128 ? 2 : tokens == 96 ? 3 : 4; }
-__host__ __device__ constexpr int w4_tile_operands(int tokens) { return tokens == 96 ? 3 : 4; }
+// Stages of the ring, operand buffers (64 columns of tensor memory beside the `tokens` of the sums) and CTAs
+// of an SM (227 KB and 512 columns).
+__host__ __device__ constexpr int w4_tile_stages(int tokens) {
+  return tokens == 32 ? 5 : tokens == 64 ? 4 : tokens == 128 ? 5 : 3;
+}
+__host__ __device__ constexpr int w4_tile_operands(int tokens, bool rest) {
+  return tokens <= 64 ? 3 : !rest ? 4 : tokens == 128 ? 3 : 2;
+}
+__host__ __device__ constexpr int w4_tile_ctas(int tokens, bool rest) { return tokens <= 64 && !rest ? 2 : 1; }
 
 struct TileWait {
   volatile uint32_t* abort;   // shared: some wait of this CTA has run out
@@ -76,19 +78,15 @@ __device__ __forceinline__ bool w4_wait_warp(const TileWait& c, uint32_t bar, ui
   return __all_sync(~0u, w4_wait(c, bar, parity));
 }
 
-template <typename T, int TOKENS, int GROUP>
-__global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_constant__ W4Params p,
-                                                                 const __grid_constant__ CUtensorMap map) {
+template <typename T, int TOKENS, int GROUP, bool REST>
+__global__ void __launch_bounds__(kTileThreads, w4_tile_ctas(TOKENS, REST))
+    w4_tile_kernel(const __grid_constant__ W4Params p, const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int kTokens = TOKENS;
-  constexpr int kSets = TOKENS <= 64 ? 2 : 1;       // of warps, that take turns at the steps
-  constexpr int kSubs = kSets == 2 ? 2 : 4;         // warps of a set on a quadrant
-  constexpr int TH = TOKENS / kSubs;                // sums of a thread
   constexpr int kStages = w4_tile_stages(kTokens);
-  constexpr int kSteps = kW4Block / GROUP;          // of a block
-  constexpr int kSums = w4_tile_sums(kTokens), kOperands = w4_tile_operands(kTokens);
-  constexpr uint32_t kUsed = kSums * kTokens + kOperands * (GROUP / 2), kCols = kUsed <= 256 ? 256 : 512;
-  static_assert(kUsed <= 512, "tensor memory has 512 columns");
+  constexpr int kOperands = w4_tile_operands(kTokens, REST), kOperand = REST ? 128 : 64;   // columns of one
+  constexpr uint32_t kCols = kTokens + kOperand * kOperands <= 256 ? 256 : 512;
+  static_assert(kTokens + kOperand * kOperands <= 512 / w4_tile_ctas(TOKENS, REST), "tensor memory has 512 columns");
   constexpr int kXHalf = kTokens * 128;             // bytes of 64 columns of the tokens
 
   const W4Form& f = p.form;
@@ -96,12 +94,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* const base_ptr = smem_raw + (base - raw);
-  // control words: full[8] empty[8] a_full[4] d_full[4] d_free[4] | tensor memory address, abort flag
+  // control words: full[5] empty[5] a_full[4] a_empty[4] done | tensor memory address, abort flag
   auto full = [&](int s) { return base + 8u * s; };
   auto empty = [&](int s) { return base + 64u + 8u * s; };
   auto a_full = [&](int i) { return base + 128u + 8u * i; };
-  auto d_full = [&](int i) { return base + 160u + 8u * i; };
-  auto d_free = [&](int i) { return base + 192u + 8u * i; };
+  auto a_empty = [&](int i) { return base + 160u + 8u * i; };
+  const uint32_t done = base + 192u;
   volatile uint32_t* const s_tmem = reinterpret_cast<volatile uint32_t*>(base_ptr + 224);
   volatile uint32_t* const s_abort = s_tmem + 1;
   const uint32_t ring = base + kTileControl;
@@ -121,14 +119,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       ptx::mbar_init(full(s), p.vec ? 1 : kTileLoaders * 32);
-      // the warps that decode from it, and the issuing warps that multiply by it
-      ptx::mbar_init(empty(s), GROUP == 128 ? kTileCompute / kSets + 1 : kTileCompute + kTileIssue);
+      ptx::mbar_init(empty(s), kTileCompute + 1);
     }
-    for (int i = 0; i < kOperands; ++i) ptx::mbar_init(a_full(i), kTileCompute / kSets);
-    for (int i = 0; i < kSums; ++i) {
-      ptx::mbar_init(d_full(i), 1);
-      ptx::mbar_init(d_free(i), kTileCompute / kSets);
+    for (int i = 0; i < kOperands; ++i) {
+      ptx::mbar_init(a_full(i), kTileCompute);
+      ptx::mbar_init(a_empty(i), 1);
     }
+    ptx::mbar_init(done, 1);
     *s_abort = 0u;
     ptx::fence_mbar_init();
   }
@@ -136,14 +133,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  const uint32_t tmem_a = tmem + kSums * kTokens;
+  const uint32_t tmem_a = tmem + kTokens;
   const TileWait wc{s_abort, p.wait_limit_ns};
 
   const size_t strip_bytes = (size_t)f.blocks * f.chunk_bytes;
   const uint8_t* const data = p.data + (size_t)strip0 * strip_bytes + (size_t)rank * f.chunk_bytes;
-  if (warp >= kTileCompute + kTileIssue) {
+  if (warp > kTileCompute) {
     // what is read first may be asked into L2 before the kernel ahead has finished
-    const int lt = threadIdx.x - (kTileCompute + kTileIssue) * 32;
+    const int lt = threadIdx.x - (kTileCompute + 1) * 32;
     for (int b = 0; b < kStages && b < blocks; ++b)
       for (int o = lt * 128; o < f.chunk_bytes; o += kTileLoaders * 32 * 128)
         for (int i = 0; i <= (int)two; ++i)
@@ -152,174 +149,99 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
-  float acc[TH];
+  const int quad = warp & 3, half = warp >> 2;
+  bool ok = true;
   if (warp < kTileCompute) {
-    // ---------------- decode, rescale ----------------
-    const int set = kSets == 2 ? warp >> 3 : 0, quad = warp & 3, g = lane >> 2;
-    const int sub = kSets == 2 ? (warp >> 2) & 1 : warp >> 2;
+    // ---------------- decode ----------------
+    const int g = lane >> 2;
     const int strip = quad >> 1, tile0 = (quad & 1) * 2;
-    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const int codes_at = kTokens * 256 + strip * f.chunk_bytes;
-    // scale of the accumulator's lane, in 16-bit units behind the codes
-    const int row = (quad & 1) * 32 + lane;
-    const int scale_at = codes_at + kW4CodeBytes + ((row & 7) * 8 + (row >> 4) * 2 + ((row >> 3) & 1)) * 2;
-    const int offset_at = codes_at + kW4CodeBytes + kSteps * 128 + g * 16;
+    constexpr int kGroups = kW4Block / GROUP;
+    // of a stage: this lane's codes of two tiles, and the scales and zero points of its rows there
+    const int codes_at = kTokens * 256 + strip * f.chunk_bytes + ((half * 4 + tile0) * 32 + lane) * 16;
+    const int scales_at = kTokens * 256 + strip * f.chunk_bytes + kW4CodeBytes + g * 16 + tile0 * 4 +
+                          (half * 64 / GROUP) * 128;
+    const uint32_t a_at = tmem_a + ((uint32_t)(quad * 32) << 16) + half * 32;
+    int s = 0, operand = 0;
+    uint32_t parity = 0, a_parity = 1;   // a fresh barrier has "completed" the phase before its first
+    for (int b = 0; b < blocks; ++b) {
+      ok = w4_wait_warp(wc, full(s), parity);
+      if (!ok) break;
+      const uint8_t* stage = ring_ptr + s * p.stage_bytes;
+      uint4 codes[2];
+      uint2 scales[GROUP == 32 ? 2 : 1], zeros[GROUP == 32 ? 2 : 1];
 #pragma unroll
-    for (int i = 0; i < TH; ++i) acc[i] = 0.0f;
-    // The parts of a step that a warp decodes: the quadrant's two tiles, the GROUP columns, cut into kSubs.
-    // kWords words of a lane's four in kUnits tiles, 8 columns of tensor memory a word.
-    constexpr int kUnits = GROUP == 128 && kSubs == 2 ? 2 : 1;
-    constexpr int kWords = (GROUP == 32 ? 2 : 4) / (GROUP < 128 && kSubs == 4 ? 2 : 1);
-    const int my_tile = kUnits == 2 ? 0 : sub & 1;
-    const int my_half = GROUP == 128 ? (kSubs == 4 ? sub >> 1 : sub) : 0;      // of the step
-    const int my_word = GROUP < 128 && kSubs == 4 ? (sub >> 1) * kWords : 0;   // of the step's part of a lane's words
-    auto load_codes = [&](const uint8_t* stage, int gi, uint32_t (&c)[kUnits][kWords]) {
+      for (int i = 0; i < 2; ++i) codes[i] = *reinterpret_cast<const uint4*>(stage + codes_at + i * 512);
 #pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
-        const int half = GROUP == 128 ? my_half : GROUP == 64 ? gi : gi >> 1;
-        const int word = (GROUP == 32 ? (gi & 1) * 2 : 0) + my_word;
-        const uint8_t* from = stage + codes_at + ((half * 4 + tile0 + my_tile + i) * 32 + lane) * 16 + word * 4;
-        if constexpr (kWords == 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(from);
-          c[i][0] = v.x; c[i][1] = v.y; c[i][2] = v.z; c[i][3] = v.w;
-        } else if constexpr (kWords == 2) {
-          const uint2 v = *reinterpret_cast<const uint2*>(from);
-          c[i][0] = v.x; c[i][1] = v.y;
-        } else {
-          c[i][0] = *reinterpret_cast<const uint32_t*>(from);
-        }
+      for (int i = 0; i < (GROUP == 32 ? 2 : 1); ++i) {
+        scales[i] = *reinterpret_cast<const uint2*>(stage + scales_at + i * 128);
+        zeros[i] = make_uint2(W4Traits<T>::kMinusEight, W4Traits<T>::kMinusEight);
+        if (f.zeros) zeros[i] = *reinterpret_cast<const uint2*>(stage + scales_at + (kGroups + i) * 128);
       }
-    };
-
-    constexpr int kAhead = kOperands / kSets - 1;   // steps that a set decodes before one is rescaled
-    float scale[kAhead + 1];                        // of this step and the last ones
-#pragma unroll
-    for (int i = 0; i <= kAhead; ++i) scale[i] = 0.0f;
-    bool ok = true;
-    int sums = set;                                 // accumulator of the step that is rescaled next
-    uint32_t parity = 0;
-    constexpr int kBatch = TH % 16 == 0 ? 16 : 8;
-    auto rescale = [&](float by) {
-      if (!w4_wait_warp(wc, d_full(sums), parity)) return false;
+      ok = w4_wait_warp(wc, a_empty(operand), a_parity);
+      if (!ok) break;
       ptx::tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < TH; c += kBatch) {
-        float d[kBatch];
-        ptx::tmem_ld<kBatch>(tmem + lane_base + sums * kTokens + sub * TH + c, d);
-        ptx::tmem_ld_wait();
-        if (c + kBatch == TH) {
-          ptx::tc_fence_before();
-          __syncwarp();
-          if (kOperands > kSums && lane == 0) ptx::mbar_arrive(d_free(sums));
-        }
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t words[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+        uint32_t r[16], rest[16];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) acc[c + i] = fmaf(by, d[i], acc[c + i]);
-      }
-      sums += kSets;
-      if (sums >= kSums) { sums -= kSums; parity ^= 1; }
-      return true;
-    };
-    int operand = set, step = 0;                    // steps of this set
-    // one step in two blocks, one in a block's two, two in its four; or every one
-    for (int b = GROUP == 128 ? set : 0; ok && b < blocks; b += GROUP == 128 ? kSets : 1) {
-      const int s = b % kStages;
-      if (!w4_wait_warp(wc, full(s), (b / kStages) & 1)) { ok = false; break; }
-      const uint8_t* stage = ring_ptr + s * p.stage_bytes;
-      constexpr int kMine = GROUP == 128 ? 1 : kSteps / kSets;
+        for (int v = 0; v < 4; v += 2) {
+          const int gi = GROUP == 32 ? v / 2 : 0;
+          const uint32_t sc = i ? scales[gi].y : scales[gi].x, z = i ? zeros[gi].y : zeros[gi].x;
+          const W4Round<T> weights(__byte_perm(z, 0, 0x1010), __byte_perm(z, 0, 0x3232), __byte_perm(sc, 0, 0x1010),
+                                   __byte_perm(sc, 0, 0x3232));
 #pragma unroll
-      for (int j = 0; j < kMine; ++j, ++step) {
-        const int gi = GROUP == 128 ? 0 : j * kSets + set;
-        const uint32_t a_at = tmem_a + lane_base + operand * (GROUP / 2);
-        uint32_t codes[kUnits][kWords];
-        load_codes(stage, gi, codes);
-#pragma unroll
-        for (int i = kAhead; i > 0; --i) scale[i] = scale[i - 1];
-        const uint16_t scale_bits = *reinterpret_cast<const uint16_t*>(stage + scale_at + gi * 128);
-        // The last step that used this operand buffer has been rescaled, so the tensor core has left it.
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-          uint32_t off0 = W4Traits<T>::kMinusEight, off1 = off0;
-          if (f.zeros) {
-            const uint32_t both = *reinterpret_cast<const uint32_t*>(stage + offset_at + gi * 128 + (tile0 + my_tile + i) * 4);
-            off0 = __byte_perm(both, 0, 0x1010);
-            off1 = __byte_perm(both, 0, 0x3232);
-          }
-          uint32_t r[kWords * 4];
-#pragma unroll
-          for (int w = 0; w < kWords; ++w) {
-            uint32_t a[4];
-            w4_decode<T>(codes[i][w], off0, off1, a);
+          for (int w = v; w < v + 2; ++w) {
+            uint32_t a[4], b[4];
+            weights.template get<REST>(words[w], a, b);
             r[4 * w] = a[0]; r[4 * w + 1] = a[2]; r[4 * w + 2] = a[1]; r[4 * w + 3] = a[3];
+            if (REST) { rest[4 * w] = b[0]; rest[4 * w + 1] = b[2]; rest[4 * w + 2] = b[1]; rest[4 * w + 3] = b[3]; }
           }
-          ptx::tmem_st_16x256(a_at + ((uint32_t)((my_tile + i) * 16) << 16) + my_half * 32 + my_word * 8, r);
         }
-        scale[0] = W4Traits<T>::to_float(scale_bits);
-        ptx::tmem_st_wait();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          ptx::mbar_arrive(a_full(operand));
-          if (j == kMine - 1) ptx::mbar_arrive(empty(s));
-        }
-        operand += kSets;
-        if (operand >= kOperands) operand -= kOperands;
-        if (step >= kAhead && !rescale(scale[kAhead])) { ok = false; break; }
+        ptx::tmem_st_16x256(a_at + operand * kOperand + ((uint32_t)(i * 16) << 16), r);
+        if (REST) ptx::tmem_st_16x256(a_at + operand * kOperand + 64 + ((uint32_t)(i * 16) << 16), rest);
       }
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        ptx::mbar_arrive(a_full(operand));
+        ptx::mbar_arrive(empty(s));
+      }
+      if (++s == kStages) { s = 0; parity ^= 1; }
+      if (++operand == kOperands) { operand = 0; a_parity ^= 1; }
     }
-#pragma unroll
-    for (int i = kAhead - 1; i >= 0; --i)
-      if (ok && step > i) ok = rescale(scale[i]);
-    if (!ok) {
-#pragma unroll
-      for (int i = 0; i < TH; ++i) acc[i] = __int_as_float(0x7fc00000);
-    }
-    ptx::tc_fence_before();
-  } else if (warp < kTileCompute + kTileIssue) {
+    ok = ok && w4_wait_warp(wc, done, 0);
+  } else if (warp == kTileCompute) {
     // ---------------- MMA issue: the whole warp, one lane elected inside the statement ----------------
-    // Two warps take turns at the steps: one would be the slowest part of the pipeline (a wait is 150
-    // cycles, the instructions of a step 260, its commits 120).  They need not wait for the tokens: who
-    // decoded the step has.
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t idesc = (1u << 4) | (kType << 7) | (kType << 10) | ((kTokens >> 3) << 17) | ((128u >> 4) << 24);
     const uint32_t desc_hi = static_cast<uint32_t>(ptx::make_smem_desc_sw128(0, 16, 1024) >> 32);
-    const int me = warp - kTileCompute;
-    int operand = me, sums = me;
-    uint32_t a_parity = 0, free_parity = 1;   // a fresh barrier has "completed" the phase before its first
-    constexpr int kMine = GROUP == 128 ? 1 : kSteps / kTileIssue;
-    for (int b = GROUP == 128 ? me : 0; b < blocks; b += GROUP == 128 ? kTileIssue : 1) {
-      const int s = b % kStages;
-      const uint32_t b_lo = static_cast<uint32_t>(ptx::make_smem_desc_sw128(ring + s * p.stage_bytes, 16, 1024));
-      bool ok = true;
-#pragma unroll
-      for (int j = 0; j < kMine; ++j) {
-        const int gi = GROUP == 128 ? 0 : j * kTileIssue + me;
-        ok = w4_wait_warp(wc, a_full(operand), a_parity);
-        // Decoders that run no further ahead than there are accumulators have emptied this one.
-        if (kOperands > kSums) ok = ok && w4_wait_warp(wc, d_free(sums), free_parity);
-        if (!ok) break;
-        if (!p.vec) ptx::fence_proxy_async();   // the tokens were written by ordinary stores
-        ptx::tc_fence_after();
-        const uint32_t d = tmem + sums * kTokens, a = tmem_a + operand * (GROUP / 2);
-        if constexpr (GROUP == 128) {
-          ptx::umma_ts<4>(d, a, b_lo, desc_hi, idesc, 0);
-          ptx::umma_ts<4>(d, a + 32, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
-        } else if constexpr (GROUP == 64) {
-          ptx::umma_ts<4>(d, a, b_lo + gi * (kXHalf >> 4), desc_hi, idesc, 0);
-        } else {
-          ptx::umma_ts<2>(d, a, b_lo + (gi >> 1) * (kXHalf >> 4) + (gi & 1) * 4, desc_hi, idesc, 0);
-        }
-        ptx::umma_commit_elect<1>(d_full(sums), 0);
-        operand += kTileIssue;
-        if (operand >= kOperands) { operand -= kOperands; a_parity ^= 1; }
-        sums += kTileIssue;
-        if (sums >= kSums) { sums -= kSums; free_parity ^= 1; }
-      }
+    const uint32_t b_lo0 = static_cast<uint32_t>(ptx::make_smem_desc_sw128(ring, 16, 1024));
+    int s = 0, operand = 0;
+    uint32_t a_parity = 0;
+    for (int b = 0; b < blocks; ++b) {
+      // The tokens need no wait of their own: who decoded the block has waited for them.
+      ok = w4_wait_warp(wc, a_full(operand), a_parity);
       if (!ok) break;
+      if (!p.vec) ptx::fence_proxy_async();   // the tokens were written by ordinary stores
+      ptx::tc_fence_after();
+      const uint32_t a = tmem_a + operand * kOperand, b_lo = b_lo0 + s * (p.stage_bytes >> 4);
+      ptx::umma_ts<4>(tmem, a, b_lo, desc_hi, idesc, b > 0 ? 1u : 0u);
+      ptx::umma_ts<4>(tmem, a + 32, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
+      if (REST) {
+        ptx::umma_ts<4>(tmem, a + 64, b_lo, desc_hi, idesc, 1);
+        ptx::umma_ts<4>(tmem, a + 96, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
+      }
+      ptx::umma_commit_elect<1>(a_empty(operand), 0);
       ptx::umma_commit_elect<1>(empty(s), 0);
+      if (++s == kStages) s = 0;
+      if (++operand == kOperands) { operand = 0; a_parity ^= 1; }
     }
+    if (ok) ptx::umma_commit_elect<1>(done, 0);
   } else if (p.vec) {
     // ---------------- copies: one thread, tokens by tensor copies, codes by plain ones ----------------
-    if (warp == kTileCompute + kTileIssue && lane == 0) {
+    if (warp == kTileCompute + 1 && lane == 0) {
       const uint32_t tx = kTokens * 256 + f.chunk_bytes * (two ? 2 : 1);
       for (int b = 0; b < blocks; ++b) {
         const int s = b % kStages;
@@ -336,7 +258,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
     }
   } else {
     // ---------------- copies where rows of tokens start on no 16 bytes ----------------
-    const int lt = threadIdx.x - (kTileCompute + kTileIssue) * 32, lw = lt >> 5;
+    const int lt = threadIdx.x - (kTileCompute + 1) * 32, lw = lt >> 5;
     const int pieces = f.chunk_bytes / 16 * (two ? 2 : 1);
     // lane = 4 columns of a token, in the 128-byte swizzle
     const uint32_t unit = lane >> 1 & 7, low = (lane >> 4) * kXHalf + (lane & 1) * 8;
@@ -371,20 +293,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   // a wait that ran out leaves MMAs that may still read the ring
   if (*s_abort != 0u) __nanosleep(50000);
   __syncthreads();
-  if (warp == kTileCompute) {
-    ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, kCols);
-  }
 
   // The sums, token by token, over the ring; the CTAs of a cluster then share the tokens.
   float* const red = reinterpret_cast<float*>(ring_ptr);
   if (warp < kTileCompute) {
-    const int set = kSets == 2 ? warp >> 3 : 0, quad = warp & 3, sub = kSets == 2 ? (warp >> 2) & 1 : warp >> 2;
+    ptx::tc_fence_after();
 #pragma unroll
-    for (int i = 0; i < TH; ++i) red[((set * kTokens) + sub * TH + i) * kTilePitch + quad * 32 + lane] = acc[i] * (1.0f / W4Traits<T>::kUnit);
+    for (int c = 0; c < kTokens / 2; c += 16) {
+      float d[16];
+      ptx::tmem_ld<16>(tmem + ((uint32_t)(quad * 32) << 16) + half * (kTokens / 2) + c, d);
+      ptx::tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        red[(half * (kTokens / 2) + c + i) * kTilePitch + quad * 32 + lane] = ok ? d[i] : __int_as_float(0x7fc00000);
+    }
+    ptx::tc_fence_before();
   }
   if (p.split > 1) ptx::cluster_sync_all();
   else __syncthreads();
+  if (warp == kTileCompute) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, kCols);
+  }
   // Four pairs of a token at a time: rows r .. r + 3 and r + 8 .. r + 11 of a tile.
   const int items = min(kTokens, p.M - token0) * (two ? 16 : 8);
   for (int e = rank * kTileThreads + threadIdx.x; e < items; e += p.split * kTileThreads) {
@@ -393,26 +323,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
     const uint32_t at = ring + (token * kTilePitch + r) * 4;
     float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
     for (int c = 0; c < p.split; ++c) {
-#pragma unroll
-      for (int set = 0; set < kSets; ++set) {
-        const uint32_t own = at + set * kTokens * kTilePitch * 4;
-        const uint32_t a = p.split > 1 ? ptx::map_to_cta(own, c) : own;
-        const float4 x = ptx::ld_cluster_f4(a), y = ptx::ld_cluster_f4(a + 32);
-        u.x += x.x; u.y += x.y; u.z += x.z; u.w += x.w;
-        v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
-      }
+      const uint32_t a = p.split > 1 ? ptx::map_to_cta(at, c) : at;
+      const float4 x = ptx::ld_cluster_f4(a), y = ptx::ld_cluster_f4(a + 32);
+      u.x += x.x; u.y += x.y; u.z += x.z; u.w += x.w;
+      v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
     }
     w4_epilogue4<T>(p, strip0 + (quad >> 3), (quad & 7) * 4, token0 + token, u, v);
   }
   if (p.split > 1) ptx::cluster_sync_all();   // nobody leaves while its shared memory is read
 }
 
-template <typename T, int TOKENS, int GROUP>
+template <typename T, int TOKENS, int GROUP, bool REST>
 static int w4_tile_kernel_launch(const W4Params& p, const CUtensorMap& map, unsigned grid, cudaStream_t stream) {
   constexpr int kStages = w4_tile_stages(TOKENS);
-  const int ring = kStages * p.stage_bytes, sums = (TOKENS <= 64 ? 2 : 1) * TOKENS * kTilePitch * 4;
+  const int ring = kStages * p.stage_bytes, sums = TOKENS * kTilePitch * 4;
   const int smem = 1024 + kTileControl + (ring > sums ? ring : sums);
-  auto kern = w4_tile_kernel<T, TOKENS, GROUP>;
+  auto kern = w4_tile_kernel<T, TOKENS, GROUP, REST>;
   static bool attr_set[64];
   int dev = 0;
   MKB_CUDA(cudaGetDevice(&dev));
@@ -423,20 +349,25 @@ static int w4_tile_kernel_launch(const W4Params& p, const CUtensorMap& map, unsi
   return w4_launch(kern, dim3(grid, 1, 1), kTileThreads, smem, p.split, stream, p, map);
 }
 
-template <typename T, int TOKENS>
+template <typename T, int TOKENS, bool REST>
 static int w4_tile_group(const W4Params& p, const CUtensorMap& map, unsigned grid, cudaStream_t stream) {
-  if (p.form.group == 32) return w4_tile_kernel_launch<T, TOKENS, 32>(p, map, grid, stream);
-  if (p.form.group == 64) return w4_tile_kernel_launch<T, TOKENS, 64>(p, map, grid, stream);
-  return w4_tile_kernel_launch<T, TOKENS, 128>(p, map, grid, stream);
+  if (p.form.group == 32) return w4_tile_kernel_launch<T, TOKENS, 32, REST>(p, map, grid, stream);
+  if (p.form.group == 64) return w4_tile_kernel_launch<T, TOKENS, 64, REST>(p, map, grid, stream);
+  return w4_tile_kernel_launch<T, TOKENS, 128, REST>(p, map, grid, stream);
+}
+template <typename T, int TOKENS>
+static int w4_tile_rest(const W4Params& p, const CUtensorMap& map, unsigned grid, cudaStream_t stream) {
+  return p.epilogue == W4_EPI_SWIGLU ? w4_tile_group<T, TOKENS, true>(p, map, grid, stream)
+                                     : w4_tile_group<T, TOKENS, false>(p, map, grid, stream);
 }
 
 template <typename T>
 static int w4_tile_tokens(const W4Params& p, const CUtensorMap& map, int tokens, unsigned grid, cudaStream_t stream) {
   switch (tokens) {
-    case 32: return w4_tile_group<T, 32>(p, map, grid, stream);
-    case 64: return w4_tile_group<T, 64>(p, map, grid, stream);
-    case 96: return w4_tile_group<T, 96>(p, map, grid, stream);
-    default: return w4_tile_group<T, 128>(p, map, grid, stream);
+    case 32: return w4_tile_rest<T, 32>(p, map, grid, stream);
+    case 64: return w4_tile_rest<T, 64>(p, map, grid, stream);
+    case 128: return w4_tile_rest<T, 128>(p, map, grid, stream);
+    default: return w4_tile_rest<T, 256>(p, map, grid, stream);
   }
 }
 
@@ -467,19 +398,21 @@ static int w4_tile_map(CUtensorMap* map, const W4Params& p, int dtype, int token
 int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
   const W4Form& f = p.form;
   const long long row_tiles = (f.strips + 1) / 2;
-  // Tokens to a CTA and CTAs to a cluster along K: whichever finishes first by a rough count of cycles,
-  // 330 or 5 a token for a block, 4000 to start and end, 1500 more for a cluster.
+  // Tokens to a CTA and CTAs to a cluster along K: whichever finishes first by a rough count of cycles, 500 or
+  // 4.3 a token for a block, 5000 to start and end, 2000 more for a cluster.
   int tokens = 128;
   long long best = -1;
-  for (int t = 32; t <= 128; t += 32)
+  for (int t = 32; t <= 256; t *= 2)
     for (int split = 1; split <= 8 && split <= f.blocks; split *= 2) {
       const long long units = row_tiles * ((p.M + t - 1) / t) * split;
       const long long waves = (units + sms - 1) / sms;
       if (split > 1 && waves > 1) continue;
-      const long long cost = waves * ((long long)((f.blocks + split - 1) / split) * (5 * t < 330 ? 330 : 5 * t) + 4000) +
-                             (split > 1 ? 1500 : 0);
+      const long long cost = waves * ((long long)((f.blocks + split - 1) / split) * (t <= 64 ? 400 : t * 43 / 10) + 5000) +
+                             (split > 1 ? 2000 : 0);
       if (best < 0 || cost < best) { best = cost; tokens = t; p.split = split; }
     }
+  if (getenv("W4T")) tokens = atoi(getenv("W4T"));
+  if (getenv("W4S")) p.split = atoi(getenv("W4S"));
   p.token_tiles = (p.M + tokens - 1) / tokens;
   p.stage_bytes = (tokens * 256 + 2 * f.chunk_bytes + 1023) / 1024 * 1024;
   p.vec = (reinterpret_cast<uintptr_t>(p.A) & 15) == 0 && p.lda % 8 == 0;

@@ -4,7 +4,10 @@ Tolerances: an output is rounded once to its type (half a step: 2^-8 of the valu
 fp16).  Before that it is a sum of K exact products in fp32, taken 16 at a time by the matrix
 instruction; each of the at most K / 16 + 64 additions that a term passes through may lose one unit
 in the last place of the running magnitude (2^-23; twice that is allowed for the instruction's
-truncation), so the sum is off by at most (K / 16 + 64) 2^-22 of the sum of the products' magnitudes."""
+truncation), so the sum is off by at most (K / 16 + 64) 2^-22 of the sum of the products' magnitudes.
+For more than 16 tokens the weights are first rounded to the type, as ``dequantize`` gives them (``held``),
+but in the SwiGLU form: there a weight is the sum of two 16-bit numbers, exactly, and twice as many products
+are added."""
 import pytest
 import torch
 
@@ -36,6 +39,11 @@ def activations(M, K, dtype, seed=1):
     return torch.randn((M, K), generator=g).to(dtype)
 
 
+def held(w, dtype, M):
+    """The weights that a product of M rows multiplies by."""
+    return w if M <= 16 else w.to(dtype).double()
+
+
 def slack(x, w):
     K = x.shape[1]
     return (K / 16 + 64) * 2.0 ** -22 * (x.double().abs() @ w.abs().t())
@@ -63,7 +71,7 @@ SHAPES = [
 @pytest.mark.parametrize("M,N,K,group,zeros,dtype", SHAPES)
 def test_product_matches_definition(M, N, K, group, zeros, dtype):
     codes, scales, zp, w = weights(N, K, group, zeros, dtype)
-    x = activations(M, K, dtype)
+    x, w = activations(M, K, dtype), held(w, dtype, M)
     W = pack(codes, scales, zp, zeros)
     C = torch.full((M, N), float("nan"), device=DEV, dtype=dtype)
     ops.w4_gemm(x.to(DEV), W, C)
@@ -97,7 +105,7 @@ def test_whole_numbers_are_exact(M):
 def test_row_strides_and_alignment(M, offset, stride):
     N, K = 144, 264
     codes, scales, zp, w = weights(N, K, 64, True, BF, seed=3)
-    x = activations(M, K, BF)
+    x, w = activations(M, K, BF), held(w, BF, M)
     big = torch.full((M * stride + 16,), float("nan"), dtype=BF, device=DEV)   # what lies around A is never used
     A = big[offset:offset + M * stride].view(M, stride)[:, :K]
     A.copy_(x)
@@ -112,7 +120,7 @@ def test_row_strides_and_alignment(M, offset, stride):
 def test_not_a_number_stays_in_its_row(M):
     N, K = 80, 384
     codes, scales, zp, w = weights(N, K, 128, False, HF, seed=4)
-    x = activations(M, K, HF)
+    x, w = activations(M, K, HF), held(w, HF, M)
     x[M // 2, 77] = float("nan")
     C = torch.zeros((M, N), device=DEV, dtype=HF)
     ops.w4_gemm(x.to(DEV), pack(codes, scales, zp, False), C)
@@ -138,7 +146,7 @@ def test_swiglu_matches_definition(M, I, K, group, zeros, dtype):
     x = activations(M, K, dtype)
     H = torch.full((M, I), float("nan"), device=DEV, dtype=dtype)
     ops.w4_gemm_swiglu(x.to(DEV), pack(codes, scales, zp, zeros, form="gate_up"), H)
-    y, t = x.double() @ w.t(), slack(x, w)
+    y, t = x.double() @ w.t(), 2 * slack(x, w)
     ref = orc.silu_mul(y)
     (gate, up), (tg, tu) = y.chunk(2, dim=1), t.chunk(2, dim=1)
     # silu changes by at most 1.1 times its argument's change; the fast exponential is good to
@@ -170,7 +178,7 @@ def test_swiglu_far_gates():
 ])
 def test_rotary_product_matches_definition(M, heads, rotated, D, rot, K, dtype, interleaved):
     codes, scales, zp, w = weights(heads * D, K, 64, True, dtype, seed=6)
-    x = activations(M, K, dtype)
+    x, w = activations(M, K, dtype), held(w, dtype, M)
     W = pack(codes, scales, zp, True, form="rotary", head_dim=D, rotary_dim=rot, rotated_heads=rotated,
              interleaved=interleaved)
     inv_freq, scale = ops.rotary_frequencies(rot, scaling="parts", factor=4.0, original_length=4096, device="cpu")
@@ -309,15 +317,16 @@ def test_mlp_of_a_few_tokens():
     with pytest.raises(RuntimeError):
         mlp.forward_tokens(torch.zeros((1, K), device=DEV, dtype=BF))
     mlp.load_weights_w4(wg.to(DEV), wu.to(DEV), wd.to(DEV), group=64)
-    deq = lambda w: orc.dequantize(*orc.quantize(w, 64, False, BF), 64)
     for m in (1, 3, 24):
+        deq = lambda w: orc.dequantize(*orc.quantize(w, 64, False, BF), 64)
+        down = held(deq(wd), BF, m)
         x = activations(m, K, BF, seed=m)
         y = mlp.forward_tokens(x.to(DEV)).cpu()
         gu = x.double() @ torch.cat((deq(wg), deq(wu))).t()
         h = orc.silu_mul(gu)
-        ref = h @ deq(wd).t()
+        ref = h @ down.t()
         # the activation is held in bf16 between the two products: half a step of each entry, plus that of y
-        tol = (2.0 ** -8 + 2.0 ** -12) * (h.abs() @ deq(wd).abs().t())
+        tol = (2.0 ** -8 + 2.0 ** -12) * (h.abs() @ down.abs().t())
         check(y, ref, tol, BF)
     mlp.free()
 
