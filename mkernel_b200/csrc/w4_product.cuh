@@ -82,6 +82,33 @@ __device__ __forceinline__ void w4_epilogue4(const W4Params& p, int strip, int p
       return;
     }
   }
+  if (p.epilogue == W4_EPI_ROTARY) {
+    // the four angles at once, so that their loads and sines overlap
+    T* row = static_cast<T*>(p.C) + (long long)token * p.ldc;
+    const int half = f.head_dim / 2, n_pairs = f.N / 2;
+    int index = strip * (kW4Strip / 2) + pair, head = index / half, at = index - head * half;
+    const long long position = rotary_position(p.rotary, token);
+    float2 v[4];
+    int n[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool rotated = head < f.rotated_heads && at < f.rotary_dim / 2;
+      const bool apart = rotated && !f.interleaved;
+      n[i][0] = index + i < n_pairs ? head * f.head_dim + (apart ? at : 2 * at) : -1;
+      n[i][1] = n[i][0] + (apart ? f.rotary_dim / 2 : 1);
+      v[i] = make_float2(a[i], b[i]);
+      if (rotated && n[i][0] >= 0)
+        v[i] = rotary_turn(a[i], b[i], rotary_cos_sin(position, __ldg(p.rotary.inv_freq + at), p.rotary.scale));
+      if (++at == half) { at = 0; ++head; }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n[i][0] >= 0) {
+        row[n[i][0]] = W4Traits<T>::from_float(v[i].x);
+        row[n[i][1]] = W4Traits<T>::from_float(v[i].y);
+      }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) w4_epilogue<T>(p, strip, pair + i, token, make_float2(a[i], b[i]));
 }

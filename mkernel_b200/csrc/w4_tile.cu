@@ -14,15 +14,16 @@
 // SwiGLU form two such sums are multiplied and it would be larger (2.1e-3), so there what the rounding left
 // (REST) is multiplied as well, and nothing is lost.
 //
-// Warps 0..7 decode (quadrant warp % 4 of the lanes, half warp / 4 of a block's 128 columns) and at the end
-// read the sums, warp 8 issues the MMAs, a thread of warp 9 (warps 9..11 where rows are not aligned)
-// copies a ring of stages (a block: codes of two strips, tokens in the 128-byte swizzle).  Decoders
-// run ahead of the tensor core by the operand buffers that tensor memory has room for.  Up to 64 tokens
-// two CTAs share an SM, which hides their starts, ends and waits behind one another.
+// Warps 0..15 decode, in two sets that take turns at the blocks of 128 columns (quadrant warp % 4 of the
+// lanes, half of the columns by warp / 4 % 2), and at the end read the sums; warps 16 and 17 issue the
+// MMAs; a thread each of warps 18 to 21 (all of them where rows are not aligned) copies a ring of stages (a
+// block: codes of two strips, tokens in the 128-byte swizzle; one thread for it all needs 0.33 us a block).  A block is little work and a long way: a wait for
+// a barrier alone takes some 150 cycles, issuing eight MMAs and a commit 350, whatever the tokens.  So what
+// bounds a narrow product is how many blocks are under way, and up to 128 tokens two warps issue, every
+// other block each, into sums of their own (one warp: 0.39 us a block at 64 tokens).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
-#include <cstdlib>
 #include <type_traits>
 
 #include "../../include/mkernel_b200.h"
@@ -31,21 +32,23 @@
 namespace mkb {
 
 constexpr int kTileRows = 2 * kW4Strip;
-constexpr int kTileCompute = 8;                    // warps
-constexpr int kTileLoaders = 3;
-constexpr int kTileThreads = (kTileCompute + 1 + kTileLoaders) * 32;
+constexpr int kTileCompute = 16;                   // warps, in two sets
+constexpr int kTileSet = 8;
+constexpr int kTileIssue = 2;
+constexpr int kTileLoaders = 4;
+constexpr int kTileThreads = (kTileCompute + kTileIssue + kTileLoaders) * 32;
 constexpr int kTileControl = 1024;                 // bytes before the ring
 constexpr int kTilePitch = kTileRows + 4;          // floats of a token's sums
 
-// Stages of the ring, operand buffers (64 columns of tensor memory beside the `tokens` of the sums) and CTAs
-// of an SM (227 KB and 512 columns).
+// Sums that the issuing warps add to, stages of the ring, and operand buffers (64 columns of tensor memory,
+// or 128): what 512 columns and 227 KB hold.
+__host__ __device__ constexpr int w4_tile_sums(int tokens) { return tokens <= 128 ? 2 : 1; }
 __host__ __device__ constexpr int w4_tile_stages(int tokens) {
-  return tokens == 32 ? 5 : tokens == 64 ? 4 : tokens == 128 ? 5 : 3;
+  return tokens == 32 ? 7 : tokens == 64 ? 6 : tokens == 128 ? 4 : 3;
 }
 __host__ __device__ constexpr int w4_tile_operands(int tokens, bool rest) {
-  return tokens <= 64 ? 3 : !rest ? 4 : tokens == 128 ? 3 : 2;
+  return !rest ? w4_tile_stages(tokens) : tokens <= 64 ? 3 : 2;
 }
-__host__ __device__ constexpr int w4_tile_ctas(int tokens, bool rest) { return tokens <= 64 && !rest ? 2 : 1; }
 
 struct TileWait {
   volatile uint32_t* abort;   // shared: some wait of this CTA has run out
@@ -79,14 +82,16 @@ __device__ __forceinline__ bool w4_wait_warp(const TileWait& c, uint32_t bar, ui
 }
 
 template <typename T, int TOKENS, int GROUP, bool REST>
-__global__ void __launch_bounds__(kTileThreads, w4_tile_ctas(TOKENS, REST))
+__global__ void __launch_bounds__(kTileThreads, 1)
     w4_tile_kernel(const __grid_constant__ W4Params p, const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int kTokens = TOKENS;
   constexpr int kStages = w4_tile_stages(kTokens);
   constexpr int kOperands = w4_tile_operands(kTokens, REST), kOperand = REST ? 128 : 64;   // columns of one
-  constexpr uint32_t kCols = kTokens + kOperand * kOperands <= 256 ? 256 : 512;
-  static_assert(kTokens + kOperand * kOperands <= 512 / w4_tile_ctas(TOKENS, REST), "tensor memory has 512 columns");
+  constexpr int kSums = w4_tile_sums(kTokens);
+  constexpr uint32_t kCols = 512;
+  static_assert(kSums * kTokens + kOperand * kOperands <= kCols, "tensor memory has 512 columns");
+  constexpr bool kOwn = kOperands < kStages;        // else an operand buffer is free when its stage is
   constexpr int kXHalf = kTokens * 128;             // bytes of 64 columns of the tokens
 
   const W4Form& f = p.form;
@@ -94,12 +99,12 @@ __global__ void __launch_bounds__(kTileThreads, w4_tile_ctas(TOKENS, REST))
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* const base_ptr = smem_raw + (base - raw);
-  // control words: full[5] empty[5] a_full[4] a_empty[4] done | tensor memory address, abort flag
+  // control words: full[7] empty[7] a_full[7] a_empty[3] done | tensor memory address, abort flag
   auto full = [&](int s) { return base + 8u * s; };
   auto empty = [&](int s) { return base + 64u + 8u * s; };
   auto a_full = [&](int i) { return base + 128u + 8u * i; };
-  auto a_empty = [&](int i) { return base + 160u + 8u * i; };
-  const uint32_t done = base + 192u;
+  auto a_empty = [&](int i) { return base + 192u + 8u * i; };
+  const uint32_t done = base + 216u;
   volatile uint32_t* const s_tmem = reinterpret_cast<volatile uint32_t*>(base_ptr + 224);
   volatile uint32_t* const s_abort = s_tmem + 1;
   const uint32_t ring = base + kTileControl;
@@ -118,14 +123,14 @@ __global__ void __launch_bounds__(kTileThreads, w4_tile_ctas(TOKENS, REST))
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(full(s), p.vec ? 1 : kTileLoaders * 32);
-      ptx::mbar_init(empty(s), kTileCompute + 1);
+      ptx::mbar_init(full(s), p.vec ? 2 : kTileLoaders * 32);
+      ptx::mbar_init(empty(s), kTileSet + 1);
     }
     for (int i = 0; i < kOperands; ++i) {
-      ptx::mbar_init(a_full(i), kTileCompute);
-      ptx::mbar_init(a_empty(i), 1);
+      ptx::mbar_init(a_full(i), kTileSet);
+      if (kOwn) ptx::mbar_init(a_empty(i), 1);
     }
-    ptx::mbar_init(done, 1);
+    ptx::mbar_init(done, kSums);
     *s_abort = 0u;
     ptx::fence_mbar_init();
   }
@@ -133,14 +138,14 @@ __global__ void __launch_bounds__(kTileThreads, w4_tile_ctas(TOKENS, REST))
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  const uint32_t tmem_a = tmem + kTokens;
+  const uint32_t tmem_a = tmem + kSums * kTokens;
   const TileWait wc{s_abort, p.wait_limit_ns};
 
   const size_t strip_bytes = (size_t)f.blocks * f.chunk_bytes;
   const uint8_t* const data = p.data + (size_t)strip0 * strip_bytes + (size_t)rank * f.chunk_bytes;
-  if (warp > kTileCompute) {
+  if (warp >= kTileCompute + kTileIssue) {
     // what is read first may be asked into L2 before the kernel ahead has finished
-    const int lt = threadIdx.x - (kTileCompute + 1) * 32;
+    const int lt = threadIdx.x - (kTileCompute + kTileIssue) * 32;
     for (int b = 0; b < kStages && b < blocks; ++b)
       for (int o = lt * 128; o < f.chunk_bytes; o += kTileLoaders * 32 * 128)
         for (int i = 0; i <= (int)two; ++i)
@@ -149,7 +154,7 @@ __global__ void __launch_bounds__(kTileThreads, w4_tile_ctas(TOKENS, REST))
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
-  const int quad = warp & 3, half = warp >> 2;
+  const int quad = warp & 3, half = warp >> 2 & 1;
   bool ok = true;
   if (warp < kTileCompute) {
     // ---------------- decode ----------------
@@ -161,10 +166,9 @@ __global__ void __launch_bounds__(kTileThreads, w4_tile_ctas(TOKENS, REST))
     const int scales_at = kTokens * 256 + strip * f.chunk_bytes + kW4CodeBytes + g * 16 + tile0 * 4 +
                           (half * 64 / GROUP) * 128;
     const uint32_t a_at = tmem_a + ((uint32_t)(quad * 32) << 16) + half * 32;
-    int s = 0, operand = 0;
-    uint32_t parity = 0, a_parity = 1;   // a fresh barrier has "completed" the phase before its first
-    for (int b = 0; b < blocks; ++b) {
-      ok = w4_wait_warp(wc, full(s), parity);
+    for (int b = warp / kTileSet; b < blocks; b += 2) {
+      const int s = b % kStages, operand = b % kOperands;
+      ok = w4_wait_warp(wc, full(s), (b / kStages) & 1);
       if (!ok) break;
       const uint8_t* stage = ring_ptr + s * p.stage_bytes;
       uint4 codes[2];
@@ -177,8 +181,10 @@ __global__ void __launch_bounds__(kTileThreads, w4_tile_ctas(TOKENS, REST))
         zeros[i] = make_uint2(W4Traits<T>::kMinusEight, W4Traits<T>::kMinusEight);
         if (f.zeros) zeros[i] = *reinterpret_cast<const uint2*>(stage + scales_at + (kGroups + i) * 128);
       }
-      ok = w4_wait_warp(wc, a_empty(operand), a_parity);
-      if (!ok) break;
+      if (kOwn && b >= kOperands) {
+        ok = w4_wait_warp(wc, a_empty(operand), (b / kOperands - 1) & 1);
+        if (!ok) break;
+      }
       ptx::tc_fence_after();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -208,57 +214,57 @@ __global__ void __launch_bounds__(kTileThreads, w4_tile_ctas(TOKENS, REST))
         ptx::mbar_arrive(a_full(operand));
         ptx::mbar_arrive(empty(s));
       }
-      if (++s == kStages) { s = 0; parity ^= 1; }
-      if (++operand == kOperands) { operand = 0; a_parity ^= 1; }
     }
     ok = ok && w4_wait_warp(wc, done, 0);
-  } else if (warp == kTileCompute) {
+  } else if (warp < kTileCompute + kTileIssue) {
     // ---------------- MMA issue: the whole warp, one lane elected inside the statement ----------------
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t idesc = (1u << 4) | (kType << 7) | (kType << 10) | ((kTokens >> 3) << 17) | ((128u >> 4) << 24);
     const uint32_t desc_hi = static_cast<uint32_t>(ptx::make_smem_desc_sw128(0, 16, 1024) >> 32);
     const uint32_t b_lo0 = static_cast<uint32_t>(ptx::make_smem_desc_sw128(ring, 16, 1024));
-    int s = 0, operand = 0;
-    uint32_t a_parity = 0;
-    for (int b = 0; b < blocks; ++b) {
+    const int me = warp - kTileCompute;
+    const uint32_t d = tmem + me * kTokens;
+    for (int b = me; me < kSums && b < blocks; b += kSums) {
+      const int s = b % kStages, operand = b % kOperands;
       // The tokens need no wait of their own: who decoded the block has waited for them.
-      ok = w4_wait_warp(wc, a_full(operand), a_parity);
+      ok = w4_wait_warp(wc, a_full(operand), (b / kOperands) & 1);
       if (!ok) break;
       if (!p.vec) ptx::fence_proxy_async();   // the tokens were written by ordinary stores
       ptx::tc_fence_after();
       const uint32_t a = tmem_a + operand * kOperand, b_lo = b_lo0 + s * (p.stage_bytes >> 4);
-      ptx::umma_ts<4>(tmem, a, b_lo, desc_hi, idesc, b > 0 ? 1u : 0u);
-      ptx::umma_ts<4>(tmem, a + 32, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
+      ptx::umma_ts<4>(d, a, b_lo, desc_hi, idesc, b >= kSums ? 1u : 0u);
+      ptx::umma_ts<4>(d, a + 32, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
       if (REST) {
-        ptx::umma_ts<4>(tmem, a + 64, b_lo, desc_hi, idesc, 1);
-        ptx::umma_ts<4>(tmem, a + 96, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
+        ptx::umma_ts<4>(d, a + 64, b_lo, desc_hi, idesc, 1);
+        ptx::umma_ts<4>(d, a + 96, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
       }
-      ptx::umma_commit_elect<1>(a_empty(operand), 0);
+      if (kOwn) ptx::umma_commit_elect<1>(a_empty(operand), 0);
       ptx::umma_commit_elect<1>(empty(s), 0);
-      if (++s == kStages) s = 0;
-      if (++operand == kOperands) { operand = 0; a_parity ^= 1; }
     }
-    if (ok) ptx::umma_commit_elect<1>(done, 0);
+    if (ok && me < kSums) ptx::umma_commit_elect<1>(done, 0);
   } else if (p.vec) {
-    // ---------------- copies: one thread, tokens by tensor copies, codes by plain ones ----------------
-    if (warp == kTileCompute + 1 && lane == 0) {
-      const uint32_t tx = kTokens * 256 + f.chunk_bytes * (two ? 2 : 1);
-      for (int b = 0; b < blocks; ++b) {
-        const int s = b % kStages;
-        if (b >= kStages && !w4_wait(wc, empty(s), (b / kStages - 1) & 1)) break;
-        const uint32_t stage = ring + s * p.stage_bytes;
-        const uint8_t* chunk = data + (size_t)b * p.split * f.chunk_bytes;
+    // ---------------- copies: two threads for the codes, two for the tokens (tensor copies) ----------------
+    const int me = warp - kTileCompute - kTileIssue;
+    const bool tokens = me >= 2;
+    const uint32_t tx = tokens ? kTokens * 256 : f.chunk_bytes * (two ? 2 : 1);
+    for (int b = me & 1; lane == 0 && b < blocks; b += 2) {
+      const int s = b % kStages;
+      if (b >= kStages && !w4_wait(wc, empty(s), (b / kStages - 1) & 1)) break;
+      const uint32_t stage = ring + s * p.stage_bytes;
+      ptx::mbar_expect_tx(full(s), tx);
+      if (tokens) {
         const int k = (rank + b * p.split) * kW4Block;
-        ptx::mbar_expect_tx(full(s), tx);
-        ptx::bulk_g2s(stage + kTokens * 256, chunk, f.chunk_bytes, full(s));
-        if (two) ptx::bulk_g2s(stage + kTokens * 256 + f.chunk_bytes, chunk + strip_bytes, f.chunk_bytes, full(s));
         ptx::tma_load_2d(stage, &map, full(s), k, token0);
         ptx::tma_load_2d(stage + kXHalf, &map, full(s), k + 64, token0);
+      } else {
+        const uint8_t* chunk = data + (size_t)b * p.split * f.chunk_bytes;
+        ptx::bulk_g2s(stage + kTokens * 256, chunk, f.chunk_bytes, full(s));
+        if (two) ptx::bulk_g2s(stage + kTokens * 256 + f.chunk_bytes, chunk + strip_bytes, f.chunk_bytes, full(s));
       }
     }
   } else {
     // ---------------- copies where rows of tokens start on no 16 bytes ----------------
-    const int lt = threadIdx.x - (kTileCompute + 1) * 32, lw = lt >> 5;
+    const int lt = threadIdx.x - (kTileCompute + kTileIssue) * 32, lw = lt >> 5;
     const int pieces = f.chunk_bytes / 16 * (two ? 2 : 1);
     // lane = 4 columns of a token, in the 128-byte swizzle
     const uint32_t unit = lane >> 1 & 7, low = (lane >> 4) * kXHalf + (lane & 1) * 8;
@@ -298,14 +304,23 @@ __global__ void __launch_bounds__(kTileThreads, w4_tile_ctas(TOKENS, REST))
   float* const red = reinterpret_cast<float*>(ring_ptr);
   if (warp < kTileCompute) {
     ptx::tc_fence_after();
+    constexpr int kEach = kTokens / 4, kBatch = kEach < 16 ? 8 : 16;
+    const int c0 = (warp >> 2) * kEach;
 #pragma unroll
-    for (int c = 0; c < kTokens / 2; c += 16) {
-      float d[16];
-      ptx::tmem_ld<16>(tmem + ((uint32_t)(quad * 32) << 16) + half * (kTokens / 2) + c, d);
+    for (int c = 0; c < kEach; c += kBatch) {
+      float d[kBatch];
+      ptx::tmem_ld<kBatch>(tmem + ((uint32_t)(quad * 32) << 16) + c0 + c, d);
       ptx::tmem_ld_wait();
+      if (kSums == 2 && blocks > 1) {   // the second sums are of the blocks 1, 3, ...
+        float e[kBatch];
+        ptx::tmem_ld<kBatch>(tmem + ((uint32_t)(quad * 32) << 16) + kTokens + c0 + c, e);
+        ptx::tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        red[(half * (kTokens / 2) + c + i) * kTilePitch + quad * 32 + lane] = ok ? d[i] : __int_as_float(0x7fc00000);
+        for (int i = 0; i < kBatch; ++i) d[i] += e[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        red[(c0 + c + i) * kTilePitch + quad * 32 + lane] = ok ? d[i] : __int_as_float(0x7fc00000);
     }
     ptx::tc_fence_before();
   }
@@ -398,21 +413,22 @@ static int w4_tile_map(CUtensorMap* map, const W4Params& p, int dtype, int token
 int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
   const W4Form& f = p.form;
   const long long row_tiles = (f.strips + 1) / 2;
-  // Tokens to a CTA and CTAs to a cluster along K: whichever finishes first by a rough count of cycles, 500 or
-  // 4.3 a token for a block, 5000 to start and end, 2000 more for a cluster.
+  // Tokens to a CTA and CTAs to a cluster along K: whichever finishes first by what a block and a start and end
+  // take in ns (measured at 32, 64, 128 and 256 tokens; 1.5 us more for a cluster of two).
+  const bool rest = p.epilogue == W4_EPI_SWIGLU;
+  const int block_ns[2][4] = {{280, 290, 370, 500}, {400, 540, 800, 1250}}, ends_ns[4] = {3000, 3000, 4500, 8000};
   int tokens = 128;
   long long best = -1;
-  for (int t = 32; t <= 256; t *= 2)
+  for (int i = 0; i < 4; ++i)
     for (int split = 1; split <= 8 && split <= f.blocks; split *= 2) {
+      const int t = 32 << i;
       const long long units = row_tiles * ((p.M + t - 1) / t) * split;
       const long long waves = (units + sms - 1) / sms;
       if (split > 1 && waves > 1) continue;
-      const long long cost = waves * ((long long)((f.blocks + split - 1) / split) * (t <= 64 ? 400 : t * 43 / 10) + 5000) +
-                             (split > 1 ? 2000 : 0);
+      const long long each = (long long)((f.blocks + split - 1) / split) * block_ns[rest][i] + ends_ns[i];
+      const long long cost = waves * each + (split > 1 ? 750 * split : 0);
       if (best < 0 || cost < best) { best = cost; tokens = t; p.split = split; }
     }
-  if (getenv("W4T")) tokens = atoi(getenv("W4T"));
-  if (getenv("W4S")) p.split = atoi(getenv("W4S"));
   p.token_tiles = (p.M + tokens - 1) / tokens;
   p.stage_bytes = (tokens * 256 + 2 * f.chunk_bytes + 1023) / 1024 * 1024;
   p.vec = (reinterpret_cast<uintptr_t>(p.A) & 15) == 0 && p.lda % 8 == 0;
