@@ -40,15 +40,16 @@ constexpr int kTileThreads = (kTileCompute + kTileIssue + kTileLoaders) * 32;
 constexpr int kTileControl = 1024;                 // bytes before the ring
 constexpr int kTilePitch = kTileRows + 4;          // floats of a token's sums
 
-// Sums that the issuing warps add to, stages of the ring, and operand buffers (64 columns of tensor memory,
-// or 128): what 512 columns and 227 KB hold.
-__host__ __device__ constexpr int w4_tile_sums(int tokens) { return tokens <= 128 ? 2 : 1; }
-__host__ __device__ constexpr int w4_tile_stages(int tokens) {
-  return tokens == 32 ? 7 : tokens == 64 ? 6 : tokens == 128 ? 4 : 3;
-}
-__host__ __device__ constexpr int w4_tile_operands(int tokens, bool rest) {
-  return !rest ? w4_tile_stages(tokens) : tokens <= 64 ? 3 : 2;
-}
+// Up to 128 tokens two of everybody (sets of decoding warps, issuing warps with sums of their own, copying
+// threads) take turns at the blocks; for 256, whose MMAs are long enough to hide the rest, all decoding
+// warps share every block, and one warp issues.
+// Who takes turns sees every other phase of a barrier only if the number of stages (or operand buffers) is odd,
+// and could then take the phase before the last for the last: both numbers are multiples of the turns.
+__host__ __device__ constexpr int w4_tile_turns(int tokens) { return tokens <= 128 ? 2 : 1; }
+// Stages of the ring, and operand buffers (64 columns of tensor memory, or 128): what 227 KB and, beside the
+// sums, 512 columns hold.
+__host__ __device__ constexpr int w4_tile_stages(int tokens) { return tokens <= 64 ? 6 : tokens == 128 ? 4 : 3; }
+__host__ __device__ constexpr int w4_tile_operands(int tokens, bool rest) { return rest ? 2 : w4_tile_stages(tokens); }
 
 struct TileWait {
   volatile uint32_t* abort;   // shared: some wait of this CTA has run out
@@ -88,7 +89,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   constexpr int kTokens = TOKENS;
   constexpr int kStages = w4_tile_stages(kTokens);
   constexpr int kOperands = w4_tile_operands(kTokens, REST), kOperand = REST ? 128 : 64;   // columns of one
-  constexpr int kSums = w4_tile_sums(kTokens);
+  constexpr int kTurns = w4_tile_turns(kTokens), kSums = kTurns;
+  static_assert(kStages % kTurns == 0 && kOperands % kTurns == 0, "no phase of a barrier is skipped");
   constexpr uint32_t kCols = 512;
   static_assert(kSums * kTokens + kOperand * kOperands <= kCols, "tensor memory has 512 columns");
   constexpr bool kOwn = kOperands < kStages;        // else an operand buffer is free when its stage is
@@ -99,7 +101,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* const base_ptr = smem_raw + (base - raw);
-  // control words: full[7] empty[7] a_full[7] a_empty[3] done | tensor memory address, abort flag
+  // control words: full[6] empty[6] a_full[6] a_empty[2] done | tensor memory address, abort flag
   auto full = [&](int s) { return base + 8u * s; };
   auto empty = [&](int s) { return base + 64u + 8u * s; };
   auto a_full = [&](int i) { return base + 128u + 8u * i; };
@@ -124,10 +126,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       ptx::mbar_init(full(s), p.vec ? 2 : kTileLoaders * 32);
-      ptx::mbar_init(empty(s), kTileSet + 1);
+      ptx::mbar_init(empty(s), kTileCompute / kTurns + 1);
     }
     for (int i = 0; i < kOperands; ++i) {
-      ptx::mbar_init(a_full(i), kTileSet);
+      ptx::mbar_init(a_full(i), kTileCompute / kTurns);
       if (kOwn) ptx::mbar_init(a_empty(i), 1);
     }
     ptx::mbar_init(done, kSums);
@@ -159,41 +161,45 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (warp < kTileCompute) {
     // ---------------- decode ----------------
     const int g = lane >> 2;
-    const int strip = quad >> 1, tile0 = (quad & 1) * 2;
+    const int strip = quad >> 1;
     constexpr int kGroups = kW4Block / GROUP;
     // of a stage: this lane's codes of two tiles, and the scales and zero points of its rows there
+    constexpr int kTiles = kTurns;         // of the quadrant's two that a warp decodes
+    const int tile0 = (quad & 1) * 2 + (kTiles == 1 ? warp / kTileSet : 0);
     const int codes_at = kTokens * 256 + strip * f.chunk_bytes + ((half * 4 + tile0) * 32 + lane) * 16;
     const int scales_at = kTokens * 256 + strip * f.chunk_bytes + kW4CodeBytes + g * 16 + tile0 * 4 +
                           (half * 64 / GROUP) * 128;
-    const uint32_t a_at = tmem_a + ((uint32_t)(quad * 32) << 16) + half * 32;
-    for (int b = warp / kTileSet; b < blocks; b += 2) {
+    const uint32_t a_at = tmem_a + ((uint32_t)(strip * 64 + tile0 * 16) << 16) + half * 32;
+    for (int b = kTurns == 2 ? warp / kTileSet : 0; b < blocks; b += kTurns) {
       const int s = b % kStages, operand = b % kOperands;
       ok = w4_wait_warp(wc, full(s), (b / kStages) & 1);
       if (!ok) break;
       const uint8_t* stage = ring_ptr + s * p.stage_bytes;
-      uint4 codes[2];
-      uint2 scales[GROUP == 32 ? 2 : 1], zeros[GROUP == 32 ? 2 : 1];
+      uint4 codes[kTiles];
+      uint32_t scales[GROUP == 32 ? 2 : 1][kTiles], zeros[GROUP == 32 ? 2 : 1][kTiles];   // of rows g, g + 8
 #pragma unroll
-      for (int i = 0; i < 2; ++i) codes[i] = *reinterpret_cast<const uint4*>(stage + codes_at + i * 512);
+      for (int i = 0; i < kTiles; ++i) codes[i] = *reinterpret_cast<const uint4*>(stage + codes_at + i * 512);
 #pragma unroll
-      for (int i = 0; i < (GROUP == 32 ? 2 : 1); ++i) {
-        scales[i] = *reinterpret_cast<const uint2*>(stage + scales_at + i * 128);
-        zeros[i] = make_uint2(W4Traits<T>::kMinusEight, W4Traits<T>::kMinusEight);
-        if (f.zeros) zeros[i] = *reinterpret_cast<const uint2*>(stage + scales_at + (kGroups + i) * 128);
-      }
+      for (int gi = 0; gi < (GROUP == 32 ? 2 : 1); ++gi)
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          const uint8_t* from = stage + scales_at + gi * 128 + i * 4;
+          scales[gi][i] = *reinterpret_cast<const uint32_t*>(from);
+          zeros[gi][i] = f.zeros ? *reinterpret_cast<const uint32_t*>(from + kGroups * 128) : W4Traits<T>::kMinusEight;
+        }
       if (kOwn && b >= kOperands) {
         ok = w4_wait_warp(wc, a_empty(operand), (b / kOperands - 1) & 1);
         if (!ok) break;
       }
       ptx::tc_fence_after();
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < kTiles; ++i) {
         const uint32_t words[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
         uint32_t r[16], rest[16];
 #pragma unroll
         for (int v = 0; v < 4; v += 2) {
           const int gi = GROUP == 32 ? v / 2 : 0;
-          const uint32_t sc = i ? scales[gi].y : scales[gi].x, z = i ? zeros[gi].y : zeros[gi].x;
+          const uint32_t sc = scales[gi][i], z = zeros[gi][i];
           const W4Round<T> weights(__byte_perm(z, 0, 0x1010), __byte_perm(z, 0, 0x3232), __byte_perm(sc, 0, 0x1010),
                                    __byte_perm(sc, 0, 0x3232));
 #pragma unroll
@@ -245,9 +251,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   } else if (p.vec) {
     // ---------------- copies: two threads for the codes, two for the tokens (tensor copies) ----------------
     const int me = warp - kTileCompute - kTileIssue;
-    const bool tokens = me >= 2;
+    const bool tokens = me >= 2, active = lane == 0 && (me & 1) < kTurns;
     const uint32_t tx = tokens ? kTokens * 256 : f.chunk_bytes * (two ? 2 : 1);
-    for (int b = me & 1; lane == 0 && b < blocks; b += 2) {
+    for (int b = me & 1; active && b < blocks; b += kTurns) {
       const int s = b % kStages;
       if (b >= kStages && !w4_wait(wc, empty(s), (b / kStages - 1) & 1)) break;
       const uint32_t stage = ring + s * p.stage_bytes;
