@@ -11,105 +11,111 @@
 
 namespace mkb {
 
-// Division of an int below 2^31 by a fixed positive int, as a multiplication (Granlund and Montgomery).
-struct FastDiv {
-  uint32_t d, mul, shift;
-  FastDiv() = default;
-  explicit FastDiv(int divisor) : d((uint32_t)divisor), shift(0) {
-    while ((1ull << shift) < d) ++shift;
-    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
-};
-
 struct RotaryParams {
   const void* x;
   void* y;
   long long x_row, x_head, y_row, y_head;   // strides in elements
   long long rows;
   int heads, head_dim, rotary_dim;
-  int turned;              // slots of a head that turn; the others copy
+  int slots, turned;       // of a head; the first `turned` turn, the others copy
+  int per_row;             // slots of a row
   int rows_each;           // rows of a CTA
-  FastDiv slots, per_row;  // slots of a head; of a row
+  int rows_abreast;        // rows that its threads take at once
   float sign;
   RotaryArgs rotary;
 };
 
-constexpr int kRotaryThreads = 256;
-constexpr int kRotaryAhead = 2;      // slots whose loads a thread has in flight
+constexpr int kRotaryThreads = 512;  // at most
+constexpr int kRotaryAhead = 2;      // rows whose loads a thread has in flight
 constexpr int kRotaryAngles = 2048;  // of a CTA (16 KB of shared memory)
 
 template <typename T, int P> struct alignas(sizeof(T) * P) RotaryVec { T v[P]; };
 
+// Written as data that passes through: 8192 rows of 40 heads of 128 take 31 us so, 35 without.
+template <typename T, int P>
+__device__ __forceinline__ void rotary_store(T* to, const RotaryVec<T, P>& v) {
+  if constexpr (sizeof(v) == 16) __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&v));
+  else *reinterpret_cast<RotaryVec<T, P>*>(to) = v;
+}
+
 // A slot is P pairs of features of a head: vector 0 and vector 1 of P elements each, which are the
-// first and second features of the pairs, or, interleaved, the pairs one after another.  A CTA has a few
-// whole rows.  Its threads ask for their first slots' features, then work out the rows' angles, each
-// once (sine and cosine, in 64 bits up to the turn, cost as much as turning several heads), and
-// find them in shared memory for every head.
+// first and second features of the pairs, or, interleaved, the pairs one after another.  A CTA has some
+// whole rows; a thread has one slot of one head and goes down the rows, several loads ahead, so that
+// nothing but pointers changes from one to the next.  The rows' angles are worked out once by all
+// threads (sine and cosine, in 64 bits up to the turn, cost as much as turning several heads) while the
+// first rows are on their way, and found in shared memory for every head.
 template <typename T, int P, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, 2) rotary_kernel(const __grid_constant__ RotaryParams p) {
   using Vec = RotaryVec<T, P>;
   __shared__ __align__(16) float2 angles[kRotaryAngles];
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const long long row0 = (long long)blockIdx.x * p.rows_each;
   const int rows = (int)min((long long)p.rows_each, p.rows - row0);
-  const uint32_t items = rows * p.per_row.d;
   const int pairs = p.rotary_dim / 2;
+  const int abreast = p.rows_abreast;
 
-  struct Item { const T* x; T* y; int a, b, angle; bool turns, second; };
-  auto item = [&](uint32_t e) {
-    const uint32_t r = p.per_row.div(e), in_row = e - r * p.per_row.d;
-    const uint32_t h = p.slots.div(in_row);
-    const int slot = (int)(in_row - h * p.slots.d);
-    Item i;
-    i.x = static_cast<const T*>(p.x) + (row0 + r) * p.x_row + h * p.x_head;
-    i.y = static_cast<T*>(p.y) + (row0 + r) * p.y_row + h * p.y_head;
-    i.turns = slot < p.turned;
-    i.a = !i.turns ? p.rotary_dim + (slot - p.turned) * 2 * P : INTERLEAVED ? slot * 2 * P : slot * P;
-    i.b = i.turns && !INTERLEAVED ? i.a + pairs : i.a + P;
-    i.second = i.b < p.head_dim;        // the last vector of a head's copied features may not exist
-    i.angle = (int)r * pairs + slot * P;
-    return i;
+  auto work_out_angles = [&] {
+    for (int e = threadIdx.x; e < rows * pairs; e += blockDim.x) {
+      const int r = rows == 1 ? 0 : e / pairs;
+      float2 cs = rotary_cos_sin(rotary_position(p.rotary, row0 + r), __ldg(p.rotary.inv_freq + (e - r * pairs)),
+                                 p.rotary.scale);
+      cs.y *= p.sign;
+      angles[e] = cs;
+    }
+    __syncthreads();
   };
-  auto load = [&](uint32_t e, Vec& u, Vec& v) {
-    if (e >= items) return;
-    const Item i = item(e);
-    u = *reinterpret_cast<const Vec*>(i.x + i.a);
-    if (i.second) v = *reinterpret_cast<const Vec*>(i.x + i.b);
-  };
-
-  Vec u[kRotaryAhead], v[kRotaryAhead];
-#pragma unroll
-  for (int c = 0; c < kRotaryAhead; ++c) load(threadIdx.x + c * kRotaryThreads, u[c], v[c]);
-  for (int e = threadIdx.x; e < rows * pairs; e += kRotaryThreads) {
-    const int r = rows == 1 ? 0 : e / pairs;
-    float2 cs = rotary_cos_sin(rotary_position(p.rotary, row0 + r), __ldg(p.rotary.inv_freq + (e - r * pairs)),
-                               p.rotary.scale);
-    cs.y *= p.sign;
-    angles[e] = cs;
-  }
-  __syncthreads();
-  for (uint32_t e0 = threadIdx.x; e0 < items; e0 += kRotaryAhead * kRotaryThreads) {
-#pragma unroll
-    for (int c = 0; c < kRotaryAhead; ++c) {
-      const uint32_t e = e0 + c * kRotaryThreads;
-      if (e >= items) break;
-      const Item i = item(e);
-      if (i.turns) {
-#pragma unroll
-        for (int k = 0; k < P; ++k) {
-          // pair k: elements k of both vectors, or elements 2 k and 2 k + 1 of the two in a row
-          T& first = INTERLEAVED ? (2 * k < P ? u[c].v[2 * k % P] : v[c].v[2 * k % P]) : u[c].v[k];
-          T& second = INTERLEAVED ? (2 * k + 1 < P ? u[c].v[(2 * k + 1) % P] : v[c].v[(2 * k + 1) % P]) : v[c].v[k];
-          const float2 r = rotary_turn((float)first, (float)second, angles[i.angle + k]);
-          first = (T)r.x;
-          second = (T)r.y;
-        }
+  const int first_row = abreast == 1 ? 0 : threadIdx.x / p.per_row;
+  bool have_angles = false;
+  for (int in_row = threadIdx.x - first_row * p.per_row; in_row < p.per_row || !have_angles; in_row += blockDim.x) {
+    const bool mine = in_row < p.per_row && first_row < abreast;   // the last warp may have threads to spare
+    const int h = in_row / p.slots, slot = in_row - h * p.slots;
+    const bool turns = slot < p.turned;
+    const int a = !turns ? p.rotary_dim + (slot - p.turned) * 2 * P : INTERLEAVED ? slot * 2 * P : slot * P;
+    const int b = turns && !INTERLEAVED ? a + pairs : a + P;
+    const bool second = b < p.head_dim;   // the last vector of a head's copied features may not exist
+    const T* x = static_cast<const T*>(p.x) + (row0 + first_row) * p.x_row + h * p.x_head;
+    T* y = static_cast<T*>(p.y) + (row0 + first_row) * p.y_row + h * p.y_head;
+    const long long x_step = abreast * p.x_row, y_step = abreast * p.y_row;
+    Vec u[kRotaryAhead], v[kRotaryAhead];
+    int next = first_row;                 // row of the next load
+    auto load = [&](int c) {
+      if (mine && next < rows) {
+        u[c] = *reinterpret_cast<const Vec*>(x + a);
+        if (second) v[c] = *reinterpret_cast<const Vec*>(x + b);
       }
-      *reinterpret_cast<Vec*>(i.y + i.a) = u[c];
-      if (i.second) *reinterpret_cast<Vec*>(i.y + i.b) = v[c];
-      load(e + kRotaryAhead * kRotaryThreads, u[c], v[c]);
+      x += x_step;
+      next += abreast;
+    };
+#pragma unroll
+    for (int c = 0; c < kRotaryAhead; ++c) load(c);
+    if (!have_angles) {
+      work_out_angles();
+      have_angles = true;
+    }
+    if (!mine) continue;
+    for (int r0 = first_row; r0 < rows; r0 += kRotaryAhead * abreast) {
+#pragma unroll
+      for (int c = 0; c < kRotaryAhead; ++c) {
+        const int r = r0 + c * abreast;
+        if (r >= rows) break;
+        if (turns) {
+          const float2* cs = angles + r * pairs + slot * P;
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            // pair k: elements k of both vectors, or elements 2 k and 2 k + 1 of the two in a row
+            T& first = INTERLEAVED ? (2 * k < P ? u[c].v[2 * k % P] : v[c].v[2 * k % P]) : u[c].v[k];
+            T& other = INTERLEAVED ? (2 * k + 1 < P ? u[c].v[(2 * k + 1) % P] : v[c].v[(2 * k + 1) % P]) : v[c].v[k];
+            const float2 t = rotary_turn((float)first, (float)other, cs[k]);
+            first = (T)t.x;
+            other = (T)t.y;
+          }
+        }
+        rotary_store(y + a, u[c]);
+        if (second) rotary_store(y + b, v[c]);
+        y += y_step;
+        load(c);
+      }
     }
   }
 }
@@ -117,27 +123,32 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
 template <typename T, int P>
 static int rotary_launch(RotaryParams& p, bool interleaved, bool in_place, int sms, cudaStream_t stream) {
   p.turned = p.rotary_dim / 2 / P;
-  const int slots = p.turned + (in_place ? 0 : (p.head_dim - p.rotary_dim + 2 * P - 1) / (2 * P));
-  const long long per_row = (long long)p.heads * slots;
+  p.slots = p.turned + (in_place ? 0 : (p.head_dim - p.rotary_dim + 2 * P - 1) / (2 * P));
+  const long long per_row = (long long)p.heads * p.slots;
   if (per_row > 1 << 30 || p.rotary_dim / 2 > kRotaryAngles)
     return set_error(MK_ERR_INVALID, "mk_rotary: heads of %d (%d turned) features, %d to a row, are too many", p.head_dim,
                      p.rotary_dim, p.heads);
-  // Rows of a CTA: enough to give every thread its first slots, and so many that one wave of four CTAs to an
-  // SM has them all (8192 rows of 40 heads of 128: 54 us with a CTA to each row, whose latency comes
-  // back with every wave); their angles must fit shared memory.
-  long long rows_each = kRotaryAhead * kRotaryThreads / per_row;
-  const long long wave = (p.rows + 4 * sms - 1) / (4 * sms);
-  if (rows_each < wave) rows_each = wave;
-  if (rows_each > kRotaryAngles / (p.rotary_dim / 2)) rows_each = kRotaryAngles / (p.rotary_dim / 2);
-  if (rows_each < 1) rows_each = 1;
+  p.per_row = (int)per_row;
+  // Rows abreast up to about 256 threads; rows of a CTA such that one wave of 1024 threads to an SM has them
+  // all (with a CTA to each row its latency comes back with every wave: 8192 rows of 40 heads of 128 took 54
+  // us, 4097 rows of 9 heads 7.7 with 600 threads), within what their angles leave room for.
+  const int room = kRotaryAngles / (p.rotary_dim / 2);
+  int abreast = per_row >= 256 ? 1 : (int)(256 / per_row);
+  if (abreast > room) abreast = room;
+  if (abreast > p.rows) abreast = (int)p.rows;
+  long long threads = (abreast * per_row + 31) / 32 * 32;
+  if (threads > kRotaryThreads) threads = kRotaryThreads;
+  const long long wave = 1024 / threads * sms;
+  long long rows_each = (p.rows + wave - 1) / wave;
+  rows_each = (rows_each + abreast - 1) / abreast * abreast;
+  if (rows_each > room) rows_each = room;
+  p.rows_abreast = abreast;
   p.rows_each = (int)rows_each;
-  p.slots = FastDiv(slots);
-  p.per_row = FastDiv((int)per_row);
   const long long blocks = (p.rows + rows_each - 1) / rows_each;
   if (blocks > 0x7fffffffLL) return set_error(MK_ERR_INVALID, "mk_rotary: %lld rows are too many", p.rows);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks, 1, 1);
-  cfg.blockDim = dim3(kRotaryThreads, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

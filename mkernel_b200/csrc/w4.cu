@@ -15,11 +15,11 @@ namespace mkb {
 // ------------------------------------------------------------------------------------------
 // laying the weights out
 // ------------------------------------------------------------------------------------------
-// The unit of all three kernels is 16 consecutive columns of a pair of rows: one word of the layout for
-// each of four lanes.  Four neighbouring threads have the 64 columns of a half, and after exchanging
-// words (w4_transpose) each has the 16 bytes of one lane.  A chunk has as many units as a CTA has
-// threads, a unit is read and written with 16-byte accesses, a group is reduced by shuffles, and
-// nothing passes through shared memory.
+// A thread of all three kernels has a pair of rows and, of a half of a block, 8 consecutive columns and the 8
+// that lie 32 further: 16-byte accesses, four neighbouring threads covering 64 bytes in order.  That is
+// two words of the layout for each of two lanes; after exchanging one of each piece with its neighbour
+// (w4_exchange) it has the 16 bytes of one lane.  A group is reduced by shuffles, and nothing passes
+// through shared memory.
 constexpr int kW4PackThreads = 256;
 
 struct W4PackParams {
@@ -35,27 +35,24 @@ struct W4PackParams {
   int vec;   // 16-byte accesses to eight columns are aligned
 };
 
-struct W4Unit { int pair, col; };   // columns col .. col + 15 of the block
-__device__ __forceinline__ W4Unit w4_unit() { return {(int)threadIdx.x >> 3, ((int)threadIdx.x & 7) * 16}; }
+struct W4Unit { int pair, col; };   // columns col .. col + 7 and col + 32 .. col + 39 of the block
+__device__ __forceinline__ W4Unit w4_unit() {
+  const int t = threadIdx.x & 3;
+  return {(int)threadIdx.x >> 3, (threadIdx.x >> 2 & 1) * 64 + (t & 1) * 16 + (t >> 1) * 8};
+}
 // Place of the lane that the unit's thread has after the exchange: t = thread % 4.
 __device__ __forceinline__ int w4_unit_offset(const W4Unit& u) {
-  return (((u.col >> 6) * 4 + (u.pair >> 3)) * 32 + (u.pair & 7) * 4 + (u.col >> 4 & 3)) * 16;
+  return (((u.col >> 6) * 4 + (u.pair >> 3)) * 32 + (u.pair & 7) * 4 + (threadIdx.x & 3)) * 16;
 }
 
-// Word i of thread j for word j of thread i, among four neighbouring threads.
-__device__ __forceinline__ void w4_transpose(uint32_t (&w)[4]) {
-  const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
+// Between the words of a thread's columns, {first four, last four} of both pieces, and the words of its lane.
+__device__ __forceinline__ void w4_exchange(uint32_t (&w)[4]) {
+  const bool odd = threadIdx.x & 1;
 #pragma unroll
-  for (int i = 0; i < 4; i += 2) {
-    const uint32_t other = __shfl_xor_sync(~0u, odd ? w[i] : w[i + 1], 1);
-    if (odd) w[i] = other;
-    else w[i + 1] = other;
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t other = __shfl_xor_sync(~0u, upper ? w[i] : w[i + 2], 2);
-    if (upper) w[i] = other;
-    else w[i + 2] = other;
+  for (int p = 0; p < 4; p += 2) {
+    const uint32_t other = __shfl_xor_sync(~0u, odd ? w[p] : w[p + 1], 1);
+    if (odd) w[p] = other;
+    else w[p + 1] = other;
   }
 }
 
@@ -94,16 +91,17 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_pack_kernel(W4PackParams p)
   uint8_t* chunk = p.data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
   const long long row_bytes = ((long long)f.K + 1) / 2, groups = ((long long)f.K + f.group - 1) / f.group;
   const W4Unit u = w4_unit();
-  const long long k0 = (long long)block * kW4Block + u.col;
-  uint32_t bytes[2][4];   // row, four columns; a byte each
-  uint16_t scale[2] = {0, 0};
-  int zero[2] = {8, 8};
+  uint32_t words[4];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int n = w4_row(f, strip, u.pair, j);
+  for (int q = 0; q < 2; ++q) {
+    const int col = u.col + 32 * q;
+    const long long k = (long long)block * kW4Block + col;
+    uint32_t low[2], high[2];
+    uint16_t scale[2] = {0, 0};
+    int zero[2] = {8, 8};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const long long k = k0 + 8 * h;
+    for (int j = 0; j < 2; ++j) {
+      const int n = w4_row(f, strip, u.pair, j);
       uint32_t v = 0x88888888u;   // nibbles of 8 columns
       if (n >= 0 && k < f.K) {
         const uint8_t* c = p.codes + n * row_bytes + k / 2;
@@ -114,21 +112,20 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_pack_kernel(W4PackParams p)
           const uint32_t mask = (1u << (4 * (int)(f.K - k))) - 1;
           v = (v & mask) | (0x88888888u & ~mask);
         }
+        if (col % f.group == 0) {
+          scale[j] = __ldg(p.scales + n * groups + k / f.group);
+          if (f.zeros) zero[j] = __ldg(p.zero_points + n * groups + k / f.group) & 15;
+        }
       }
-      bytes[j][2 * h] = __byte_perm(v & 0x0f0f, (v >> 4) & 0x0f0f, 0x5140);
-      bytes[j][2 * h + 1] = __byte_perm((v >> 16) & 0x0f0f, (v >> 20) & 0x0f0f, 0x5140);
+      low[j] = __byte_perm(v & 0x0f0f, (v >> 4) & 0x0f0f, 0x5140);
+      high[j] = __byte_perm((v >> 16) & 0x0f0f, (v >> 20) & 0x0f0f, 0x5140);
     }
-    if (u.col % f.group == 0 && n >= 0 && k0 < f.K) {
-      scale[j] = __ldg(p.scales + n * groups + k0 / f.group);
-      if (f.zeros) zero[j] = __ldg(p.zero_points + n * groups + k0 / f.group) & 15;
-    }
+    words[2 * q] = w4_word(low[0], low[1]);
+    words[2 * q + 1] = w4_word(high[0], high[1]);
+    if (col % f.group == 0) w4_store_scales<T>(f, chunk, u.pair, col, scale, zero);
   }
-  uint32_t words[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) words[i] = w4_word(bytes[0][i], bytes[1][i]);
-  w4_transpose(words);
+  w4_exchange(words);
   *reinterpret_cast<uint4*>(chunk + w4_unit_offset(u)) = make_uint4(words[0], words[1], words[2], words[3]);
-  if (u.col % f.group == 0) w4_store_scales<T>(f, chunk, u.pair, u.col, scale, zero);
 }
 
 // Eight columns of a source row, and the smallest and largest of them and 0 (symmetric: the largest
@@ -214,7 +211,7 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParam
   uint8_t* chunk = p.data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
   const W4Unit u = w4_unit();
   const int k0 = block * kW4Block + u.col;
-  W4Source<S> w[2][2];   // row, eight columns
+  W4Source<S> w[2][2];   // row, piece
   bool row[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -222,84 +219,93 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParam
     row[j] = n >= 0;
     const S* src = static_cast<const S*>(p.src) + (long long)(n < 0 ? 0 : n) * p.ld + k0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = k0 + 8 * h;
-      if (row[j] && p.vec && k + 8 <= f.K) w[j][h].load(src + 8 * h);
-      else w[j][h].load(src + 8 * h, row[j] ? f.K - k : 0);
+    for (int q = 0; q < 2; ++q) {
+      const int k = k0 + 32 * q;
+      if (row[j] && p.vec && k + 8 <= f.K) w[j][q].load(src + 32 * q);
+      else w[j][q].load(src + 32 * q, row[j] ? f.K - k : 0);
     }
   }
-  uint16_t scale_bits[2];
-  int zeros[2];
-  uint32_t codes[2][4];   // row, four columns; a byte each
+  uint32_t words[4];
+  uint32_t codes[2][2][2];                       // row, piece, first or last four columns; a byte each
+  constexpr int kPasses = GROUP == 32 ? 2 : 1;   // groups that a thread meets
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    float lo = 0.0f, hi = 0.0f;
+  for (int pass = 0; pass < kPasses; ++pass) {
+    const int col = u.col + 32 * pass;
+    uint16_t scale_bits[2];
+    int zeros[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) w[j][h].template range<ZEROS>(lo, hi);
+    for (int j = 0; j < 2; ++j) {
+      float lo = 0.0f, hi = 0.0f;
 #pragma unroll
-    for (int d = 1; d < GROUP / 16; d *= 2) {
-      if (ZEROS) lo = w4_min_nan(lo, __shfl_xor_sync(~0u, lo, d));
-      hi = w4_max_nan(hi, __shfl_xor_sync(~0u, hi, d));
-    }
-    const float span = ZEROS ? hi - lo : hi;
-    // Markstein's division by a constant is the division, but for subnormal results
-    const float n = ZEROS ? 15.0f : 7.0f;
-    float range = span < 0x1p-100f ? __fdiv_rn(span, n) : w4_quotient(span, n, 1.0f / n);
-    if (!(span <= 3.402823466e38f)) range = __int_as_float(0x7fc00000);   // an infinity or NaN in the group
-    const T scale_t = W4Traits<T>::from_float(range);
-    scale_bits[j] = *reinterpret_cast<const uint16_t*>(&scale_t);
-    const float scale = W4Traits<T>::to_float(scale_bits[j]);
-    const float divisor = scale == 0.0f ? 1.0f : scale;
-    const float least = std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-90f;
-    zeros[j] = 8;
-    if (sizeof(S) == 2 && scale >= least && scale <= 0x1p90f) {
+      for (int q = 0; q < 2; ++q)
+        if (kPasses == 1 || q == pass) w[j][q].template range<ZEROS>(lo, hi);
+#pragma unroll
+      for (int d = 1; d < (GROUP == 128 ? 8 : 4); d *= 2) {
+        if (ZEROS) lo = w4_min_nan(lo, __shfl_xor_sync(~0u, lo, d));
+        hi = w4_max_nan(hi, __shfl_xor_sync(~0u, hi, d));
+      }
+      const float span = ZEROS ? hi - lo : hi;
+      // Markstein's division by a constant is the division, but for subnormal results
+      const float n = ZEROS ? 15.0f : 7.0f;
+      float range = span < 0x1p-100f ? __fdiv_rn(span, n) : w4_quotient(span, n, 1.0f / n);
+      if (!(span <= 3.402823466e38f)) range = __int_as_float(0x7fc00000);   // an infinity or NaN in the group
+      const T scale_t = W4Traits<T>::from_float(range);
+      scale_bits[j] = *reinterpret_cast<const uint16_t*>(&scale_t);
+      const float scale = W4Traits<T>::to_float(scale_bits[j]);
+      const float divisor = scale == 0.0f ? 1.0f : scale;
+      const float least = std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-90f;
+      const bool plain = sizeof(S) == 2 && scale >= least && scale <= 0x1p90f;
       // quotient + 1.5 2^23 is the rounded quotient in the low bits (ties to even)
       constexpr float kRound = 12582912.0f;
       float inverse;
       asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(divisor));
-      if (ZEROS) zeros[j] = (int)(__float_as_uint(w4_quotient(-lo, divisor, inverse) + kRound) & 15);
+      zeros[j] = 8;
+      if (ZEROS)
+        zeros[j] = plain ? (int)(__float_as_uint(w4_quotient(-lo, divisor, inverse) + kRound) & 15)
+                         : (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, divisor)), 0.0f), 15.0f);
       const float most = kRound + (15 - zeros[j]);
       const uint32_t add = zeros[j] * 0x01010101u;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t b[4];
+      for (int q = 0; q < 2; ++q) {
+        if (kPasses == 2 && q != pass) continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = w4_quotient(w[j][e / 2][e % 2 * 4 + i], divisor, inverse) + kRound;
-          b[i] = __float_as_uint(ZEROS ? fminf(x, most) : x);
+        for (int e = 0; e < 2; ++e) {
+          if (plain) {
+            uint32_t b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float x = w4_quotient(w[j][q][4 * e + i], divisor, inverse) + kRound;
+              b[i] = __float_as_uint(ZEROS ? fminf(x, most) : x);
+            }
+            // the low bytes are -15..15: their low nibbles plus the zero point, modulo 16
+            const uint32_t v = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+            codes[j][q][e] = ZEROS ? ((v & 0x0f0f0f0fu) + add) & 0x0f0f0f0fu : (v & 0x0f0f0f0fu) ^ 0x08080808u;
+          } else {
+            codes[j][q][e] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float c = fminf(fmaxf(rintf(__fdiv_rn(w[j][q][4 * e + i], divisor)) + zeros[j], 0.0f), 15.0f);
+              codes[j][q][e] |= (uint32_t)(int)c << (8 * i);
+            }
+          }
         }
-        // the low bytes are -15..15: their low nibbles plus the zero point, modulo 16
-        const uint32_t v = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-        codes[j][e] = ZEROS ? ((v & 0x0f0f0f0fu) + add) & 0x0f0f0f0fu : (v & 0x0f0f0f0fu) ^ 0x08080808u;
-      }
-    } else {
-      if (ZEROS) zeros[j] = (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, divisor)), 0.0f), 15.0f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        codes[j][e] = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float c = fminf(fmaxf(rintf(__fdiv_rn(w[j][e / 2][e % 2 * 4 + i], divisor)) + zeros[j], 0.0f), 15.0f);
-          codes[j][e] |= (uint32_t)(int)c << (8 * i);
+        const int have = row[j] ? f.K - k0 - 32 * q : 0;
+        if (have < 8) {   // behind the matrix: as pack leaves it
+          const uint32_t keep0 = have >= 4 ? ~0u : have <= 0 ? 0u : (1u << (8 * have)) - 1;
+          const uint32_t keep1 = have <= 4 ? 0u : (1u << (8 * (have - 4))) - 1;
+          codes[j][q][0] = (codes[j][q][0] & keep0) | (0x08080808u & ~keep0);
+          codes[j][q][1] = (codes[j][q][1] & keep1) | (0x08080808u & ~keep1);
         }
       }
+      if (!row[j] || block * kW4Block + col - col % GROUP >= f.K) zeros[j] = 8;
     }
-    const int have = row[j] ? f.K - k0 : 0;
-    if (have < 16) {   // behind the matrix: as pack leaves it
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int m = have - 4 * e;
-        const uint32_t keep = m >= 4 ? ~0u : m <= 0 ? 0u : (1u << (8 * m)) - 1;
-        codes[j][e] = (codes[j][e] & keep) | (0x08080808u & ~keep);
-      }
-    }
-    if (!row[j] || k0 - u.col % GROUP >= f.K) zeros[j] = 8;
+    if (col % GROUP == 0) w4_store_scales<T>(f, chunk, u.pair, col, scale_bits, zeros);
   }
-  if (u.col % GROUP == 0) w4_store_scales<T>(f, chunk, u.pair, u.col, scale_bits, zeros);
-  uint32_t words[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) words[i] = w4_word(codes[0][i], codes[1][i]);
-  w4_transpose(words);
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) words[2 * q + e] = w4_word(codes[0][q][e], codes[1][q][e]);
+  w4_exchange(words);
   *reinterpret_cast<uint4*>(chunk + w4_unit_offset(u)) = make_uint4(words[0], words[1], words[2], words[3]);
 }
 
@@ -313,51 +319,50 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f,
   const W4Unit u = w4_unit();
   const uint4 code = __ldg(reinterpret_cast<const uint4*>(chunk + w4_unit_offset(u)));
   uint32_t words[4] = {code.x, code.y, code.z, code.w};
-  w4_transpose(words);
-  const int k0 = block * kW4Block + u.col;
-  if (k0 >= f.K) return;
-  const uint8_t* sp = chunk + w4_scale_offset(u.pair, u.col / f.group);
-  const float2 scale = W4Traits<T>::to_float2(__ldg(reinterpret_cast<const uint32_t*>(sp)));
-  uint32_t off0 = W4Traits<T>::kMinusEight, off1 = off0;
-  if (f.zeros) {
-    const uint32_t both = __ldg(reinterpret_cast<const uint32_t*>(sp + kW4Block / f.group * 128));
-    off0 = __byte_perm(both, 0, 0x1010);
-    off1 = __byte_perm(both, 0, 0x3232);
-  }
-  float v[2][16];
+  w4_exchange(words);
+  const int n[2] = {w4_row(f, strip, u.pair, 0), w4_row(f, strip, u.pair, 1)};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    uint32_t a[4];   // row of the pair: i % 2; columns 2 (i / 2) and the next
-    w4_decode<T>(words[e], off0, off1, a);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 two = W4Traits<T>::to_float2(W4Traits<T>::fma2(a[i], W4Traits<T>::kBack, 0x80008000u));
-      const float by = i & 1 ? scale.y : scale.x;
-      v[i & 1][4 * e + 2 * (i >> 1)] = two.x * by;
-      v[i & 1][4 * e + 2 * (i >> 1) + 1] = two.y * by;
+  for (int q = 0; q < 2; ++q) {
+    const int col = u.col + 32 * q, k = block * kW4Block + col;
+    if (k >= f.K) break;
+    const uint8_t* sp = chunk + w4_scale_offset(u.pair, col / f.group);
+    const float2 scale = W4Traits<T>::to_float2(__ldg(reinterpret_cast<const uint32_t*>(sp)));
+    uint32_t off0 = W4Traits<T>::kMinusEight, off1 = off0;
+    if (f.zeros) {
+      const uint32_t both = __ldg(reinterpret_cast<const uint32_t*>(sp + kW4Block / f.group * 128));
+      off0 = __byte_perm(both, 0, 0x1010);
+      off1 = __byte_perm(both, 0, 0x3232);
     }
-  }
+    float v[2][8];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int n = w4_row(f, strip, u.pair, j);
-    if (n < 0) continue;
+    for (int e = 0; e < 2; ++e) {
+      uint32_t a[4];   // row of the pair: i % 2; columns 2 (i / 2) and the next
+      w4_decode<T>(words[2 * q + e], off0, off1, a);
 #pragma unroll
-    for (int h = 0; h < 16; h += 8) {
-      const int k = k0 + h;
-      O* dst = out + (long long)n * ld + k;
+      for (int i = 0; i < 4; ++i) {
+        const float2 two = W4Traits<T>::to_float2(W4Traits<T>::fma2(a[i], W4Traits<T>::kBack, 0x80008000u));
+        const float by = i & 1 ? scale.y : scale.x;
+        v[i & 1][4 * e + 2 * (i >> 1)] = two.x * by;
+        v[i & 1][4 * e + 2 * (i >> 1) + 1] = two.y * by;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (n[j] < 0) continue;
+      O* dst = out + (long long)n[j] * ld + k;
       if (vec && k + 8 <= f.K) {
         if constexpr (sizeof(O) == 4) {
-          reinterpret_cast<float4*>(dst)[0] = make_float4(v[j][h], v[j][h + 1], v[j][h + 2], v[j][h + 3]);
-          reinterpret_cast<float4*>(dst)[1] = make_float4(v[j][h + 4], v[j][h + 5], v[j][h + 6], v[j][h + 7]);
+          reinterpret_cast<float4*>(dst)[0] = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
+          reinterpret_cast<float4*>(dst)[1] = make_float4(v[j][4], v[j][5], v[j][6], v[j][7]);
         } else {
           *reinterpret_cast<uint4*>(dst) =
-              make_uint4(w4_round2(v[j][h], v[j][h + 1], O()), w4_round2(v[j][h + 2], v[j][h + 3], O()),
-                         w4_round2(v[j][h + 4], v[j][h + 5], O()), w4_round2(v[j][h + 6], v[j][h + 7], O()));
+              make_uint4(w4_round2(v[j][0], v[j][1], O()), w4_round2(v[j][2], v[j][3], O()),
+                         w4_round2(v[j][4], v[j][5], O()), w4_round2(v[j][6], v[j][7], O()));
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (k + e < f.K) dst[e] = (O)v[j][h + e];
+          if (k + e < f.K) dst[e] = (O)v[j][e];
       }
     }
   }

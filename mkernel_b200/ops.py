@@ -40,6 +40,17 @@ def _raw_stream_of(index: int):
     return torch.cuda.current_stream(index).cuda_stream
 
 
+def _call_on(index: int, call, *args) -> None:
+    """call(*args, stream) on device `index` and its current stream; raises what the library reports."""
+    if _current_device() != index:
+        with _on_device(index):
+            rc = call(*args, _raw_stream_of(index))
+    else:
+        rc = call(*args, _raw_stream_of(index))
+    if rc < 0:
+        _lib.check(rc)
+
+
 class _on_device:
     """Make `index` the current CUDA device for the duration of a call; free when it already is
     (the common case: one process per GPU), since these wrappers sit on latency-bound paths."""
@@ -171,13 +182,15 @@ class W4Weight:
         self.shape, self.K, self.group, self.dtype, self.form = (N, K), K, group, dtype, form
         self.n_out = N // 2 if form == "gate_up" else N
         self.zero_points, self.rotary_dim = bool(zero_points), rotary_dim
-        self.view = _lib.W4View(None, N, K, group, _DTYPES[dtype], bool(zero_points), _W4_FORMS[form],
-                                head_dim, rotary_dim, rotated_heads, bool(interleaved))
-        self.view_ref = ctypes.byref(self.view)
-        nbytes = _lib.check(_lib.lib().mk_w4_bytes(self.view_ref))
-        self.data = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        self.device, self.index = self.data.device, self.data.get_device()
-        self.view.data = self.data.data_ptr()
+        view = _lib.W4View(None, N, K, group, _DTYPES[dtype], self.zero_points, _W4_FORMS[form], head_dim,
+                           rotary_dim, rotated_heads, bool(interleaved))
+        self.view, self.view_ref = view, ctypes.byref(view)
+        nbytes = _lib.lib().mk_w4_bytes(self.view_ref)
+        if nbytes < 0:
+            _lib.check(nbytes)
+        self.data = data = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self.device, self.index = data.device, data.get_device()
+        view.data = data.data_ptr()
 
     def dequantize(self, out: torch.Tensor | None = None) -> torch.Tensor:
         """The matrix these weights stand for, rows in the order given to ``w4_quantize`` or
@@ -188,9 +201,8 @@ class W4Weight:
         if out.get_device() != self.index or out.dtype not in _DTYPES or out.shape != self.shape or \
                 (step != 1 and K > 1) or (ld < K and N > 1):
             _require(False, f"out must be {self.shape} on {self.device}, bfloat16, float16 or float32, rows contiguous")
-        with _on_device(self.index):
-            _lib.check(_lib.lib().mk_w4_dequantize(self.view_ref, out.data_ptr(), ld if N > 1 else K,
-                                                   _DTYPES[out.dtype], _raw_stream_of(self.index)))
+        _call_on(self.index, _lib.lib().mk_w4_dequantize, self.view_ref, out.data_ptr(), ld if N > 1 else K,
+                 _DTYPES[out.dtype])
         return out
 
 
@@ -202,17 +214,15 @@ def w4_quantize(weight: torch.Tensor, group: int = 128, zero_points: bool = Fals
     ``form``: nothing for ``w4_gemm``; ``form="gate_up"`` for ``w4_gemm_swiglu`` (gate rows, then up
     rows); ``form="rotary", head_dim=, rotary_dim=, rotated_heads=, interleaved=`` for
     ``w4_gemm_rotary``."""
-    _require(isinstance(weight, torch.Tensor) and weight.is_cuda and weight.dim() == 2 and
-             weight.dtype in _DTYPES, "weight must be a CUDA matrix of bfloat16, float16 or float32")
-    _require(weight.stride(1) == 1 or weight.shape[1] == 1, "weight's rows must be contiguous")
-    dtype = dtype or (weight.dtype if weight.dtype != torch.float32 else torch.bfloat16)
-    N, K = weight.shape
-    ld = weight.stride(0) if N > 1 else K
-    _require(ld >= K, "weight's rows overlap")
+    if not isinstance(weight, torch.Tensor) or not weight.is_cuda or weight.dim() != 2 or weight.dtype not in _DTYPES:
+        _require(False, "weight must be a CUDA matrix of bfloat16, float16 or float32")
+    src_dtype, (N, K), (ld, step) = weight.dtype, weight.shape, weight.stride()
+    if (step != 1 and K > 1) or (ld < K and N > 1):
+        _require(False, "weight's rows must be contiguous and not overlap")
+    if dtype is None:
+        dtype = src_dtype if src_dtype is not torch.float32 else torch.bfloat16
     W = W4Weight(N, K, group, dtype, zero_points, weight.device, **form)
-    with _on_device(W.index):
-        _lib.check(_lib.lib().mk_w4_quantize(W.view_ref, weight.data_ptr(), ld, _DTYPES[weight.dtype],
-                                             _raw_stream_of(W.index)))
+    _call_on(W.index, _lib.lib().mk_w4_quantize, W.view_ref, weight.data_ptr(), ld if N > 1 else K, _DTYPES[src_dtype])
     return W
 
 
@@ -235,10 +245,8 @@ def w4_pack(codes: torch.Tensor, scales: torch.Tensor, zero_points: torch.Tensor
              f"scales must be [N, ceil(K / group)] with a group of 32, 64 or 128 (K={K})")
     _require(zero_points is None or zero_points.shape == scales.shape, "zero_points must have the scales' shape")
     W = W4Weight(N, K, group, scales.dtype, zero_points is not None, codes.device, **form)
-    with _on_device(W.index):
-        _lib.check(_lib.lib().mk_w4_pack(W.view_ref, codes.data_ptr(), scales.data_ptr(),
-                                         zero_points.data_ptr() if zero_points is not None else None,
-                                         _raw_stream_of(W.index)))
+    _call_on(W.index, _lib.lib().mk_w4_pack, W.view_ref, codes.data_ptr(), scales.data_ptr(),
+             zero_points.data_ptr() if zero_points is not None else None)
     return W
 
 
@@ -264,12 +272,7 @@ def _w4_launch(call, A: torch.Tensor, W: W4Weight, C: torch.Tensor, form: str, *
     lda, ldc = (a_stride[0], c_stride[0]) if M > 1 else (K, n_out)     # one row may have any stride
     if M > 1 and ldc < n_out:
         _require(False, "rows of C overlap")
-    if _current_device() != index:
-        with _on_device(index):
-            _lib.check(call(A.data_ptr(), lda, W.view_ref, C.data_ptr(), ldc, M, *more, _raw_stream_of(index)))
-        return
-    if call(A.data_ptr(), lda, W.view_ref, C.data_ptr(), ldc, M, *more, _raw_stream_of(index)) < 0:
-        _lib.check(-1)
+    _call_on(index, call, A.data_ptr(), lda, W.view_ref, C.data_ptr(), ldc, M, *more)
 
 
 def w4_gemm(A: torch.Tensor, W: W4Weight, C: torch.Tensor) -> None:
@@ -321,15 +324,18 @@ def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     [rows, (heads + ...) * head_dim] are a view of its output."""
     if not isinstance(X, torch.Tensor) or not X.is_cuda or X.dtype not in _DTYPES or X.dim() != 3:
         _require(False, "X must be a CUDA tensor [rows, heads, head_dim] of bfloat16, float16 or float32")
-    shape, xs, index = X.shape, X.stride(), X.get_device()
+    shape, xs, index, dtype, x = X.shape, X.stride(), X.get_device(), X.dtype, X.data_ptr()
     rows, heads, dim = shape
     if Y is None or Y is X:
-        Y, ys = X, xs
+        Y, ys, y = X, xs, x
     else:
-        if Y.get_device() != index or Y.dtype is not X.dtype or Y.shape != shape:
+        if Y.get_device() != index or Y.dtype is not dtype or Y.shape != shape:
             _require(False, "Y must have X's device, type and shape")
-        ys = Y.stride()
-        if _overlap(X, xs, Y, ys, shape):
+        ys, y = Y.stride(), Y.data_ptr()
+        # the address ranges of the two must not meet
+        size = 4 if dtype is torch.float32 else 2
+        if rows and heads and x < y + size * ((rows - 1) * ys[0] + (heads - 1) * ys[1] + dim) and \
+                y < x + size * ((rows - 1) * xs[0] + (heads - 1) * xs[1] + dim):
             _require(False, "Y must be X or share no memory with it")
     if dim > 1 and (xs[2] != 1 or ys[2] != 1):
         _require(False, "features of X and Y must be contiguous")
@@ -338,20 +344,9 @@ def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
             (rows < 2 or ys[0] >= dim) and (heads < 2 or ys[1] >= (rows - 1) * ys[0] + dim)):
         _require(False, "two elements of Y share memory")
     wide = _rotary_operands(positions, inv_freq, rows, -1, index)
-    with _on_device(index):
-        _lib.check(_lib.lib().mk_rotary(X.data_ptr(), xs[0], xs[1], Y.data_ptr(), ys[0], ys[1], rows, heads, dim,
-                                        2 * inv_freq.shape[0], _DTYPES[X.dtype], positions.data_ptr(), wide,
-                                        inv_freq.data_ptr(), scale, interleaved, inverse, _raw_stream_of(index)))
+    _call_on(index, _lib.lib().mk_rotary, x, xs[0], xs[1], y, ys[0], ys[1], rows, heads, dim, 2 * inv_freq.shape[0],
+             _DTYPES[dtype], positions.data_ptr(), wide, inv_freq.data_ptr(), scale, interleaved, inverse)
     return Y
-
-
-def _overlap(a: torch.Tensor, a_stride, b: torch.Tensor, b_stride, shape) -> bool:
-    """Whether the address ranges of two tensors of one shape and type meet."""
-    if 0 in shape:
-        return False
-    a0, b0, size = a.data_ptr(), b.data_ptr(), a.element_size()
-    last = lambda strides: size * (1 + sum((n - 1) * s for n, s in zip(shape, strides)))
-    return a0 < b0 + last(b_stride) and b0 < a0 + last(a_stride)
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | None = None,
