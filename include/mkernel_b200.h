@@ -218,8 +218,16 @@ int mk_w4_quantize(const mk_w4* w, const void* src, long long ld, int src_dtype,
  * once to out_dtype; row stride ld elements. */
 int mk_w4_dequantize(const mk_w4* w, void* out, long long ld, int out_dtype, void* stream);
 
+/* Copies rows of 16-bit elements to a buffer that is 16-byte aligned and whose row stride ld_dst is a multiple
+ * of 8 elements; elements behind the last column become 0. */
+int mk_align_rows(const void* src, long long ld, int rows, int cols, void* dst, long long ld_dst,
+                  void* stream);
+
 /* C[M, N] = A[M, K] * W^T.  A and C have w's dtype and row strides lda, ldc (elements); fp32 sums,
- * rounded once.  M = 0 does nothing.  w->form = MK_W4_PLAIN. */
+ * rounded once.  M = 0 does nothing.  w->form = MK_W4_PLAIN.
+ * For M <= 16 the products are of the weights as they are.  For more the weights are rounded to w's
+ * dtype first, as mk_w4_dequantize gives them (not in the SwiGLU form, which takes what the rounding
+ * leaves as well), and rows of A must start on 16 bytes (A aligned, lda a multiple of 8). */
 int mk_w4_gemm(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
                void* stream);
 /* H[M, N/2] = silu(A * G^T) * (A * U^T) with w->form = MK_W4_GATE_UP: the single-token form of

@@ -112,6 +112,7 @@ _SIGNATURES = {
     "mk_w4_pack": (c_int, [POINTER(W4View), c_void_p, c_void_p, c_void_p, c_void_p]),
     "mk_w4_quantize": (c_int, [POINTER(W4View), c_void_p, c_longlong, c_int, c_void_p]),
     "mk_w4_dequantize": (c_int, [POINTER(W4View), c_void_p, c_longlong, c_int, c_void_p]),
+    "mk_align_rows": (c_int, [c_void_p, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p]),
     "mk_w4_gemm": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong, c_int,
                            c_void_p]),
     "mk_w4_gemm_swiglu": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong,

@@ -652,6 +652,24 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
   if (p.split > 1) ptx::cluster_sync_all();   // nobody leaves while its shared memory is read
 }
 
+// Rows of 16-bit elements copied to where 16-byte accesses can read them: eight elements a thread.
+__global__ void __launch_bounds__(128) align_rows_kernel(const uint16_t* src, long long ld, int rows, int cols,
+                                                         uint16_t* dst, long long ld_dst) {
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const long long pieces = ld_dst / 8, total = rows * pieces;
+  for (long long e = (long long)blockIdx.x * 128 + threadIdx.x; e < total; e += (long long)gridDim.x * 128) {
+    const long long row = e / pieces;
+    const int col = (int)(e - row * pieces) * 8;
+    const uint16_t* from = src + row * ld + col;
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? __ldg(from + i) : 0u;
+    *reinterpret_cast<uint4*>(dst + row * ld_dst + col) =
+        make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+  }
+}
+
 // ------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------
@@ -773,13 +791,16 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.form = w4_form(*w);
   p.data = static_cast<const uint8_t*>(w->data);
   p.A = A; p.lda = lda; p.C = C; p.ldc = ldc; p.M = M;
-  p.vec = (reinterpret_cast<uintptr_t>(A) & 15) == 0 && lda % 8 == 0 && w->K % 8 == 0;
+  p.vec = (reinterpret_cast<uintptr_t>(A) & 15) == 0 && (lda % 8 == 0 || M == 1);
   p.epilogue = epilogue;
   p.rotary = rotary;
   p.wide = (reinterpret_cast<uintptr_t>(C) & 7) == 0 && ldc % 4 == 0 && (form != MK_W4_GATE_UP || w->N / 2 % 4 == 0);
   p.wait_limit_ns = option_wait_limit_ns();
   // Up to 16 tokens the stream kernel is bound by memory as it should be; every 16 more cost it another
   // pass over the weights.
+  if (M > 16 && !p.vec)
+    return set_error(MK_ERR_INVALID, "%s: for more than 16 rows A's must start on 16 bytes (mk_align_rows copies them so)",
+                     what);
   if (M > 16) return w4_tile_launch(p, w->dtype, sms, static_cast<cudaStream_t>(stream));
   const W4StreamPlan pl = w4_stream_plan(p.form, M, sms);
   p.stage_bytes = pl.stage_bytes;
@@ -907,6 +928,21 @@ int mk_w4_dequantize(const mk_w4* w, void* out, long long ld, int out_dtype, voi
   const uint8_t* data = static_cast<const uint8_t*>(w->data);
   return w->dtype == MK_BF16 ? w4_dequantize_launch<__nv_bfloat16>(f, data, out, ld, out_dtype, vec, grid, s)
                              : w4_dequantize_launch<__half>(f, data, out, ld, out_dtype, vec, grid, s);
+}
+
+int mk_align_rows(const void* src, long long ld, int rows, int cols, void* dst, long long ld_dst, void* stream) {
+  if (rows < 0 || cols < 1) return set_error(MK_ERR_INVALID, "mk_align_rows: bad shape %d x %d", rows, cols);
+  if (rows == 0) return MK_OK;
+  if (!src || !dst || ld < cols || ld_dst < cols || ld_dst % 8 != 0 || (reinterpret_cast<uintptr_t>(dst) & 15) != 0 ||
+      (reinterpret_cast<uintptr_t>(src) & 1) != 0)
+    return set_error(MK_ERR_INVALID, "mk_align_rows: needs whole rows, a 16-byte aligned copy and its stride a multiple of 8");
+  int sms = 0;
+  const int rc = device_sm_count(&sms);
+  if (rc != MK_OK) return rc;
+  long long blocks = ((long long)rows * (ld_dst / 8) + 127) / 128;
+  if (blocks > 16LL * sms) blocks = 16LL * sms;
+  return w4_launch(align_rows_kernel, dim3((unsigned)blocks), 128, 0, 1, static_cast<cudaStream_t>(stream),
+                   static_cast<const uint16_t*>(src), ld, rows, cols, static_cast<uint16_t*>(dst), ld_dst);
 }
 
 int mk_w4_gemm(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M, void* stream) {

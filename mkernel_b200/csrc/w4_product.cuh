@@ -20,7 +20,7 @@ struct W4Params {
   void* C;
   long long ldc;
   int M;
-  int vec;             // rows of A start on 16 bytes (and, in the stream kernel, K is a multiple of 8)
+  int vec;             // rows of A start on 16 bytes
   int stage_bytes;     // of a shared-memory ring
   int split;           // CTAs of a cluster, which share a strip along K
   int token_tiles;     // tile kernel

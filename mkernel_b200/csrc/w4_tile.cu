@@ -16,8 +16,8 @@
 //
 // Warps 0..15 decode, in two sets that take turns at the blocks of 128 columns (quadrant warp % 4 of the
 // lanes, half of the columns by warp / 4 % 2), and at the end read the sums; warps 16 and 17 issue the
-// MMAs; a thread each of warps 18 to 21 (all of them where rows are not aligned) copies a ring of stages (a
-// block: codes of two strips, tokens in the 128-byte swizzle; one thread for it all needs 0.33 us a block).  A block is little work and a long way: a wait for
+// MMAs; a thread each of warps 18 to 21 copies a ring of stages (a block: codes of two strips, tokens in the
+// 128-byte swizzle; one thread for it all needs 0.33 us a block).  A block is little work and a long way: a wait for
 // a barrier alone takes some 150 cycles, issuing eight MMAs and a commit 350, whatever the tokens.  So what
 // bounds a narrow product is how many blocks are under way, and up to 128 tokens two warps issue, every
 // other block each, into sums of their own (one warp: 0.39 us a block at 64 tokens).
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(full(s), p.vec ? 2 : kTileLoaders * 32);
+      ptx::mbar_init(full(s), 2);
       ptx::mbar_init(empty(s), kTileCompute / kTurns + 1);
     }
     for (int i = 0; i < kOperands; ++i) {
@@ -235,7 +235,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // The tokens need no wait of their own: who decoded the block has waited for them.
       ok = w4_wait_warp(wc, a_full(operand), (b / kOperands) & 1);
       if (!ok) break;
-      if (!p.vec) ptx::fence_proxy_async();   // the tokens were written by ordinary stores
       ptx::tc_fence_after();
       const uint32_t a = tmem_a + operand * kOperand, b_lo = b_lo0 + s * (p.stage_bytes >> 4);
       ptx::umma_ts<4>(d, a, b_lo, desc_hi, idesc, b >= kSums ? 1u : 0u);
@@ -248,7 +247,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       ptx::umma_commit_elect<1>(empty(s), 0);
     }
     if (ok && me < kSums) ptx::umma_commit_elect<1>(done, 0);
-  } else if (p.vec) {
+  } else {
     // ---------------- copies: two threads for the codes, two for the tokens (tensor copies) ----------------
     const int me = warp - kTileCompute - kTileIssue;
     const bool tokens = me >= 2, active = lane == 0 && (me & 1) < kTurns;
@@ -268,39 +267,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (two) ptx::bulk_g2s(stage + kTokens * 256 + f.chunk_bytes, chunk + strip_bytes, f.chunk_bytes, full(s));
       }
     }
-  } else {
-    // ---------------- copies where rows of tokens start on no 16 bytes ----------------
-    const int lt = threadIdx.x - (kTileCompute + kTileIssue) * 32, lw = lt >> 5;
-    const int pieces = f.chunk_bytes / 16 * (two ? 2 : 1);
-    // lane = 4 columns of a token, in the 128-byte swizzle
-    const uint32_t unit = lane >> 1 & 7, low = (lane >> 4) * kXHalf + (lane & 1) * 8;
-    const uint16_t* A = static_cast<const uint16_t*>(p.A);
-    for (int b = 0; b < blocks; ++b) {
-      const int s = b % kStages;
-      if (b >= kStages && !w4_wait(wc, empty(s), (b / kStages - 1) & 1)) break;
-      const uint32_t stage = ring + s * p.stage_bytes;
-      const uint8_t* chunk = data + (size_t)b * p.split * f.chunk_bytes;
-      for (int i = lt; i < pieces; i += kTileLoaders * 32) {
-        const int o = i * 16;
-        ptx::cp_async_16(stage + kTokens * 256 + o,
-                         o < f.chunk_bytes ? chunk + o : chunk + strip_bytes + (o - f.chunk_bytes));
-      }
-      const long long k = (long long)(rank + b * p.split) * kW4Block + lane * 4;
-#pragma unroll 4
-      for (int m = lw; m < kTokens; m += kTileLoaders) {
-        uint32_t e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          e[i] = token0 + m < p.M && k + i < f.K ? __ldg(A + (long long)(token0 + m) * p.lda + k + i) : 0u;
-        *reinterpret_cast<uint2*>(ring_ptr + s * p.stage_bytes + low + m * 128 + ((unit ^ (m & 7)) << 4)) =
-            make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
-      }
-      ptx::cp_async_commit();
-      ptx::cp_async_wait<0>();
-      ptx::mbar_arrive(full(s));
-    }
-    ptx::cp_async_commit();
-    ptx::cp_async_wait<0>();
   }
   // a wait that ran out leaves MMAs that may still read the ring
   if (*s_abort != 0u) __nanosleep(50000);
@@ -437,12 +403,9 @@ int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
     }
   p.token_tiles = (p.M + tokens - 1) / tokens;
   p.stage_bytes = (tokens * 256 + 2 * f.chunk_bytes + 1023) / 1024 * 1024;
-  p.vec = (reinterpret_cast<uintptr_t>(p.A) & 15) == 0 && p.lda % 8 == 0;
-  CUtensorMap map = {};
-  if (p.vec) {
-    const int rc = w4_tile_map(&map, p, dtype, tokens);
-    if (rc != MK_OK) return rc;
-  }
+  CUtensorMap map;
+  const int rc = w4_tile_map(&map, p, dtype, tokens);
+  if (rc != MK_OK) return rc;
   const long long grid = row_tiles * p.token_tiles * p.split;
   if (grid > 0x7fffffffLL) return set_error(MK_ERR_INVALID, "4-bit product: M=%d, N=%d is too large", p.M, f.N);
   return dtype == MK_BF16 ? w4_tile_tokens<__nv_bfloat16>(p, map, tokens, (unsigned)grid, stream)

@@ -272,12 +272,22 @@ def _w4_launch(call, A: torch.Tensor, W: W4Weight, C: torch.Tensor, form: str, *
     lda, ldc = (a_stride[0], c_stride[0]) if M > 1 else (K, n_out)     # one row may have any stride
     if M > 1 and ldc < n_out:
         _require(False, "rows of C overlap")
-    _call_on(index, call, A.data_ptr(), lda, W.view_ref, C.data_ptr(), ldc, M, *more)
+    a = A.data_ptr()
+    if (a & 15 or (lda & 7 and M > 1)) and (M > 16 or M * K > 32768):
+        # Rows that no 16-byte access can start on: more than 16 are copied, and few where a launch costs less
+        # than reading them element by element.
+        lda = (K + 7) // 8 * 8
+        rows = torch.empty((M, lda), dtype=dtype, device=W.device)
+        if M:
+            _call_on(index, _lib.lib().mk_align_rows, a, a_stride[0] if M > 1 else K, M, K, rows.data_ptr(), lda)
+        a = rows.data_ptr()
+    _call_on(index, call, a, lda, W.view_ref, C.data_ptr(), ldc, M, *more)
 
 
 def w4_gemm(A: torch.Tensor, W: W4Weight, C: torch.Tensor) -> None:
     """C[M, N] = A[M, K] @ W^T with 4-bit weights: the single-token and small-batch form of
-    ``gemm_bf16``.  A and C in the type of W's scales, any row strides; fp32 sums, rounded once."""
+    ``gemm_bf16``.  A and C in the type of W's scales, any row strides; fp32 sums, rounded once.
+    For more than 16 rows the weights are rounded to that type first, as ``W.dequantize()`` gives them."""
     _w4_launch(_lib.lib().mk_w4_gemm, A, W, C, "plain")
 
 

@@ -60,6 +60,11 @@ def test_bad_operands_are_refused():
     assert lib.mk_w4_quantize(ok, 4098, 128, 2, None) == -1
     assert lib.mk_w4_dequantize(ok, None, 128, 0, None) == -1
     assert lib.mk_w4_dequantize(ok, 4096, 128, 7, None) == -1
+    assert lib.mk_align_rows(4096, 100, 2, 101, 8192, 104, None) == -1
+    assert lib.mk_align_rows(4096, 100, 2, 100, 8192, 100, None) == -1
+    assert lib.mk_align_rows(4096, 100, 2, 100, 8200, 104, None) == -1
+    assert lib.mk_align_rows(None, 100, 2, 100, 8192, 104, None) == -1
+    assert lib.mk_align_rows(None, 100, 0, 100, None, 104, None) == 0
     assert lib.mk_w4_gemm(None, 0, ok, None, 0, 0, None) == 0             # no rows, nothing to do
 
 
