@@ -86,6 +86,8 @@ __device__ __forceinline__ void w4_store_scales(const W4Form& f, uint8_t* chunk,
 // Codes behind the matrix are 8, their scales 0 and zero points 8, whoever lays them out.
 template <typename T>
 __global__ void __launch_bounds__(kW4PackThreads) w4_pack_kernel(W4PackParams p) {
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const W4Form& f = p.form;
   const int strip = blockIdx.y, block = blockIdx.x;
   uint8_t* chunk = p.data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
@@ -203,9 +205,12 @@ __device__ __forceinline__ float w4_quotient(float w, float d, float r) {
 // of two 16-bit values is far from half way between whole numbers (2^-12 of it) unless it is exactly
 // there, and then w4_quotient is exact too, so both go the same way.  Nor a clamp below: the
 // quotient of the largest magnitude is within 2^-8 of 7, that of hi - lo of 15.  Both need a scale that
-// is no subnormal; for others, and for fp32 weights, it is divided and clamped as the definition says.
+// is no subnormal (or 0, when all quotients round to 0); for others, and for fp32 weights, it is divided and
+// clamped as the definition says.
 template <typename T, typename S, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParams p) {
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const W4Form& f = p.form;
   const int strip = blockIdx.y, block = blockIdx.x;
   uint8_t* chunk = p.data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
@@ -254,7 +259,7 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParam
       const float scale = W4Traits<T>::to_float(scale_bits[j]);
       const float divisor = scale == 0.0f ? 1.0f : scale;
       const float least = std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-90f;
-      const bool plain = sizeof(S) == 2 && scale >= least && scale <= 0x1p90f;
+      const bool plain = sizeof(S) == 2 && (scale == 0.0f || (scale >= least && scale <= 0x1p90f));
       // quotient + 1.5 2^23 is the rounded quotient in the low bits (ties to even)
       constexpr float kRound = 12582912.0f;
       float inverse;
@@ -314,6 +319,8 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParam
 template <typename T, typename O>
 __global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f, const uint8_t* data, O* out,
                                                                        long long ld, int vec) {
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const int strip = blockIdx.y, block = blockIdx.x;
   const uint8_t* chunk = data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
   const W4Unit u = w4_unit();
@@ -819,9 +826,7 @@ static int w4_quantize_group(const W4PackParams& p, dim3 grid, cudaStream_t s) {
   auto kern = p.form.group == 32   ? (z ? w4_quantize_kernel<T, S, 32, true> : w4_quantize_kernel<T, S, 32, false>)
               : p.form.group == 64 ? (z ? w4_quantize_kernel<T, S, 64, true> : w4_quantize_kernel<T, S, 64, false>)
                                    : (z ? w4_quantize_kernel<T, S, 128, true> : w4_quantize_kernel<T, S, 128, false>);
-  kern<<<grid, kW4PackThreads, 0, s>>>(p);
-  MKB_CUDA(cudaGetLastError());
-  return MK_OK;
+  return w4_launch(kern, grid, kW4PackThreads, 0, 1, s, p);
 }
 
 template <typename T>
@@ -835,13 +840,13 @@ template <typename T>
 static int w4_dequantize_launch(const W4Form& f, const uint8_t* data, void* out, long long ld, int dtype, int vec,
                                 dim3 grid, cudaStream_t s) {
   if (dtype == MK_BF16)
-    w4_dequantize_kernel<T><<<grid, kW4PackThreads, 0, s>>>(f, data, static_cast<__nv_bfloat16*>(out), ld, vec);
-  else if (dtype == MK_FP16)
-    w4_dequantize_kernel<T><<<grid, kW4PackThreads, 0, s>>>(f, data, static_cast<__half*>(out), ld, vec);
-  else
-    w4_dequantize_kernel<T><<<grid, kW4PackThreads, 0, s>>>(f, data, static_cast<float*>(out), ld, vec);
-  MKB_CUDA(cudaGetLastError());
-  return MK_OK;
+    return w4_launch(w4_dequantize_kernel<T, __nv_bfloat16>, grid, kW4PackThreads, 0, 1, s, f, data,
+                     static_cast<__nv_bfloat16*>(out), ld, vec);
+  if (dtype == MK_FP16)
+    return w4_launch(w4_dequantize_kernel<T, __half>, grid, kW4PackThreads, 0, 1, s, f, data, static_cast<__half*>(out),
+                     ld, vec);
+  return w4_launch(w4_dequantize_kernel<T, float>, grid, kW4PackThreads, 0, 1, s, f, data, static_cast<float*>(out), ld,
+                   vec);
 }
 
 static int w4_dtype_size(int dtype) { return dtype == MK_FP32 ? 4 : 2; }
@@ -878,10 +883,8 @@ int mk_w4_pack(const mk_w4* w, const uint8_t* codes, const void* scales, const u
   p.zero_points = zero_points;
   const dim3 grid(p.form.blocks, p.form.strips, 1);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (w->dtype == MK_BF16) w4_pack_kernel<__nv_bfloat16><<<grid, kW4PackThreads, 0, s>>>(p);
-  else w4_pack_kernel<__half><<<grid, kW4PackThreads, 0, s>>>(p);
-  MKB_CUDA(cudaGetLastError());
-  return MK_OK;
+  return w->dtype == MK_BF16 ? w4_launch(w4_pack_kernel<__nv_bfloat16>, grid, kW4PackThreads, 0, 1, s, p)
+                             : w4_launch(w4_pack_kernel<__half>, grid, kW4PackThreads, 0, 1, s, p);
 }
 
 int mk_w4_quantize(const mk_w4* w, const void* src, long long ld, int src_dtype, void* stream) {
