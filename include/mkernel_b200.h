@@ -177,8 +177,8 @@ int mk_gemm_ar_launch(const void* A, const void* B, const mk_symm_view* C,
  *   w[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group].
  * `data` is a device buffer of mk_w4_bytes() bytes, 16-byte aligned, in the library's own layout;
  * mk_w4_pack or mk_w4_quantize fills it once.  dtype is the type of the scales and of the
- * activations that the products take.  N and K may be any positive number; a group that reaches
- * past K is short.  The struct itself is read during the call only. */
+ * activations that the products take.  N (up to 4194240) and K (up to 2^30) need no divisor; a group
+ * that reaches past K is short.  The struct itself is read during the call only. */
 #define MK_BF16 0
 #define MK_FP16 1
 #define MK_FP32 2
@@ -227,7 +227,9 @@ int mk_align_rows(const void* src, long long ld, int rows, int cols, void* dst, 
  * rounded once.  M = 0 does nothing.  w->form = MK_W4_PLAIN.
  * For M <= 16 the products are of the weights as they are.  For more the weights are rounded to w's
  * dtype first, as mk_w4_dequantize gives them (not in the SwiGLU form, which takes what the rounding
- * leaves as well), and rows of A must start on 16 bytes (A aligned, lda a multiple of 8). */
+ * leaves as well) -- one beyond the dtype's range, and any with a bf16 scale of 2^121 or more, is not finite
+ * there --, and rows of A must start on 16 bytes (A aligned, lda a multiple of 8).
+ * C and A share no memory.  A device wait that runs out (see "wait_limit_ms") leaves NaN in C. */
 int mk_w4_gemm(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
                void* stream);
 /* H[M, N/2] = silu(A * G^T) * (A * U^T) with w->form = MK_W4_GATE_UP: the single-token form of

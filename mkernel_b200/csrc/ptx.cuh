@@ -358,17 +358,13 @@ __device__ __forceinline__ void umma_kblock(uint32_t d_tmem, uint32_t a_lo, uint
         : "memory");
   }
 }
-// MMAs of 16-bit operands whose A operand lies in tensor memory, N = 2 or 4 of them along K (8 columns of A,
-// 32 bytes of B each), by the elected lane of a converged warp.  `accumulate` = 0 makes the first one
-// overwrite the accumulator.
-template <int N>
+// Four MMAs of 16-bit operands along K (8 columns of A, 32 bytes of B each) whose A operand lies in tensor memory,
+// by the elected lane of a converged warp.  `accumulate` = 0 makes the first one overwrite the accumulator.
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t desc_hi,
                                         uint32_t idesc, uint32_t accumulate) {
-  static_assert(N == 2 || N == 4, "");
   asm volatile(
-      "{\n\t.reg .pred pe, pa, pm;\n\t.reg .b64 db;\n\t.reg .b32 ra, rb;\n\t"
+      "{\n\t.reg .pred pe, pa;\n\t.reg .b64 db;\n\t.reg .b32 ra, rb;\n\t"
       "elect.sync _|pe, 0xffffffff;\n\t"
-      "setp.ne.and.b32 pm, %6, 0, pe;\n\t"
       "setp.ne.b32 pa, %5, 0;\n\t"
       "mov.b64 db, {%2, %3};\n\t"
       "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, pa;\n\t"
@@ -380,16 +376,16 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32
       "add.u32 ra, ra, 8;\n\t"
       "add.u32 rb, rb, 2;\n\t"
       "mov.b64 db, {rb, %3};\n\t"
-      "@pm tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %4, pa;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %4, pa;\n\t"
       "add.u32 ra, ra, 8;\n\t"
       "add.u32 rb, rb, 2;\n\t"
       "mov.b64 db, {rb, %3};\n\t"
-      "@pm tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %4, pa;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %4, pa;\n\t"
       "}\n"
-      ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate), "r"(N == 4 ? 1u : 0u)
+      ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 16 lanes x N / 4 times 8 columns: thread (g, t) = (lane / 4, lane % 4) holds, of each eight columns,
+// 16 lanes x 4 times 8 columns: thread (g, t) = (lane / 4, lane % 4) holds, of each eight columns,
 // columns 2 t and 2 t + 1 of lanes g and g + 8.
 __device__ __forceinline__ void tmem_st_16x256(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -398,15 +394,6 @@ __device__ __forceinline__ void tmem_st_16x256(uint32_t taddr, const uint32_t (&
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-__device__ __forceinline__ void tmem_st_16x256(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-__device__ __forceinline__ void tmem_st_16x256(uint32_t taddr, const uint32_t (&r)[4]) {
-  asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%0], {%1, %2, %3, %4};"
-               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");

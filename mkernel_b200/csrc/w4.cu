@@ -397,7 +397,7 @@ __device__ __forceinline__ void w4_mma(float (&d)[4], const uint32_t (&a)[4], ui
   }
 }
 
-// C^T = W A^T with the weights as the 16-row operand and up to 8 NT tokens as columns.  A warp takes
+// C^T = W A^T with the weights as the 16-row operand and the tokens, at most 8 NT, as columns.  A warp takes
 // every so many-th chunk of one strip; codes go to the matrix instruction as whole numbers
 // (code - zero, times a power of two), which the 16-bit types hold exactly.  The sums of a group are exact products
 // added in fp32, then times the group's scale in fp32: no weight is rounded on the way.  The warps
@@ -427,7 +427,8 @@ __device__ __forceinline__ int w4_x_slot(int token, int slot) { return token * 2
 // x: column 8 t of this lane's token (g of each eight); x_to: where its columns 8 t and 32 + 8 t go.
 template <int NT, int TILES, int TAIL>
 __device__ __forceinline__ void w4_fill(const W4Params& p, const uint8_t* chunk, const uint8_t* tail,
-                                        int block, int token0, const uint16_t* const (&x)[NT], const bool (&have)[NT], const int (&x_to)[2], uint32_t stage, uint8_t* stage_ptr, int lane) {
+                                        int block, const uint16_t* const (&x)[NT], const bool (&have)[NT],
+                                        const int (&x_to)[2], uint32_t stage, uint8_t* stage_ptr, int lane) {
   const uint32_t dst = stage + lane * 16;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
@@ -450,12 +451,12 @@ __device__ __forceinline__ void w4_fill(const W4Params& p, const uint8_t* chunk,
     // The last block of K, and rows that no 16-byte access can start on: lanes take consecutive
     // elements.  Columns behind K are zeroed, so that no product there is a NaN.
     const uint16_t* A = static_cast<const uint16_t*>(p.A) + k0 + lane;
-    const int tokens = min(NT * 8, p.M - token0);
+    const int tokens = p.M;
     for (int m0 = 0; m0 < tokens; m0 += 8) {
       uint16_t v[8][4];
 #pragma unroll
       for (int m = 0; m < 8; ++m) {
-        const uint16_t* row = A + (long long)(token0 + m0 + m) * p.lda;
+        const uint16_t* row = A + (long long)(m0 + m) * p.lda;
 #pragma unroll
         for (int hq = 0; hq < 4; ++hq)
           v[m][hq] = m0 + m < tokens && k0 + hq * 32 + lane < p.form.K ? __ldg(row + hq * 32) : (uint16_t)0;
@@ -495,7 +496,6 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
   const int strip = blockIdx.x / p.split / (4 / TILES);
   const int tile0 = blockIdx.x / p.split % (4 / TILES) * TILES;
   const int rank = blockIdx.x % p.split;
-  const int token0 = blockIdx.y * 8 * NT;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* const ring_ptr = smem + warp * p.stage_bytes * kW4Stages;
   const uint32_t ring = ptx::smem_u32(ring_ptr);
@@ -520,11 +520,11 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
   // their lanes read another token's activations.
   const uint16_t* x[NT];
   bool have[NT];
-  const int last = min(NT * 8, p.M - token0) - 1;
+  const int last = p.M - 1;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     have[n] = n * 8 + g <= last;
-    x[n] = static_cast<const uint16_t*>(p.A) + (long long)(token0 + (have[n] ? n * 8 + g : 0)) * p.lda + 8 * t;
+    x[n] = static_cast<const uint16_t*>(p.A) + (long long)(have[n] ? n * 8 + g : 0) * p.lda + 8 * t;
   }
   const int gx = min(g, last);
   const int x_to[2] = {kCodes + kTail + w4_x_slot(gx, t >> 1) + (t & 1) * 16,
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
 #pragma unroll
   for (int i = 0; i < kW4Stages; ++i) {
     if (first + i * step < f.blocks)
-      w4_fill<NT, TILES, kTail>(p, chunk, tail, first + i * step, token0, x, have, x_to,
+      w4_fill<NT, TILES, kTail>(p, chunk, tail, first + i * step, x, have, x_to,
                                 ring + i * p.stage_bytes, ring_ptr + i * p.stage_bytes, lane);
     chunk += chunk_step;
     tail += chunk_step;
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
     __syncwarp();
     const int ahead = block + kW4Stages * step;
     if (ahead < f.blocks)
-      w4_fill<NT, TILES, kTail>(p, chunk, tail, ahead, token0, x, have, x_to, ring + at, ring_ptr + at,
+      w4_fill<NT, TILES, kTail>(p, chunk, tail, ahead, x, have, x_to, ring + at, ring_ptr + at,
                                 lane);
     chunk += chunk_step;
     tail += chunk_step;
@@ -626,7 +626,14 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
     at = at == 0 ? p.stage_bytes : 0;
   }
 
-  // the warp's sums over its own ring, which nothing is copied into any more
+  // The first result's angle is worked out while other warps still multiply.
+  const int entry = rank * (warps * 32) + threadIdx.x;
+  W4Turn turn = {};
+  if (p.epilogue == W4_EPI_ROTARY && entry < p.M * 8 * TILES)
+    turn = w4_turn(p, strip, tile0 * 8 + entry % (8 * TILES), entry / (8 * TILES));
+  // The warp's sums over its own ring, which nothing is copied into any more and which has room for them: at least
+  // 2816 bytes for 8 tokens' 2176, and from 9 tokens on 6912 for 4352.
+  static_assert(2 * w4_stage_bytes(kW4CodeBytes + 128, 1, NT == 1 ? 1 : 9) >= NT * 8 * kW4Pitch * 8, "room for the sums");
   float2* red = reinterpret_cast<float2*>(ring_ptr);
   __syncwarp();
 #pragma unroll
@@ -641,9 +648,8 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
   else __syncthreads();
   // the CTAs of a cluster share the entries of the result among themselves
   const uint32_t red0 = ptx::smem_u32(smem);
-  for (int e = rank * (warps * 32) + threadIdx.x; e < NT * 8 * 8 * TILES; e += step * 32) {
+  for (int e = entry; e < p.M * 8 * TILES; e += step * 32) {
     const int token = e / (8 * TILES), pair = e % (8 * TILES);
-    if (token0 + token >= p.M) break;
     float2 v = make_float2(0.0f, 0.0f);
     for (int c = 0; c < p.split; ++c) {
       const uint32_t base = p.split > 1 ? ptx::map_to_cta(red0, c) : red0;
@@ -654,7 +660,8 @@ __global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __
         v.y += a.y;
       }
     }
-    w4_epilogue<T>(p, strip, tile0 * 8 + pair, token0 + token, v);
+    if (p.epilogue == W4_EPI_ROTARY && e != entry) turn = w4_turn(p, strip, tile0 * 8 + pair, token);
+    w4_epilogue<T>(p, strip, tile0 * 8 + pair, token, v, turn);
   }
   if (p.split > 1) ptx::cluster_sync_all();   // nobody leaves while its shared memory is read
 }
@@ -704,6 +711,7 @@ static int w4_check(const mk_w4* w, const char* what, bool need_data) {
   const W4Form f = w4_form(*w);
   if (f.strips > 65535)
     return set_error(MK_ERR_INVALID, "%s: N=%d is above %d", what, w->N, 65535 * kW4Strip);
+  if (w->K > 1 << 30) return set_error(MK_ERR_INVALID, "%s: K=%d is above %d", what, w->K, 1 << 30);
   if (need_data && (!w->data || (reinterpret_cast<uintptr_t>(w->data) & 15) != 0))
     return set_error(MK_ERR_INVALID, "%s: packed weights must be a 16-byte aligned device buffer", what);
   return MK_OK;
@@ -711,31 +719,26 @@ static int w4_check(const mk_w4* w, const char* what, bool need_data) {
 
 // How the few-token product is cut.  All choices follow from how many CTAs there are to fill the SMs;
 // figures are microseconds, 1 token, bf16, group 128, medians of graph replays.
-struct W4StreamPlan { int nt, tiles, warps, split, stage_bytes; long long token_tiles, ctas; };
+struct W4StreamPlan { int nt, tiles, warps, split, ctas, stage_bytes; };
 
 static W4StreamPlan w4_stream_plan(const W4Form& f, int M, int sms) {
   W4StreamPlan pl;
   pl.nt = M <= 8 ? 1 : 2;
-  pl.token_tiles = ((long long)M + 8 * pl.nt - 1) / (8 * pl.nt);
-  const long long units = f.strips * pl.token_tiles;
   // Four tiles of rows to a warp share each load of activations, but a narrow matrix gives too few
   // CTAs then: 1280 x 8192 takes 5.6 with 4 tiles (cut along K into clusters), 5.1 with 2, 4.5 with 1;
   // 3584 x 8192: 6.9, 6.1, 7.0; 8192 x 8192: 9.1, 10.0, 12.3.
-  pl.tiles = units * 2 > sms ? 4 : units * 4 > sms ? 2 : 1;
-  pl.ctas = (long long)f.strips * (4 / pl.tiles);
+  pl.tiles = f.strips * 2 > sms ? 4 : f.strips * 4 > sms ? 2 : 1;
+  pl.ctas = f.strips * (4 / pl.tiles);
   // One CTA to an SM brings as many warps as fit; more CTAs than SMs share them with fewer (28672 x
   // 8192: 28 with 8 warps, 36 with 16).  A warp without a chunk is of no use.
-  pl.warps = pl.ctas * pl.token_tiles > sms ? 8 : pl.nt == 1 ? 16 : 12;
+  pl.warps = pl.ctas > sms ? 8 : pl.nt == 1 ? 16 : 12;
   if (pl.warps > f.blocks) pl.warps = f.blocks < 4 ? 4 : f.blocks;
   // Clusters along K only where most SMs would be idle: one costs 0.7 (1024 x 1024: 2.1 and 2.9).
   pl.split = 1;
-  while (pl.split < 8 && pl.ctas * pl.token_tiles * pl.split * 4 <= sms && pl.split * 16 <= f.blocks) pl.split *= 2;
+  while (pl.split < 8 && pl.ctas * pl.split * 4 <= sms && pl.split * 16 <= f.blocks) pl.split *= 2;
   if (pl.split > 1) pl.warps = 8;
   pl.ctas *= pl.split;
-  pl.stage_bytes = w4_stage_bytes(f.chunk_bytes, pl.tiles, M < 8 * pl.nt ? M : 8 * pl.nt);
-  // a warp leaves its sums in its ring
-  const int sums = 8 * pl.nt * kW4Pitch * 8;
-  if (pl.stage_bytes * kW4Stages < sums) pl.stage_bytes = sums / kW4Stages;
+  pl.stage_bytes = w4_stage_bytes(f.chunk_bytes, pl.tiles, M);
   return pl;
 }
 
@@ -790,6 +793,10 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
                      w->K, n_out);
   if (((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(C)) & 1) != 0)
     return set_error(MK_ERR_INVALID, "%s: operands must be 2-byte aligned", what);
+  const bool vec = (reinterpret_cast<uintptr_t>(A) & 15) == 0 && (lda % 8 == 0 || M == 1);
+  if (M > 16 && !vec)
+    return set_error(MK_ERR_INVALID, "%s: for more than 16 rows A's must start on 16 bytes (mk_align_rows copies them so)",
+                     what);
   int sms = 0;
   rc = device_sm_count(&sms);
   if (rc != MK_OK) return rc;
@@ -798,23 +805,18 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.form = w4_form(*w);
   p.data = static_cast<const uint8_t*>(w->data);
   p.A = A; p.lda = lda; p.C = C; p.ldc = ldc; p.M = M;
-  p.vec = (reinterpret_cast<uintptr_t>(A) & 15) == 0 && (lda % 8 == 0 || M == 1);
+  p.vec = vec;
   p.epilogue = epilogue;
   p.rotary = rotary;
-  p.wide = (reinterpret_cast<uintptr_t>(C) & 7) == 0 && ldc % 4 == 0 && (form != MK_W4_GATE_UP || w->N / 2 % 4 == 0);
+  p.wide = (reinterpret_cast<uintptr_t>(C) & 7) == 0 && ldc % 4 == 0;
   p.wait_limit_ns = option_wait_limit_ns();
   // Up to 16 tokens the stream kernel is bound by memory as it should be; every 16 more cost it another
   // pass over the weights.
-  if (M > 16 && !p.vec)
-    return set_error(MK_ERR_INVALID, "%s: for more than 16 rows A's must start on 16 bytes (mk_align_rows copies them so)",
-                     what);
   if (M > 16) return w4_tile_launch(p, w->dtype, sms, static_cast<cudaStream_t>(stream));
   const W4StreamPlan pl = w4_stream_plan(p.form, M, sms);
   p.stage_bytes = pl.stage_bytes;
   p.split = pl.split;
-  if (pl.token_tiles > 65535 || pl.ctas > 0x7fffffffLL)
-    return set_error(MK_ERR_INVALID, "%s: M=%d, N=%d is too large", what, M, w->N);
-  const dim3 grid((unsigned)pl.ctas, (unsigned)pl.token_tiles, 1);
+  const dim3 grid(pl.ctas, 1, 1);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return w->dtype == MK_BF16 ? w4_stream_type<__nv_bfloat16>(p, pl, grid, s)
                              : w4_stream_type<__half>(p, pl, grid, s);

@@ -39,9 +39,18 @@ __device__ __forceinline__ uint32_t w4_round2(float a, float b, __half) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// C's entries of one pair of rows and one token.
+// Whether a pair of rows is turned for a token, and by which cosine and sine.
+struct W4Turn { bool on; float2 angle; };
+__device__ __forceinline__ W4Turn w4_turn(const W4Params& p, int strip, int pair, int token) {
+  const W4Form& f = p.form;
+  const int half = f.head_dim / 2, index = strip * (kW4Strip / 2) + pair, head = index / half, i = index - head * half;
+  if (head >= f.rotated_heads || i >= f.rotary_dim / 2) return {false, make_float2(1.0f, 0.0f)};
+  return {true, rotary_cos_sin(rotary_position(p.rotary, token), __ldg(p.rotary.inv_freq + i), p.rotary.scale)};
+}
+
+// C's entries of one pair of rows and one token.  turn: w4_turn, in the rotary form.
 template <typename T>
-__device__ __forceinline__ void w4_epilogue(const W4Params& p, int strip, int pair, int token, float2 v) {
+__device__ __forceinline__ void w4_epilogue(const W4Params& p, int strip, int pair, int token, float2 v, const W4Turn& turn) {
   const W4Form& f = p.form;
   const int n0 = w4_row(f, strip, pair, 0);
   if (n0 < 0) return;
@@ -51,13 +60,7 @@ __device__ __forceinline__ void w4_epilogue(const W4Params& p, int strip, int pa
     return;
   }
   const int n1 = w4_row(f, strip, pair, 1);
-  if (p.epilogue == W4_EPI_ROTARY) {
-    const int half = f.head_dim / 2;
-    const int index = strip * (kW4Strip / 2) + pair, head = index / half, i = index % half;
-    if (head < f.rotated_heads && i < f.rotary_dim / 2)
-      v = rotary_turn(v.x, v.y, rotary_cos_sin(rotary_position(p.rotary, token),
-                                               __ldg(p.rotary.inv_freq + i), p.rotary.scale));
-  }
+  if (turn.on) v = rotary_turn(v.x, v.y, turn.angle);
   row[n0] = W4Traits<T>::from_float(v.x);
   if (n1 >= 0) row[n1] = W4Traits<T>::from_float(v.y);
 }
@@ -110,7 +113,7 @@ __device__ __forceinline__ void w4_epilogue4(const W4Params& p, int strip, int p
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w4_epilogue<T>(p, strip, pair + i, token, make_float2(a[i], b[i]));
+  for (int i = 0; i < 4; ++i) w4_epilogue<T>(p, strip, pair + i, token, make_float2(a[i], b[i]), {});
 }
 
 template <typename K, typename... Args>

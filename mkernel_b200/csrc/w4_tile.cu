@@ -237,11 +237,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (!ok) break;
       ptx::tc_fence_after();
       const uint32_t a = tmem_a + operand * kOperand, b_lo = b_lo0 + s * (p.stage_bytes >> 4);
-      ptx::umma_ts<4>(d, a, b_lo, desc_hi, idesc, b >= kSums ? 1u : 0u);
-      ptx::umma_ts<4>(d, a + 32, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
+      ptx::umma_ts(d, a, b_lo, desc_hi, idesc, b >= kSums ? 1u : 0u);
+      ptx::umma_ts(d, a + 32, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
       if (REST) {
-        ptx::umma_ts<4>(d, a + 64, b_lo, desc_hi, idesc, 1);
-        ptx::umma_ts<4>(d, a + 96, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
+        ptx::umma_ts(d, a + 64, b_lo, desc_hi, idesc, 1);
+        ptx::umma_ts(d, a + 96, b_lo + (kXHalf >> 4), desc_hi, idesc, 1);
       }
       if (kOwn) ptx::umma_commit_elect<1>(a_empty(operand), 0);
       ptx::umma_commit_elect<1>(empty(s), 0);
@@ -394,14 +394,14 @@ int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
   for (int i = 0; i < 4; ++i)
     for (int split = 1; split <= 8 && split <= f.blocks; split *= 2) {
       const int t = 32 << i;
-      const long long units = row_tiles * ((p.M + t - 1) / t) * split;
+      const long long units = row_tiles * (((long long)p.M + t - 1) / t) * split;
       const long long waves = (units + sms - 1) / sms;
       if (split > 1 && waves > 1) continue;
       const long long each = (long long)((f.blocks + split - 1) / split) * block_ns[rest][i] + ends_ns[i];
       const long long cost = waves * each + (split > 1 ? 750 * split : 0);
       if (best < 0 || cost < best) { best = cost; tokens = t; p.split = split; }
     }
-  p.token_tiles = (p.M + tokens - 1) / tokens;
+  p.token_tiles = (int)(((long long)p.M + tokens - 1) / tokens);
   p.stage_bytes = (tokens * 256 + 2 * f.chunk_bytes + 1023) / 1024 * 1024;
   CUtensorMap map;
   const int rc = w4_tile_map(&map, p, dtype, tokens);

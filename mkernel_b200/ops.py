@@ -174,6 +174,7 @@ class W4Weight:
     def __init__(self, N: int, K: int, group: int, dtype: torch.dtype, zero_points: bool, device,
                  form: str = "plain", head_dim: int = 0, rotary_dim: int = 0, rotated_heads: int = 0,
                  interleaved: bool = False):
+        _require(0 < N <= 0x7fffffff and 0 < K <= 0x7fffffff, f"bad shape [{N}, {K}]")
         if form not in _W4_FORMS:
             _require(False, f"form must be one of {sorted(_W4_FORMS)}")
         _require(dtype in (torch.bfloat16, torch.float16), "4-bit weights have bfloat16 or float16 scales")
@@ -270,8 +271,8 @@ def _w4_launch(call, A: torch.Tensor, W: W4Weight, C: torch.Tensor, form: str, *
     if (a_stride[1] != 1 and K != 1) or (c_stride[1] != 1 and n_out != 1):
         _require(False, "rows of A and C must be contiguous")
     lda, ldc = (a_stride[0], c_stride[0]) if M > 1 else (K, n_out)     # one row may have any stride
-    if M > 1 and ldc < n_out:
-        _require(False, "rows of C overlap")
+    if M > 1 and (ldc < n_out or M > 0x7fffffff):
+        _require(False, "rows of C overlap, or are more than 2^31 - 1")
     a = A.data_ptr()
     if (a & 15 or (lda & 7 and M > 1)) and (M > 16 or M * K > 32768):
         # Rows that no 16-byte access can start on: more than 16 are copied, and few where a launch costs less
@@ -286,7 +287,7 @@ def _w4_launch(call, A: torch.Tensor, W: W4Weight, C: torch.Tensor, form: str, *
 
 def w4_gemm(A: torch.Tensor, W: W4Weight, C: torch.Tensor) -> None:
     """C[M, N] = A[M, K] @ W^T with 4-bit weights: the single-token and small-batch form of
-    ``gemm_bf16``.  A and C in the type of W's scales, any row strides; fp32 sums, rounded once.
+    ``gemm_bf16``.  A and C in the type of W's scales, any row strides, sharing no memory; fp32 sums, rounded once.
     For more than 16 rows the weights are rounded to that type first, as ``W.dequantize()`` gives them."""
     _w4_launch(_lib.lib().mk_w4_gemm, A, W, C, "plain")
 
@@ -336,6 +337,8 @@ def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
         _require(False, "X must be a CUDA tensor [rows, heads, head_dim] of bfloat16, float16 or float32")
     shape, xs, index, dtype, x = X.shape, X.stride(), X.get_device(), X.dtype, X.data_ptr()
     rows, heads, dim = shape
+    if heads > 0x7fffffff or dim > 0x7fffffff:
+        _require(False, "too many heads or features")
     if Y is None or Y is X:
         Y, ys, y = X, xs, x
     else:

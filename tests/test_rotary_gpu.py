@@ -152,7 +152,8 @@ def test_refusals():
     for args in ((X.double(), pos, freq), (X[0], pos, freq), (X, pos[:3], freq), (X, pos.float(), freq),
                  (X, pos, torch.ones(9, device=DEV)), (X, pos, freq.half()), (X, pos.cpu(), freq),
                  (X.transpose(1, 2), pos, freq), (X, pos, freq, X[:, :1]), (X, pos, freq, X.float()),
-                 (X, pos, torch.ones(0, device=DEV))):
+                 (X, pos, torch.ones(0, device=DEV)),
+                 (torch.zeros((4, 1, 4200), device=DEV, dtype=BF), pos, torch.ones(2050, device=DEV))):
         with pytest.raises(RuntimeError):
             ops.rotary(*args)
     both = torch.zeros((4, 4, 16), device=DEV, dtype=BF)

@@ -60,6 +60,12 @@ def test_bad_operands_are_refused():
     assert lib.mk_w4_quantize(ok, 4098, 128, 2, None) == -1
     assert lib.mk_w4_dequantize(ok, None, 128, 0, None) == -1
     assert lib.mk_w4_dequantize(ok, 4096, 128, 7, None) == -1
+    assert lib.mk_w4_bytes(ctypes.byref(view(N=65536 * 64, K=64))) == -1
+    assert lib.mk_w4_bytes(ctypes.byref(view(N=64, K=(1 << 30) + 1))) == -1
+    assert lib.mk_w4_bytes(ctypes.byref(view(N=64, K=1 << 30))) == (1 << 23) * (4096 + 128 * 128 // view().group)
+    assert lib.mk_w4_gemm(4098, 128, ok, 4096, 64, 17, None) == -1      # rows that start on no 16 bytes
+    assert lib.mk_w4_gemm(4096, 132, ok, 4096, 64, 17, None) == -1
+    assert "mk_align_rows" in _lib.last_error()
     assert lib.mk_align_rows(4096, 100, 2, 101, 8192, 104, None) == -1
     assert lib.mk_align_rows(4096, 100, 2, 100, 8192, 100, None) == -1
     assert lib.mk_align_rows(4096, 100, 2, 100, 8200, 104, None) == -1

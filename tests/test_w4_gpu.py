@@ -307,6 +307,80 @@ def test_step_on_a_stream_and_in_a_graph():
         check(y, got_h.double() @ wd.t(), slack(got_h, wd), BF)
 
 
+@pytest.mark.parametrize("M", [1, 4, 12, 40])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_features_that_do_not_turn_do_not_mix(M, interleaved):
+    """An infinite feature of a head that is not turned, or behind rotary_dim, leaves its neighbours as they are."""
+    heads, D, rot, K = 4, 24, 16, 256
+    codes, scales, zp, w = weights(heads * D, K, 128, False, BF, seed=22)
+    bad = [0 * D + 17, 2 * D + 2, 3 * D + 5, 3 * D + 20]          # heads 2 and 3 are not turned
+    scales[bad] = float("inf")
+    W = pack(codes, scales, zp, False, form="rotary", head_dim=D, rotary_dim=rot, rotated_heads=2,
+             interleaved=interleaved)
+    C = torch.empty((M, heads * D), device=DEV, dtype=BF)
+    freq = torch.ones(rot // 2, device=DEV)
+    ops.w4_gemm_rotary(activations(M, K, BF).to(DEV), W, C, torch.arange(M, device=DEV), freq)
+    finite = torch.isfinite(C.cpu())
+    want = torch.ones(heads * D, dtype=torch.bool)
+    want[bad] = False
+    assert torch.equal(finite, want.expand(M, -1))
+
+
+@pytest.mark.parametrize("M", [1, 12, 32, 60, 128, 256, 300])
+@pytest.mark.parametrize("form", ["plain", "gate_up"])
+def test_many_launches_back_to_back(M, form):
+    """A long K (many turns at every stage of the ring), launches on one another's heels, all the same."""
+    N, K = 1024, 8192
+    codes, scales, zp, w = weights(N, K, 64, True, BF, seed=18)
+    W = pack(codes, scales, zp, True, form=form)
+    x = activations(M, K, BF, seed=19)
+    xd, n_out = x.to(DEV), N if form == "plain" else N // 2
+    outs = [torch.empty((M, n_out), device=DEV, dtype=BF) for _ in range(4)]
+    call = ops.w4_gemm if form == "plain" else ops.w4_gemm_swiglu
+    for i in range(200):
+        call(xd, W, outs[i % 4])
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    first = outs[0].clone()
+    with torch.cuda.graph(graph, stream=s):
+        for i in range(40):
+            call(xd, W, outs[i % 4])
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first) for o in outs)
+    if form == "plain":
+        wh = held(w, BF, M)
+        check(first, x.double() @ wh.t(), slack(x, wh), BF)
+
+
+def test_long_prompt():
+    M, N, K = 1500, 200, 384
+    codes, scales, zp, w = weights(N, K, 128, False, HF, seed=20)
+    x, w = activations(M, K, HF), w.to(HF).double()
+    C = torch.empty((M, N), device=DEV, dtype=HF)
+    ops.w4_gemm(x.to(DEV), pack(codes, scales, zp, False), C)
+    check(C, x.double() @ w.t(), slack(x, w), HF)
+
+
+def test_two_streams_share_the_weights():
+    codes, scales, zp, w = weights(512, 1024, 128, False, BF, seed=21)
+    W = pack(codes, scales, zp, False)
+    x = activations(64, 1024, BF)
+    xd = x.to(DEV)
+    one, both = torch.empty((64, 512), device=DEV, dtype=BF), []
+    ops.w4_gemm(xd, W, one)
+    torch.cuda.synchronize()
+    for s in (torch.cuda.Stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                C = torch.empty((64, 512), device=DEV, dtype=BF)
+                ops.w4_gemm(xd, W, C)
+            both.append(C)
+    torch.cuda.synchronize()
+    assert torch.equal(both[0], one) and torch.equal(both[1], one)
+
+
 def test_mlp_of_a_few_tokens():
     """TpMlp.forward_tokens: the framework's MLP with its weights in 4 bits, beside its bf16 form."""
     M, K, I, N = 128, 192, 256, 136
