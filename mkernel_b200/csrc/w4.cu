@@ -37,8 +37,8 @@ struct W4PackParams {
 
 struct W4Unit { int pair, col; };   // columns col .. col + 7 and col + 32 .. col + 39 of the block
 __device__ __forceinline__ W4Unit w4_unit() {
-  const int t = threadIdx.x & 3;
-  return {(int)threadIdx.x >> 3, (threadIdx.x >> 2 & 1) * 64 + (t & 1) * 16 + (t >> 1) * 8};
+  const int t = (int)threadIdx.x & 3;
+  return {(int)threadIdx.x >> 3, ((int)threadIdx.x >> 2 & 1) * 64 + (t & 1) * 16 + (t >> 1) * 8};
 }
 // Place of the lane that the unit's thread has after the exchange: t = thread % 4.
 __device__ __forceinline__ int w4_unit_offset(const W4Unit& u) {

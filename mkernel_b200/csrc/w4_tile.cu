@@ -382,21 +382,57 @@ static int w4_tile_map(CUtensorMap* map, const W4Params& p, int dtype, int token
   return MK_OK;
 }
 
+// How many clusters of 2, 4 or 8 CTAs run at once on the current device: fewer than its SMs give room for, since
+// the CTAs of one share a part of the chip (of 4: 33 on 148 SMs).  All instances take an SM to a CTA.
+static int w4_tile_clusters(int split, int* out) {
+  static int cached[64][9];
+  int dev = 0;
+  MKB_CUDA(cudaGetDevice(&dev));
+  const bool keep = dev >= 0 && dev < 64;
+  if (!keep || cached[dev][split] == 0) {
+    auto kern = w4_tile_kernel<__nv_bfloat16, 64, 128, false>;
+    const int smem = 200 * 1024;
+    MKB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split, 1, 1);
+    cfg.blockDim = dim3(kTileThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MKB_CUDA(cudaOccupancyMaxActiveClusters(out, kern, &cfg));
+    if (keep) cached[dev][split] = *out;
+    return MK_OK;
+  }
+  *out = cached[dev][split];
+  return MK_OK;
+}
+
 int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
   const W4Form& f = p.form;
   const long long row_tiles = (f.strips + 1) / 2;
   // Tokens to a CTA and CTAs to a cluster along K: whichever finishes first by what a block and a start and end
-  // take in ns (measured at 32, 64, 128 and 256 tokens; 1.5 us more for a cluster of two).
+  // take in ns (measured at 32, 64, 128 and 256 tokens; 1.5 us more for a cluster of two).  Clusters only where
+  // all of them run at once: 64 tokens of 4608 x 4096 take 18.2 us in 36 clusters of 4, 10.5 in 36 of 2.
   const bool rest = p.epilogue == W4_EPI_SWIGLU;
   const int block_ns[2][4] = {{280, 290, 370, 500}, {400, 540, 800, 1250}}, ends_ns[4] = {3000, 3000, 4500, 8000};
   int tokens = 128;
   long long best = -1;
+  int clusters[9] = {};
+  for (int split = 2; split <= 8; split *= 2) {
+    const int rc = w4_tile_clusters(split, &clusters[split]);
+    if (rc != MK_OK) return rc;
+  }
   for (int i = 0; i < 4; ++i)
     for (int split = 1; split <= 8 && split <= f.blocks; split *= 2) {
       const int t = 32 << i;
-      const long long units = row_tiles * (((long long)p.M + t - 1) / t) * split;
-      const long long waves = (units + sms - 1) / sms;
-      if (split > 1 && waves > 1) continue;
+      const long long units = row_tiles * (((long long)p.M + t - 1) / t);
+      if (split > 1 && units > clusters[split]) continue;
+      const long long waves = (units * split + sms - 1) / sms;
       const long long each = (long long)((f.blocks + split - 1) / split) * block_ns[rest][i] + ends_ns[i];
       const long long cost = waves * each + (split > 1 ? 750 * split : 0);
       if (best < 0 || cost < best) { best = cost; tokens = t; p.split = split; }
