@@ -86,12 +86,31 @@ __device__ __forceinline__ void w4_epilogue4(const W4Params& p, int strip, int p
     }
   }
   if (p.epilogue == W4_EPI_ROTARY) {
-    // the four angles at once, so that their loads and sines overlap
     T* row = static_cast<T*>(p.C) + (long long)token * p.ldc;
     const int half = f.head_dim / 2, n_pairs = f.N / 2;
     int index = strip * (kW4Strip / 2) + pair, head = index / half, at = index - head * half;
     const long long position = rotary_position(p.rotary, token);
     float2 v[4];
+    // Heads of whole fours of pairs, the usual ones: the four turn or do not turn together, and their outputs are
+    // neighbours, in two rows of four or one of eight.
+    if (p.wide && half % 4 == 0 && f.rotary_dim / 2 % 4 == 0) {
+      if (index >= n_pairs) return;
+      const bool rotated = head < f.rotated_heads && at < f.rotary_dim / 2;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = make_float2(a[i], b[i]);
+        if (rotated)
+          v[i] = rotary_turn(a[i], b[i], rotary_cos_sin(position, __ldg(p.rotary.inv_freq + at + i), p.rotary.scale));
+      }
+      const bool apart = rotated && !f.interleaved;
+      T* to = row + head * f.head_dim + (apart ? at : 2 * at);
+      const float2 e[4] = {{v[0].x, apart ? v[1].x : v[0].y}, {apart ? v[2].x : v[1].x, apart ? v[3].x : v[1].y},
+                           {apart ? v[0].y : v[2].x, apart ? v[1].y : v[2].y}, {apart ? v[2].y : v[3].x, v[3].y}};
+      *reinterpret_cast<uint2*>(to) = make_uint2(w4_round2(e[0].x, e[0].y, T()), w4_round2(e[1].x, e[1].y, T()));
+      to += apart ? f.rotary_dim / 2 : 4;
+      *reinterpret_cast<uint2*>(to) = make_uint2(w4_round2(e[2].x, e[2].y, T()), w4_round2(e[3].x, e[3].y, T()));
+      return;
+    }
     int n[4][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

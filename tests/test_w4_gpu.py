@@ -175,6 +175,7 @@ def test_swiglu_far_gates():
 @pytest.mark.parametrize("M,heads,rotated,D,rot,K,dtype", [
     (1, 10, 9, 128, 128, 256, BF), (4, 3, 2, 64, 16, 300, HF), (16, 5, 5, 80, 40, 128, BF),
     (33, 7, 1, 96, 96, 200, HF), (2, 1, 0, 2, 2, 40, BF), (70, 2, 1, 256, 64, 520, BF),
+    (19, 3, 2, 20, 12, 130, BF), (24, 9, 4, 40, 24, 130, HF), (130, 5, 5, 6, 6, 77, BF),
 ])
 def test_rotary_product_matches_definition(M, heads, rotated, D, rot, K, dtype, interleaved):
     codes, scales, zp, w = weights(heads * D, K, 64, True, dtype, seed=6)
