@@ -206,7 +206,7 @@ __device__ __forceinline__ float w4_quotient(float w, float d, float r) {
 // there, and then w4_quotient is exact too, so both go the same way.  Nor a clamp below: the
 // quotient of the largest magnitude is within 2^-8 of 7, that of hi - lo of 15.  Both need a scale that
 // is no subnormal (or 0, when all quotients round to 0); for others, and for fp32 weights, it is divided and
-// clamped as the definition says.
+// clamped as the definition says.  8192 x 8192 in bf16: 39 us, 4.4 TB/s.
 template <typename T, typename S, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParams p) {
   ptx::grid_dependency_wait();
@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParam
 }
 
 // The matrix back from its layout, 8 consecutive columns of a row as one 16-byte store (two for fp32).
-// code - zero times scale is exact in fp32 (5 bits times at most 11), so it is rounded once.
+// code - zero times scale is exact in fp32 (4 bits times at most 11), so it is rounded once.  8192 x 8192 to
+// bf16: 32 us, 5.3 TB/s.
 template <typename T, typename O>
 __global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f, const uint8_t* data, O* out,
                                                                        long long ld, int vec) {
@@ -407,7 +408,9 @@ __device__ __forceinline__ void w4_mma(float (&d)[4], const uint32_t (&a)[4], ui
 // What bounds it is bytes in flight, so a warp keeps kW4Stages chunks, each with the activations that
 // meet it, in a shared-memory ring of its own that asynchronous 16-byte copies fill.  A lane copies
 // just the pieces that it will itself use, so the ring needs no barrier between warps and no
-// registers while the copies fly; lanes meet only over the scales, which four of them share.
+// registers while the copies fly; lanes meet only over the scales, which four of them share.  One token
+// of 8192 x 8192 takes 8.6 us (4.0 TB/s, of which 2 us are a launch and the last CTA's end); an SM then takes in 40
+// bytes a ns, near the 44 that are its share of the memory, and the 128 strips leave 20 SMs without one.
 constexpr int kW4Stages = 2;      // the kernel switches between two offsets
 constexpr int kW4SmemMax = 227 * 1024;
 constexpr int kW4Pitch = 34;   // float2 per token: the four tokens a warp writes at once hit different banks
@@ -718,22 +721,24 @@ static int w4_check(const mk_w4* w, const char* what, bool need_data) {
 }
 
 // How the few-token product is cut.  All choices follow from how many CTAs there are to fill the SMs;
-// figures are microseconds, 1 token, bf16, group 128, medians of graph replays.
+// figures are microseconds, bf16, group 128, 1 token where none are given, medians of graph replays.
 struct W4StreamPlan { int nt, tiles, warps, split, ctas, stage_bytes; };
 
 static W4StreamPlan w4_stream_plan(const W4Form& f, int M, int sms) {
   W4StreamPlan pl;
   pl.nt = M <= 8 ? 1 : 2;
   // Four tiles of rows to a warp share each load of activations, but a narrow matrix gives too few
-  // CTAs then: 1280 x 8192 takes 5.6 with 4 tiles (cut along K into clusters), 5.1 with 2, 4.5 with 1;
-  // 3584 x 8192: 6.9, 6.1, 7.0; 8192 x 8192: 9.1, 10.0, 12.3.
+  // CTAs then: 1280 x 8192 takes 8.4 with 4 tiles, 5.7 with 2, 4.4 with 1; 3584 x 8192: 8.5, 5.8, 7.1;
+  // 8192 x 8192: 8.6, 9.7, 12.3.
   pl.tiles = f.strips * 2 > sms ? 4 : f.strips * 4 > sms ? 2 : 1;
   pl.ctas = f.strips * (4 / pl.tiles);
   // One CTA to an SM brings as many warps as fit; more CTAs than SMs share them with fewer (28672 x
-  // 8192: 28 with 8 warps, 36 with 16).  A warp without a chunk is of no use.
-  pl.warps = pl.ctas > sms ? 8 : pl.nt == 1 ? 16 : 12;
+  // 8192: 28 with 8 warps, 33 with 16; 13 tokens, whose CTAs are larger: 42 with 4, 48 with 8, 50 with 12).  A
+  // warp without a chunk is of no use.
+  pl.warps = pl.ctas > sms ? (pl.nt == 1 ? 8 : 4) : pl.nt == 1 ? 16 : 12;
   if (pl.warps > f.blocks) pl.warps = f.blocks < 4 ? 4 : f.blocks;
-  // Clusters along K only where most SMs would be idle: one costs 0.7 (1024 x 1024: 2.1 and 2.9).
+  // Clusters along K only where most SMs would be idle and a CTA keeps 8 blocks or more: 256 x 8192 takes 4.1
+  // in clusters of 4 and 4.3 without, 1024 x 1024 3.5 in clusters of 2 and 2.1 without.
   pl.split = 1;
   while (pl.split < 8 && pl.ctas * pl.split * 4 <= sms && pl.split * 16 <= f.blocks) pl.split *= 2;
   if (pl.split > 1) pl.warps = 8;
@@ -810,8 +815,9 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.rotary = rotary;
   p.wide = (reinterpret_cast<uintptr_t>(C) & 7) == 0 && ldc % 4 == 0;
   p.wait_limit_ns = option_wait_limit_ns();
-  // Up to 16 tokens the stream kernel is bound by memory as it should be; every 16 more cost it another
-  // pass over the weights.
+  // Up to 16 tokens one pass of the stream kernel over the weights does, and the next 16 would take another: 8192 x
+  // 8192 takes it 13.1 us for 16 tokens and the tile kernel 14.4 for 17 (1024 x 8192: 6.7 and 9.0; 28672 x 8192: 42
+  // and 47).
   if (M > 16) return w4_tile_launch(p, w->dtype, sms, static_cast<cudaStream_t>(stream));
   const W4StreamPlan pl = w4_stream_plan(p.form, M, sms);
   p.stage_bytes = pl.stage_bytes;

@@ -144,8 +144,8 @@ __device__ __forceinline__ void w4_decode(uint32_t word, uint32_t off0, uint32_t
 
 // The same as the weights themselves, rounded to T: (code - zero) * scale.  sc0, sc1: the scales of rows g and
 // g + 8, each twice; off0, off1: their zero points as the layout holds them.  With `rest`, what the rounding
-// left: the two together are the weight exactly (4 bits times at most 11 are 15, the two parts have
-// at least 16).
+// left: the two together are the weight exactly (4 bits times at most 11 are 15, and the two parts have
+// at least 16), down to fp16's smallest subnormal and up to the type's largest number.
 template <typename T>
 struct W4Round;
 template <>
