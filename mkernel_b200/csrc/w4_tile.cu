@@ -324,7 +324,10 @@ template <typename T, int TOKENS, int GROUP, bool REST>
 static int w4_tile_kernel_launch(const W4Params& p, const CUtensorMap& map, unsigned grid, cudaStream_t stream) {
   constexpr int kStages = w4_tile_stages(TOKENS);
   const int ring = kStages * p.stage_bytes, sums = TOKENS * kTilePitch * 4;
-  const int smem = 1024 + kTileControl + (ring > sums ? ring : sums);
+  // More than half of what an SM has, so that two CTAs never share one: the second would wait for the first's
+  // tensor memory, and two clusters might so wait for one another.
+  const int least = 120 * 1024, need = 1024 + kTileControl + (ring > sums ? ring : sums);
+  const int smem = need > least ? need : least;
   auto kern = w4_tile_kernel<T, TOKENS, GROUP, REST>;
   static bool attr_set[64];
   int dev = 0;

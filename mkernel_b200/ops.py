@@ -174,12 +174,14 @@ class W4Weight:
     def __init__(self, N: int, K: int, group: int, dtype: torch.dtype, zero_points: bool, device,
                  form: str = "plain", head_dim: int = 0, rotary_dim: int = 0, rotated_heads: int = 0,
                  interleaved: bool = False):
-        _require(0 < N <= 0x7fffffff and 0 < K <= 0x7fffffff, f"bad shape [{N}, {K}]")
+        if not (0 < N <= 0x7fffffff and 0 < K <= 0x7fffffff):
+            _require(False, f"bad shape [{N}, {K}]")
         if form not in _W4_FORMS:
             _require(False, f"form must be one of {sorted(_W4_FORMS)}")
-        _require(dtype in (torch.bfloat16, torch.float16), "4-bit weights have bfloat16 or float16 scales")
-        _require(form == "rotary" or not (head_dim or rotary_dim or rotated_heads or interleaved),
-                 "head_dim, rotary_dim, rotated_heads and interleaved belong to form 'rotary'")
+        if dtype is not torch.bfloat16 and dtype is not torch.float16:
+            _require(False, "4-bit weights have bfloat16 or float16 scales")
+        if form != "rotary" and (head_dim or rotary_dim or rotated_heads or interleaved):
+            _require(False, "head_dim, rotary_dim, rotated_heads and interleaved belong to form 'rotary'")
         self.shape, self.K, self.group, self.dtype, self.form = (N, K), K, group, dtype, form
         self.n_out = N // 2 if form == "gate_up" else N
         self.zero_points, self.rotary_dim = bool(zero_points), rotary_dim
