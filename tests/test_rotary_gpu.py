@@ -146,6 +146,16 @@ def test_graph_replay_on_another_stream():
         check(Y, x, orc.rotary(x, p, freq.cpu()), 64, False, 1.0, BF)
 
 
+def test_offsets_beyond_32_bits():
+    rows, heads, D = 70000, 256, 128
+    X = torch.zeros((rows, heads, D), device=DEV, dtype=BF)
+    X[-5:] = torch.randn((5, heads, D), device=DEV, dtype=BF)
+    pos, freq = torch.arange(rows, device=DEV), torch.rand(D // 2, device=DEV)
+    small = ops.rotary(X[-5:].clone(), pos[-5:].clone(), freq)
+    ops.rotary(X, pos, freq)
+    assert torch.equal(X[-5:], small) and not X[:-5].any()
+
+
 def test_refusals():
     X = torch.zeros((4, 2, 16), device=DEV, dtype=BF)
     pos, freq = torch.zeros(4, device=DEV, dtype=torch.int64), torch.ones(4, device=DEV)

@@ -364,6 +364,26 @@ def test_long_prompt():
     check(C, x.double() @ w.t(), slack(x, w), HF)
 
 
+def test_offsets_beyond_32_bits():
+    """More than 2^32 bytes of outputs, and of the matrix given back: the last rows are those of a small call."""
+    M, N, K = 70000, 32768, 72
+    x = activations(M, K, BF, seed=23).to(DEV)
+    W = ops.w4_quantize(torch.randn((N, K), device=DEV, dtype=BF), 64)
+    C = torch.empty((M, N), device=DEV, dtype=BF)
+    ops.w4_gemm(x, W, C)
+    last = torch.empty((300, N), device=DEV, dtype=BF)
+    ops.w4_gemm(x[-300:], W, last)
+    assert torch.equal(C[-300:], last)
+    del C
+    big = torch.randn((1, 136), device=DEV, dtype=BF).expand(300, -1).contiguous()
+    src = torch.empty((M, N), device=DEV, dtype=BF)
+    src[-300:, -136:] = big
+    src[-300:, :-136] = 0
+    src[:-300] = 0
+    tail = ops.w4_quantize(src, 32).dequantize()[-300:, -136:]
+    assert torch.equal(tail, ops.w4_quantize(src[-300:], 32).dequantize()[:, -136:]) and tail.abs().sum() > 0
+
+
 def test_two_streams_share_the_weights():
     codes, scales, zp, w = weights(512, 1024, 128, False, BF, seed=21)
     W = pack(codes, scales, zp, False)
