@@ -173,7 +173,7 @@ int mk_gemm_ar_launch(const void* A, const void* B, const mk_symm_view* C,
  * reference.
  *
  * mk_w4 describes a matrix [N, K] of codes 0..15 with one scale (and, with zeros = 1, one whole
- * zero point 0..15; else 8) per row and group of `group` columns:
+ * zero point 0..255; else 8) per row and group of `group` columns:
  *   w[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group].
  * `data` is a device buffer of mk_w4_bytes() bytes, 16-byte aligned, in the library's own layout;
  * mk_w4_pack or mk_w4_quantize fills it once.  dtype is the type of the scales and of the
@@ -204,7 +204,7 @@ typedef struct mk_w4 {
 long long mk_w4_bytes(const mk_w4* w);
 /* Lays out codes [N, (K + 1) / 2] (two per byte, the even column in the low half), scales
  * [N, ceil(K / group)] of w's dtype and zero points (bytes, same shape; NULL when w->zeros = 0).
- * Contiguous device buffers.  A zero point above 15 is taken modulo 16. */
+ * Contiguous device buffers. */
 int mk_w4_pack(const mk_w4* w, const uint8_t* codes, const void* scales, const uint8_t* zero_points,
                void* stream);
 /* Rounds a matrix [N, K] (row stride ld elements, dtype MK_*) to 4 bits.  Without zero points

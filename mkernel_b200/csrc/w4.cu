@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_pack_kernel(W4PackParams p)
         }
         if (col % f.group == 0) {
           scale[j] = __ldg(p.scales + n * groups + k / f.group);
-          if (f.zeros) zero[j] = __ldg(p.zero_points + n * groups + k / f.group) & 15;
+          if (f.zeros) zero[j] = __ldg(p.zero_points + n * groups + k / f.group);
         }
       }
       low[j] = __byte_perm(v & 0x0f0f, (v >> 4) & 0x0f0f, 0x5140);
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParam
 }
 
 // The matrix back from its layout, 8 consecutive columns of a row as one 16-byte store (two for fp32).
-// code - zero times scale is exact in fp32 (4 bits times at most 11), so it is rounded once.  8192 x 8192 to
+// code - zero times scale is exact in fp32 (8 bits times at most 11), so it is rounded once.  8192 x 8192 to
 // bf16: 32 us, 5.3 TB/s.
 template <typename T, typename O>
 __global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f, const uint8_t* data, O* out,

@@ -16,7 +16,8 @@
 // register i (row g + 8 (i % 2), column pair i / 2), element e: (word >> 4 i) & 0x000f000f is the
 // register's two codes in the low bits of its two halves.
 // Scales and offsets of a group: [g][tile][2], 16 bits each, so that a lane takes the eight that
-// belong to its rows with one 16-byte access.  An offset is -zero point * kUnit (see W4Traits).
+// belong to its rows with one 16-byte access.  An offset is -zero point * kUnit (see W4Traits); both types
+// hold it exactly for any byte, and code - zero, at most 8 bits, as well.
 //
 // A strip's rows are chosen so that rows g and g + 8 of a tile, which end in one thread, are the
 // two rows that an epilogue combines: neighbours 8 apart (plain), gate and up of one output, or
@@ -144,8 +145,8 @@ __device__ __forceinline__ void w4_decode(uint32_t word, uint32_t off0, uint32_t
 
 // The same as the weights themselves, rounded to T: (code - zero) * scale.  sc0, sc1: the scales of rows g and
 // g + 8, each twice; off0, off1: their zero points as the layout holds them.  With `rest`, what the rounding
-// left: the two together are the weight exactly (4 bits times at most 11 are 15, and the two parts have
-// at least 16), down to fp16's smallest subnormal and up to the type's largest number.
+// left: the two together are the weight exactly (8 bits times 8 in bf16, 8 times 11 in fp16, and the two
+// parts have 16 and 22), down to fp16's smallest subnormal and up to the type's largest number.
 template <typename T>
 struct W4Round;
 template <>

@@ -233,7 +233,8 @@ def w4_pack(codes: torch.Tensor, scales: torch.Tensor, zero_points: torch.Tensor
             K: int, **form) -> W4Weight:
     """Lay out weights that are in 4 bits already: ``codes`` uint8 [N, (K + 1) // 2], two per byte, the even
     column in the low half; ``scales`` [N, ceil(K / group)] bfloat16 or float16; ``zero_points`` uint8 of
-    the same shape (without: 8).  The group (32, 64 or 128) follows from the shapes.  ``form`` as in
+    the same shape (without: 8), any byte: a weight is (code - zero point) * scale.  The group (32, 64 or 128)
+    follows from the shapes.  ``form`` as in
     ``w4_quantize``."""
     for t, n in ((codes, "codes"), (scales, "scales")) + (((zero_points, "zero_points"),) if zero_points is not None else ()):
         _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.is_contiguous()
