@@ -30,6 +30,9 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+# Moves the version counters of tensors that a kernel has written through their addresses.
+_count_as_changed = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
+
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
@@ -334,7 +337,9 @@ def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     """Turn the first 2 * len(inv_freq) features of every head of X [rows, heads, head_dim] by
     positions[row] * inv_freq (radians) and multiply them by ``scale``; pairs are (i, i + rotary_dim / 2),
     or neighbours with ``interleaved``.  Into Y, or in place without one; Y shares no memory with X unless
-    it is X.  ``inverse`` turns back, which is the gradient: dX = rotary(dY, ..., inverse=True).
+    it is X.  ``inverse`` turns back, which is the gradient: dX = rotary(dY, ..., inverse=True).  No graph is
+    recorded: what is written must not require a gradient (X in place: call it on X.detach(), or under
+    torch.no_grad()), and it counts as changed, so a backward pass that needs its old value says so.
     Features contiguous, any row and head strides: the queries and keys of a projection
     [rows, (heads + ...) * head_dim] are a view of its output."""
     if not isinstance(X, torch.Tensor) or not X.is_cuda or X.dtype not in _DTYPES or X.dim() != 3:
@@ -360,9 +365,13 @@ def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     if not ((heads < 2 or ys[1] >= dim) and (rows < 2 or ys[0] >= (heads - 1) * ys[1] + dim) or
             (rows < 2 or ys[0] >= dim) and (heads < 2 or ys[1] >= (rows - 1) * ys[0] + dim)):
         _require(False, "two elements of Y share memory")
+    if Y.requires_grad and torch.is_grad_enabled():
+        _require(False, "no graph is recorded of rotary: what it writes must not require a gradient "
+                        "(detach it, or call under torch.no_grad())")
     wide = _rotary_operands(positions, inv_freq, rows, -1, index)
     _call_on(index, _lib.lib().mk_rotary, x, xs[0], xs[1], y, ys[0], ys[1], rows, heads, dim, 2 * inv_freq.shape[0],
              _DTYPES[dtype], positions.data_ptr(), wide, inv_freq.data_ptr(), scale, interleaved, inverse)
+    _count_as_changed((Y,))
     return Y
 
 
