@@ -331,13 +331,28 @@ def w4_gemm_rotary(A: torch.Tensor, W: W4Weight, C: torch.Tensor, positions: tor
     _w4_launch(_lib.lib().mk_w4_gemm_rotary, A, W, C, "rotary", positions.data_ptr(), wide, inv_freq.data_ptr(), scale)
 
 
+def _share_memory(x: int, xs, y: int, ys, rows: int, heads: int, dim: int, size: int) -> bool:
+    """Whether [rows, heads, dim] at address x with strides xs and at y with strides ys may have an element in common.
+    They have none where their address ranges do not meet, or where both step by one stride from window to
+    window and the windows lie beside one another: two ranges of heads in the rows of one projection."""
+    if not (rows and heads and x < y + size * ((rows - 1) * ys[0] + (heads - 1) * ys[1] + dim) and
+            y < x + size * ((rows - 1) * xs[0] + (heads - 1) * xs[1] + dim)):
+        return False
+    for outer, inner, n in ((0, 1, heads), (1, 0, rows)):
+        step, (apart, rest) = xs[outer], divmod(x - y, size)
+        if step > 0 and step == ys[outer] and rest == 0 and (n - 1) * ys[inner] + dim <= apart % step and \
+                apart % step + (n - 1) * xs[inner] + dim <= step:
+            return False
+    return True
+
+
 def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
            Y: torch.Tensor | None = None, *, interleaved: bool = False, inverse: bool = False,
            scale: float = 1.0) -> torch.Tensor:
     """Turn the first 2 * len(inv_freq) features of every head of X [rows, heads, head_dim] by
     positions[row] * inv_freq (radians) and multiply them by ``scale``; pairs are (i, i + rotary_dim / 2),
     or neighbours with ``interleaved``.  Into Y, or in place without one; Y shares no memory with X unless
-    it is X.  ``inverse`` turns back, which is the gradient: dX = rotary(dY, ..., inverse=True).  No graph is
+    it is X; the two may be ranges of heads of one buffer.  ``inverse`` turns back, which is the gradient: dX = rotary(dY, ..., inverse=True).  No graph is
     recorded: what is written must not require a gradient (X in place: call it on X.detach(), or under
     torch.no_grad()), and it counts as changed, so a backward pass that needs its old value says so.
     Features contiguous, any row and head strides: the queries and keys of a projection
@@ -354,11 +369,8 @@ def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
         if Y.get_device() != index or Y.dtype is not dtype or Y.shape != shape:
             _require(False, "Y must have X's device, type and shape")
         ys, y = Y.stride(), Y.data_ptr()
-        # the address ranges of the two must not meet
-        size = 4 if dtype is torch.float32 else 2
-        if rows and heads and x < y + size * ((rows - 1) * ys[0] + (heads - 1) * ys[1] + dim) and \
-                y < x + size * ((rows - 1) * xs[0] + (heads - 1) * xs[1] + dim):
-            _require(False, "Y must be X or share no memory with it")
+        if (y != x or ys != xs) and _share_memory(x, xs, y, ys, rows, heads, dim, 4 if dtype is torch.float32 else 2):
+            _require(False, "Y must be X, share no memory with it, or lie beside it in rows of the same stride")
     if dim > 1 and (xs[2] != 1 or ys[2] != 1):
         _require(False, "features of X and Y must be contiguous")
     # No two elements of Y at one address: one of the outer dimensions steps over all inside it.

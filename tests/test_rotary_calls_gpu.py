@@ -70,3 +70,21 @@ def test_as_the_forward_of_a_function():
     d = torch.randn((5, 3, 16), device=DEV)
     Turn.apply(x).backward(d)
     assert torch.equal(x.grad, ops.rotary(d.clone(), pos, freq, inverse=True))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("heads_first", [False, True])
+def test_ranges_of_heads_of_one_buffer(dtype, heads_first):
+    """From one range of heads of a projection into another; the heads around them stay as they were."""
+    rows, D = 19, 24
+    both = torch.randn((7, rows, D) if heads_first else (rows, 7, D), device=DEV).to(dtype)
+    whole = both.transpose(0, 1) if heads_first else both
+    pos, freq = operands(rows, D // 2)
+    before = whole.clone()
+    want = ops.rotary(before[:, 1:3].clone(), pos, freq)
+    assert torch.equal(ops.rotary(whole[:, 1:3], pos, freq, whole[:, 4:6]), want)
+    assert torch.equal(whole[:, :4], before[:, :4]) and torch.equal(whole[:, 6], before[:, 6])
+    with pytest.raises(RuntimeError, match="share"):
+        ops.rotary(whole[:, 1:3], pos, freq, whole[:, 2:4])
+    again = whole[:, 1:3]                     # another view of the same elements: in place
+    assert torch.equal(ops.rotary(whole[:, 1:3], pos, freq, again), want) and torch.equal(whole[:, 1:3], want)
