@@ -47,6 +47,9 @@ __device__ __forceinline__ void named_barrier_sync(int id, int n_threads) {
 
 // ---------------------------------------------------------------- programmatic dependent launch
 // No-ops unless the kernel was launched with the programmatic-stream-serialization attribute.
+// A kernel launched with programmatic serialization is resident while the kernel ahead still writes what it
+// will read, so its operands are not read-only for its life: behind the wait they take ordinary loads, which the wait
+// orders, never the read-only path (__ldg).
 __device__ __forceinline__ void grid_dependency_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

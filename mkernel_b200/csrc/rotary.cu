@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kRotaryThreads, 2) rotary_kernel(const __grid_
   auto work_out_angles = [&] {
     for (int e = threadIdx.x; e < rows * pairs; e += blockDim.x) {
       const int r = rows == 1 ? 0 : e / pairs;
-      float2 cs = rotary_cos_sin(rotary_position(p.rotary, row0 + r), __ldg(p.rotary.inv_freq + (e - r * pairs)),
+      float2 cs = rotary_cos_sin(rotary_position(p.rotary, row0 + r), p.rotary.inv_freq[e - r * pairs],
                                  p.rotary.scale);
       cs.y *= p.sign;
       angles[e] = cs;

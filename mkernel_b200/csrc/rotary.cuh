@@ -14,8 +14,8 @@ struct RotaryArgs {
 };
 
 __device__ __forceinline__ long long rotary_position(const RotaryArgs& a, long long token) {
-  return a.pos64 ? __ldg(static_cast<const long long*>(a.positions) + token)
-                 : (long long)__ldg(static_cast<const int*>(a.positions) + token);
+  return a.pos64 ? static_cast<const long long*>(a.positions)[token]
+                 : static_cast<const int*>(a.positions)[token];
 }
 
 // cos and sin of position * inv_freq, times scale.  In turns (1/2pi radians) the whole part can be

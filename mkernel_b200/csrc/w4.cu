@@ -109,14 +109,14 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_pack_kernel(W4PackParams p)
         const uint8_t* c = p.codes + n * row_bytes + k / 2;
         v = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v |= (k + 2 * e < f.K ? (uint32_t)__ldg(c + e) : 0x88u) << (8 * e);
+        for (int e = 0; e < 4; ++e) v |= (k + 2 * e < f.K ? (uint32_t)c[e] : 0x88u) << (8 * e);
         if (k + 8 > f.K) {
           const uint32_t mask = (1u << (4 * (int)(f.K - k))) - 1;
           v = (v & mask) | (0x88888888u & ~mask);
         }
         if (col % f.group == 0) {
-          scale[j] = __ldg(p.scales + n * groups + k / f.group);
-          if (f.zeros) zero[j] = __ldg(p.zero_points + n * groups + k / f.group);
+          scale[j] = p.scales[n * groups + k / f.group];
+          if (f.zeros) zero[j] = p.zero_points[n * groups + k / f.group];
         }
       }
       low[j] = __byte_perm(v & 0x0f0f, (v >> 4) & 0x0f0f, 0x5140);
@@ -147,12 +147,12 @@ template <> struct W4Source<float> {
   float v[8];
   __device__ __forceinline__ float operator[](int i) const { return v[i]; }
   __device__ __forceinline__ void load(const float* p) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
   __device__ __forceinline__ void load(const float* p, int n) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? __ldg(p + i) : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
   }
   template <bool ZEROS> __device__ __forceinline__ void range(float& lo, float& hi) const {
 #pragma unroll
@@ -169,14 +169,14 @@ template <typename S> struct W4Source16 {
     return i & 1 ? two.y : two.x;
   }
   __device__ __forceinline__ void load(const S* p) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   }
   __device__ __forceinline__ void load(const S* p, int n) {
     const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      v[i] = (2 * i < n ? (uint32_t)__ldg(e + 2 * i) : 0u) | (2 * i + 1 < n ? (uint32_t)__ldg(e + 2 * i + 1) << 16 : 0u);
+      v[i] = (2 * i < n ? (uint32_t)e[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)e[2 * i + 1] << 16 : 0u);
   }
   template <bool ZEROS> __device__ __forceinline__ void range(float& lo, float& hi) const {
     uint32_t least = 0, most = 0;
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f,
   const int strip = blockIdx.y, block = blockIdx.x;
   const uint8_t* chunk = data + ((size_t)strip * f.blocks + block) * f.chunk_bytes;
   const W4Unit u = w4_unit();
-  const uint4 code = __ldg(reinterpret_cast<const uint4*>(chunk + w4_unit_offset(u)));
+  const uint4 code = *reinterpret_cast<const uint4*>(chunk + w4_unit_offset(u));
   uint32_t words[4] = {code.x, code.y, code.z, code.w};
   w4_exchange(words);
   const int n[2] = {w4_row(f, strip, u.pair, 0), w4_row(f, strip, u.pair, 1)};
@@ -334,10 +334,10 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f,
     const int col = u.col + 32 * q, k = block * kW4Block + col;
     if (k >= f.K) break;
     const uint8_t* sp = chunk + w4_scale_offset(u.pair, col / f.group);
-    const float2 scale = W4Traits<T>::to_float2(__ldg(reinterpret_cast<const uint32_t*>(sp)));
+    const float2 scale = W4Traits<T>::to_float2(*reinterpret_cast<const uint32_t*>(sp));
     uint32_t off0 = W4Traits<T>::kMinusEight, off1 = off0;
     if (f.zeros) {
-      const uint32_t both = __ldg(reinterpret_cast<const uint32_t*>(sp + kW4Block / f.group * 128));
+      const uint32_t both = *reinterpret_cast<const uint32_t*>(sp + kW4Block / f.group * 128);
       off0 = __byte_perm(both, 0, 0x1010);
       off1 = __byte_perm(both, 0, 0x3232);
     }
@@ -462,7 +462,7 @@ __device__ __forceinline__ void w4_fill(const W4Params& p, const uint8_t* chunk,
         const uint16_t* row = A + (long long)(m0 + m) * p.lda;
 #pragma unroll
         for (int hq = 0; hq < 4; ++hq)
-          v[m][hq] = m0 + m < tokens && k0 + hq * 32 + lane < p.form.K ? __ldg(row + hq * 32) : (uint16_t)0;
+          v[m][hq] = m0 + m < tokens && k0 + hq * 32 + lane < p.form.K ? row[hq * 32] : (uint16_t)0;
       }
 #pragma unroll
       for (int m = 0; m < 8; ++m)
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(128) align_rows_kernel(const uint16_t* src, lo
     const uint16_t* from = src + row * ld + col;
     uint32_t v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? __ldg(from + i) : 0u;
+    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? from[i] : 0u;
     *reinterpret_cast<uint4*>(dst + row * ld_dst + col) =
         make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
   }

@@ -45,7 +45,7 @@ __device__ __forceinline__ W4Turn w4_turn(const W4Params& p, int strip, int pair
   const W4Form& f = p.form;
   const int half = f.head_dim / 2, index = strip * (kW4Strip / 2) + pair, head = index / half, i = index - head * half;
   if (head >= f.rotated_heads || i >= f.rotary_dim / 2) return {false, make_float2(1.0f, 0.0f)};
-  return {true, rotary_cos_sin(rotary_position(p.rotary, token), __ldg(p.rotary.inv_freq + i), p.rotary.scale)};
+  return {true, rotary_cos_sin(rotary_position(p.rotary, token), p.rotary.inv_freq[i], p.rotary.scale)};
 }
 
 // C's entries of one pair of rows and one token.  turn: w4_turn, in the rotary form.
@@ -100,7 +100,7 @@ __device__ __forceinline__ void w4_epilogue4(const W4Params& p, int strip, int p
       for (int i = 0; i < 4; ++i) {
         v[i] = make_float2(a[i], b[i]);
         if (rotated)
-          v[i] = rotary_turn(a[i], b[i], rotary_cos_sin(position, __ldg(p.rotary.inv_freq + at + i), p.rotary.scale));
+          v[i] = rotary_turn(a[i], b[i], rotary_cos_sin(position, p.rotary.inv_freq[at + i], p.rotary.scale));
       }
       const bool apart = rotated && !f.interleaved;
       T* to = row + head * f.head_dim + (apart ? at : 2 * at);
@@ -120,7 +120,7 @@ __device__ __forceinline__ void w4_epilogue4(const W4Params& p, int strip, int p
       n[i][1] = n[i][0] + (apart ? f.rotary_dim / 2 : 1);
       v[i] = make_float2(a[i], b[i]);
       if (rotated && n[i][0] >= 0)
-        v[i] = rotary_turn(a[i], b[i], rotary_cos_sin(position, __ldg(p.rotary.inv_freq + at), p.rotary.scale));
+        v[i] = rotary_turn(a[i], b[i], rotary_cos_sin(position, p.rotary.inv_freq[at], p.rotary.scale));
       if (++at == half) { at = 0; ++head; }
     }
 #pragma unroll
