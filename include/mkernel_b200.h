@@ -229,7 +229,8 @@ int mk_align_rows(const void* src, long long ld, int rows, int cols, void* dst, 
  * dtype first, as mk_w4_dequantize gives them (not in the SwiGLU form, which takes what the rounding
  * leaves as well) -- one beyond the dtype's range, and any with a bf16 scale of 2^121 or more, is not finite
  * there --, and rows of A must start on 16 bytes (A aligned, lda a multiple of 8).
- * C and A share no memory.  A device wait that runs out (see "wait_limit_ms") leaves NaN in C. */
+ * C and A share no memory.  A device wait that runs out (see "wait_limit_ms"; only for M > 16) leaves NaN in
+ * the rows and columns of C that it was for, and a record that mk_w4_status reads. */
 int mk_w4_gemm(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
                void* stream);
 /* H[M, N/2] = silu(A * G^T) * (A * U^T) with w->form = MK_W4_GATE_UP: the single-token form of
@@ -241,6 +242,13 @@ int mk_w4_gemm_swiglu(const void* A, long long lda, const mk_w4* w, void* H, lon
 int mk_w4_gemm_rotary(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
                       const void* positions, int pos64, const float* inv_freq, float scale,
                       void* stream);
+
+/* Reads the 4 status words {code, where, detail0, detail1} of the 4-bit products on the current device (synchronous
+ * device-to-host copy; the products' streams have been synchronised).  Returns MK_ERR_DEVICE_WAIT when
+ * code != 0: a wait of some launch ran out since the words were cleared.  Later launches are not affected. */
+int mk_w4_status(uint32_t out4[4]);
+/* Clears them (asynchronous memset on `stream`). */
+int mk_w4_status_clear(void* stream);
 
 /* ---- rotary positions on rows of heads, the step after a query/key projection (for instance on
  * the output of mk_ag_gemm_launch).  No counterpart in the reference.
@@ -289,7 +297,8 @@ int mk_op_status_clear(const mk_symm_view* sync, void* stream);
  *      [1, 60000]; only n_comm accepts -1).  The environment variable
  *      MKERNEL_B200_OPTIONS="name=value,..." sets start-up defaults when the library is loaded,
  *      through the same checks.  Builds made with -DMKB_DIAG add "debug_flags" and "trace_ptr"
- *      (timing diagnostics; results undefined); the default build rejects them. */
+ *      (timing diagnostics; results undefined; in the 4-bit products copies that go missing, to test the waits for them);
+ *      the default build rejects them. */
 int mk_set_option(const char* name, long long value);
 long long mk_get_option(const char* name);
 

@@ -119,6 +119,8 @@ _SIGNATURES = {
                                   c_int, c_void_p]),
     "mk_w4_gemm_rotary": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong,
                                   c_int, c_void_p, c_int, c_void_p, c_float, c_void_p]),
+    "mk_w4_status": (c_int, [POINTER(c_uint32)]),
+    "mk_w4_status_clear": (c_int, [c_void_p]),
     "mk_rotary": (c_int, [c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_longlong,
                           c_longlong, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
                           c_float, c_int, c_int, c_void_p]),

@@ -65,11 +65,11 @@ def sources() -> list[Path]:
     return [CSRC / s for s in SOURCES if (CSRC / s).exists()]
 
 
-def is_stale() -> bool:
-    if not LIB.exists():
+def is_stale(lib: Path = LIB) -> bool:
+    if not lib.exists():
         return True
     newest = max(p.stat().st_mtime_ns for p in list(CSRC.iterdir()) + [PKG.parent / "include" / "mkernel_b200.h"])
-    return newest > LIB.stat().st_mtime_ns
+    return newest > lib.stat().st_mtime_ns
 
 
 def build(force: bool = False, verbose: bool = False, diag: bool = False) -> Path:

@@ -18,6 +18,9 @@ bool option_pdl();
 // The "wait_limit_ms" option in nanoseconds.
 unsigned long long option_wait_limit_ns();
 
+// The "debug_flags" option: 0 but in builds made with -DMKB_DIAG.
+int option_debug_flags();
+
 // Looks up a driver API symbol through the runtime.  Returns MK_OK or MK_ERR_CUDA.
 int driver_entry(const char* symbol, void** fn);
 

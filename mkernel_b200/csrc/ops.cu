@@ -181,6 +181,11 @@ unsigned long long option_wait_limit_ns() {
   return (unsigned long long)g_opt.wait_limit_ms * 1000000ull;
 }
 
+int option_debug_flags() {
+  std::lock_guard<std::mutex> g(g_opt_mu);
+  return (int)g_opt.debug_flags;
+}
+
 static int make_plan(const Options& o, int op, int rank, int world, int M, int N, int K,
                      int b_layout, int num_sms, Plan* out, int epilogue = EPI_NONE) {
   if (op < OP_GEMM || op > OP_AR) return set_error(MK_ERR_INVALID, "unknown op %d", op);

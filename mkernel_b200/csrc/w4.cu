@@ -815,6 +815,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.rotary = rotary;
   p.wide = (reinterpret_cast<uintptr_t>(C) & 7) == 0 && ldc % 4 == 0;
   p.wait_limit_ns = option_wait_limit_ns();
+  p.debug_flags = option_debug_flags();
   // Up to 16 tokens one pass of the stream kernel over the weights does, and the next 16 would take another: 8192 x
   // 8192 takes it 13.1 us for 16 tokens and the tile kernel 14.4 for 17 (1024 x 8192: 6.7 and 9.0; 28672 x 8192: 42
   // and 47).

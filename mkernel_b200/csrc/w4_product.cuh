@@ -26,6 +26,7 @@ struct W4Params {
   int token_tiles;     // tile kernel
   int wide;            // C takes 8-byte stores at every fourth column
   uint64_t wait_limit_ns;
+  int debug_flags;     // diagnostics build only
   int epilogue;
   RotaryArgs rotary;
 };

@@ -24,6 +24,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cstring>
 #include <type_traits>
 
 #include "../../include/mkernel_b200.h"
@@ -52,23 +53,31 @@ __host__ __device__ constexpr int w4_tile_stages(int tokens) { return tokens <= 
 __host__ __device__ constexpr int w4_tile_operands(int tokens, bool rest) { return rest ? 2 : w4_tile_stages(tokens); }
 
 struct TileWait {
-  volatile uint32_t* abort;   // shared: some wait of this CTA has run out
+  volatile uint32_t* abort;   // shared: some wait of this CTA has run out, and the barrier that it was for
   uint64_t limit_ns;
 };
 
-// False when the wait has run out, here or elsewhere in the CTA.
-__device__ __noinline__ bool w4_slow_wait(const TileWait& c, uint32_t bar, uint32_t parity) {
+// What a wait that ran out leaves behind: {code, CTA << 8 | kind of barrier, its offset, blocks of the CTA}, of the
+// first CTA that met one since the words were cleared.
+__device__ uint32_t w4_status_words[4];
+
+// False when the wait has run out, here or elsewhere in the CTA.  `draining`: after that has happened, for what is
+// still under way; runs out by itself alone.
+__device__ __noinline__ bool w4_slow_wait(const TileWait& c, uint32_t bar, uint32_t parity, bool draining = false) {
   uint64_t t0 = 0;
   for (uint32_t it = 1;; ++it) {
     if (ptx::mbar_try_wait(bar, parity)) return true;
     if ((it & 127u) == 0u) {
-      if (*c.abort != 0u) return false;
+      if (!draining && *c.abort != 0u) return false;
       uint64_t now;
       asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
       if (t0 == 0) {
         t0 = now;
       } else if (now - t0 > c.limit_ns) {
-        *c.abort = 1u;
+        if (!draining) {
+          c.abort[1] = bar;
+          c.abort[0] = 1u;
+        }
         return false;
       }
     }
@@ -80,6 +89,17 @@ __device__ __forceinline__ bool w4_wait(const TileWait& c, uint32_t bar, uint32_
 // The same for a whole warp that goes on, or gives up, together.
 __device__ __forceinline__ bool w4_wait_warp(const TileWait& c, uint32_t bar, uint32_t parity) {
   return __all_sync(~0u, w4_wait(c, bar, parity));
+}
+
+// Whether a copying thread is to stop here: never, but in the diagnostics build, where "debug_flags" can make a copy go
+// missing (4: tokens, 8: codes; of block debug_flags >> 8 in the first CTA of each cluster) to see the waits for
+// it run out.
+__device__ __forceinline__ bool w4_copy_missing(const W4Params& p, int rank, bool tokens, int block) {
+#ifdef MKB_DIAG
+  return (p.debug_flags & (tokens ? 4 : 8)) != 0 && rank == 0 && block >= p.debug_flags >> 8;
+#else
+  return false;
+#endif
 }
 
 template <typename T, int TOKENS, int GROUP, bool REST>
@@ -101,7 +121,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* const base_ptr = smem_raw + (base - raw);
-  // control words: full[6] empty[6] a_full[6] a_empty[2] done | tensor memory address, abort flag
+  // control words: full[6] empty[6] a_full[6] a_empty[2] done | tensor memory address, abort flag, barrier, blocks
+  // issued by the four copying threads
   auto full = [&](int s) { return base + 8u * s; };
   auto empty = [&](int s) { return base + 64u + 8u * s; };
   auto a_full = [&](int i) { return base + 128u + 8u * i; };
@@ -109,6 +130,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const uint32_t done = base + 216u;
   volatile uint32_t* const s_tmem = reinterpret_cast<volatile uint32_t*>(base_ptr + 224);
   volatile uint32_t* const s_abort = s_tmem + 1;
+  volatile uint32_t* const s_issued = s_tmem + 3;
   const uint32_t ring = base + kTileControl;
   uint8_t* const ring_ptr = base_ptr + kTileControl;
 
@@ -221,7 +243,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ptx::mbar_arrive(empty(s));
       }
     }
-    ok = ok && w4_wait_warp(wc, done, 0);
+    if (ok) w4_wait_warp(wc, done, 0);
   } else if (warp < kTileCompute + kTileIssue) {
     // ---------------- MMA issue: the whole warp, one lane elected inside the statement ----------------
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -246,15 +268,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (kOwn) ptx::umma_commit_elect<1>(a_empty(operand), 0);
       ptx::umma_commit_elect<1>(empty(s), 0);
     }
-    if (ok && me < kSums) ptx::umma_commit_elect<1>(done, 0);
+    if (me < kSums) ptx::umma_commit_elect<1>(done, 0);   // given up or not: when what was issued has finished
   } else {
     // ---------------- copies: two threads for the codes, two for the tokens (tensor copies) ----------------
     const int me = warp - kTileCompute - kTileIssue;
     const bool tokens = me >= 2, active = lane == 0 && (me & 1) < kTurns;
     const uint32_t tx = tokens ? kTokens * 256 : f.chunk_bytes * (two ? 2 : 1);
-    for (int b = me & 1; active && b < blocks; b += kTurns) {
+    int b = me & 1;
+    for (; active && b < blocks; b += kTurns) {
       const int s = b % kStages;
       if (b >= kStages && !w4_wait(wc, empty(s), (b / kStages - 1) & 1)) break;
+      if (w4_copy_missing(p, rank, tokens, b)) break;
       const uint32_t stage = ring + s * p.stage_bytes;
       ptx::mbar_expect_tx(full(s), tx);
       if (tokens) {
@@ -267,14 +291,37 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (two) ptx::bulk_g2s(stage + kTokens * 256 + f.chunk_bytes, chunk + strip_bytes, f.chunk_bytes, full(s));
       }
     }
+    if (active) s_issued[me] = b;
   }
-  // a wait that ran out leaves MMAs that may still read the ring
-  if (*s_abort != 0u) __nanosleep(50000);
   __syncthreads();
+  // Every role has ended, and whether a wait ran out is settled.  Where one did, copies and MMAs may be under way: nobody
+  // writes over the ring, or leaves, before they have finished (or the limit has passed once more for each).
+  bool spoiled = *s_abort != 0u;
+  if (spoiled) {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < kStages; ++s) {
+        // Phases of full(s) that each of the stage's two copying threads has started: equal, or one ahead by one.
+        const uint32_t codes = s_issued[s % kTurns], tokens = s_issued[2 + s % kTurns];
+        const uint32_t n = (codes + kStages - 1 - s) / kStages, m = (tokens + kStages - 1 - s) / kStages;
+        if (n != m) ptx::mbar_arrive(full(s));       // in the place of the copy that was never started
+        const uint32_t last = n > m ? n : m;
+        if (last > 0) w4_slow_wait(wc, full(s), (last - 1) & 1, true);
+      }
+      w4_slow_wait(wc, done, 0, true);
+      const uint32_t at = s_abort[1] - base;
+      if (atomicCAS(&w4_status_words[0], 0u, 1u) == 0u) {
+        w4_status_words[1] = blockIdx.x << 8 | at / 64;
+        w4_status_words[2] = at;
+        w4_status_words[3] = blocks;
+        __threadfence();
+      }
+    }
+    __syncthreads();
+  }
 
   // The sums, token by token, over the ring; the CTAs of a cluster then share the tokens.
   float* const red = reinterpret_cast<float*>(ring_ptr);
-  if (warp < kTileCompute) {
+  if (warp < kTileCompute && !spoiled) {
     ptx::tc_fence_after();
     constexpr int kEach = kTokens / 4, kBatch = kEach < 16 ? 8 : 16;
     const int c0 = (warp >> 2) * kEach;
@@ -292,7 +339,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
-        red[(c0 + c + i) * kTilePitch + quad * 32 + lane] = ok ? d[i] : __int_as_float(0x7fc00000);
+        red[(c0 + c + i) * kTilePitch + quad * 32 + lane] = d[i];
     }
     ptx::tc_fence_before();
   }
@@ -302,14 +349,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, kCols);
   }
+  // Where a CTA of the cluster gave up there are no sums: NaN, whatever lies in the ring.
+  for (int c = 0; p.split > 1 && c < p.split; ++c)
+    spoiled |= ptx::ld_cluster_u32(ptx::map_to_cta(base + 228u, c)) != 0u;
+  const float nothing = spoiled ? __int_as_float(0x7fc00000) : 0.0f;
   // Four pairs of a token at a time: rows r .. r + 3 and r + 8 .. r + 11 of a tile.
   const int items = min(kTokens, p.M - token0) * (two ? 16 : 8);
   for (int e = rank * kTileThreads + threadIdx.x; e < items; e += p.split * kTileThreads) {
     const int token = two ? e >> 4 : e >> 3, quad = two ? e & 15 : e & 7;   // 8 quads of each strip
     const int r = (quad >> 3) * kW4Strip + (quad >> 1 & 3) * 16 + (quad & 1) * 4;
     const uint32_t at = ring + (token * kTilePitch + r) * 4;
-    float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
-    for (int c = 0; c < p.split; ++c) {
+    float4 u = make_float4(nothing, nothing, nothing, nothing), v = u;
+    for (int c = 0; c < p.split && !spoiled; ++c) {
       const uint32_t a = p.split > 1 ? ptx::map_to_cta(at, c) : at;
       const float4 x = ptx::ld_cluster_f4(a), y = ptx::ld_cluster_f4(a + 32);
       u.x += x.x; u.y += x.y; u.z += x.z; u.w += x.w;
@@ -452,3 +503,26 @@ int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
 }
 
 }  // namespace mkb
+
+using namespace mkb;
+
+extern "C" {
+
+int mk_w4_status(uint32_t out4[4]) {
+  uint32_t w[4] = {0, 0, 0, 0};
+  MKB_CUDA(cudaMemcpyFromSymbol(w, w4_status_words, sizeof(w)));
+  if (out4) memcpy(out4, w, sizeof(w));
+  if (w[0] != 0)
+    return set_error(MK_ERR_DEVICE_WAIT, "4-bit product: device wait expired: code=%u cta=%u role=%u detail=(%u,%u)", w[0],
+                     w[1] >> 8, w[1] & 255u, w[2], w[3]);
+  return MK_OK;
+}
+
+int mk_w4_status_clear(void* stream) {
+  void* words = nullptr;
+  MKB_CUDA(cudaGetSymbolAddress(&words, w4_status_words));
+  MKB_CUDA(cudaMemsetAsync(words, 0, sizeof(w4_status_words), static_cast<cudaStream_t>(stream)));
+  return MK_OK;
+}
+
+}  // extern "C"

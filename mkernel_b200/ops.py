@@ -305,6 +305,28 @@ def w4_gemm_swiglu(A: torch.Tensor, W: W4Weight, H: torch.Tensor) -> None:
     _w4_launch(_lib.lib().mk_w4_gemm_swiglu, A, W, H, "gate_up")
 
 
+def _device_index(device) -> int:
+    """The index of a device; of the current one for None and for "cuda" alone."""
+    index = torch.device("cuda" if device is None else device).index
+    return torch.cuda.current_device() if index is None else index
+
+
+def w4_status(device=None) -> tuple[int, int, int, int]:
+    """Status words of the 4-bit products on a device (by default the current one); raises MkError if a device wait of
+    one of them has run out since ``w4_status_clear`` (its outputs hold NaN).  Synchronises the device."""
+    out = (ctypes.c_uint32 * 4)()
+    with _on_device(_device_index(device)):
+        torch.cuda.synchronize()
+        _lib.check(_lib.lib().mk_w4_status(out))
+    return tuple(int(x) for x in out)
+
+
+def w4_status_clear(device=None) -> None:
+    """Clears what ``w4_status`` reads, on the current stream of the device."""
+    with _on_device(_device_index(device)):
+        _lib.check(_lib.lib().mk_w4_status_clear(_stream()))
+
+
 def _rotary_operands(positions: torch.Tensor, inv_freq: torch.Tensor, rows: int, pairs: int, index: int) -> int:
     """Checks the operands that say how far to turn; returns whether positions have 64 bits."""
     if positions.get_device() != index or inv_freq.get_device() != index:
