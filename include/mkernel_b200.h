@@ -233,6 +233,12 @@ int mk_align_rows(const void* src, long long ld, int rows, int cols, void* dst, 
  * the rows and columns of C that it was for, and a record that mk_w4_status reads. */
 int mk_w4_gemm(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
                void* stream);
+/* The same with flags.  MK_W4_EXACT: for any M the products are of the weights as they are, so that a row's result
+ * does not depend on how many rows come with it by more than the order of fp32 sums; up to twice the tensor
+ * core's work for M > 16 (what it is beyond the dtype's range stays as above). */
+#define MK_W4_EXACT 1
+int mk_w4_gemm_ex(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
+                  int flags, void* stream);
 /* H[M, N/2] = silu(A * G^T) * (A * U^T) with w->form = MK_W4_GATE_UP: the single-token form of
  * mk_ag_gemm_swiglu_launch. */
 int mk_w4_gemm_swiglu(const void* A, long long lda, const mk_w4* w, void* H, long long ldh, int M,
@@ -242,6 +248,9 @@ int mk_w4_gemm_swiglu(const void* A, long long lda, const mk_w4* w, void* H, lon
 int mk_w4_gemm_rotary(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
                       const void* positions, int pos64, const float* inv_freq, float scale,
                       void* stream);
+int mk_w4_gemm_rotary_ex(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
+                         const void* positions, int pos64, const float* inv_freq, float scale,
+                         int flags, void* stream);
 
 /* Reads the 4 status words {code, where, detail0, detail1} of the 4-bit products on the current device (synchronous
  * device-to-host copy; the products' streams have been synchronised).  Returns MK_ERR_DEVICE_WAIT when

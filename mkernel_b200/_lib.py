@@ -22,6 +22,7 @@ MK_AR_BARRIER_WORDS = 2 * 1024 * 1024
 
 MK_BF16, MK_FP16, MK_FP32 = 0, 1, 2
 MK_W4_PLAIN, MK_W4_GATE_UP, MK_W4_ROTARY = 0, 1, 2
+MK_W4_EXACT = 1
 
 OP_GEMM, OP_AG, OP_RS, OP_AR = 0, 1, 2, 3
 
@@ -115,10 +116,14 @@ _SIGNATURES = {
     "mk_align_rows": (c_int, [c_void_p, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p]),
     "mk_w4_gemm": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong, c_int,
                            c_void_p]),
+    "mk_w4_gemm_ex": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong, c_int,
+                              c_int, c_void_p]),
     "mk_w4_gemm_swiglu": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong,
                                   c_int, c_void_p]),
     "mk_w4_gemm_rotary": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong,
                                   c_int, c_void_p, c_int, c_void_p, c_float, c_void_p]),
+    "mk_w4_gemm_rotary_ex": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong,
+                                     c_int, c_void_p, c_int, c_void_p, c_float, c_int, c_void_p]),
     "mk_w4_status": (c_int, [POINTER(c_uint32)]),
     "mk_w4_status_clear": (c_int, [c_void_p]),
     "mk_rotary": (c_int, [c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_longlong,

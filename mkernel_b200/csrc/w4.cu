@@ -783,7 +783,7 @@ static int w4_stream_type(const W4Params& p, const W4StreamPlan& pl, dim3 grid, 
 }
 
 static int w4_product(const char* what, const void* A, long long lda, const mk_w4* w, void* C, long long ldc,
-                      int M, int form, int epilogue, const RotaryArgs& rotary, void* stream) {
+                      int M, int form, int epilogue, const RotaryArgs& rotary, int flags, void* stream) {
   int rc = w4_check(w, what, true);
   if (rc != MK_OK) return rc;
   if (w->form != form)
@@ -791,6 +791,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
                      w->form, form);
   const int n_out = epilogue == W4_EPI_SWIGLU ? w->N / 2 : w->N;
   if (M < 0) return set_error(MK_ERR_INVALID, "%s: M=%d is negative", what, M);
+  if ((flags & ~MK_W4_EXACT) != 0) return set_error(MK_ERR_INVALID, "%s: unknown flags %d", what, flags);
   if (M == 0) return MK_OK;
   if (!A || !C) return set_error(MK_ERR_INVALID, "%s: null operand", what);
   if (lda < w->K || ldc < n_out)
@@ -812,6 +813,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.A = A; p.lda = lda; p.C = C; p.ldc = ldc; p.M = M;
   p.vec = vec;
   p.epilogue = epilogue;
+  p.rest = epilogue == W4_EPI_SWIGLU || (flags & MK_W4_EXACT) != 0;
   p.rotary = rotary;
   p.wide = (reinterpret_cast<uintptr_t>(C) & 7) == 0 && ldc % 4 == 0;
   p.wait_limit_ns = option_wait_limit_ns();
@@ -957,22 +959,31 @@ int mk_align_rows(const void* src, long long ld, int rows, int cols, void* dst, 
                    static_cast<const uint16_t*>(src), ld, rows, cols, static_cast<uint16_t*>(dst), ld_dst);
 }
 
+int mk_w4_gemm_ex(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M, int flags, void* stream) {
+  return w4_product("mk_w4_gemm", A, lda, w, C, ldc, M, MK_W4_PLAIN, W4_EPI_NONE, RotaryArgs{}, flags, stream);
+}
+
 int mk_w4_gemm(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M, void* stream) {
-  return w4_product("mk_w4_gemm", A, lda, w, C, ldc, M, MK_W4_PLAIN, W4_EPI_NONE, RotaryArgs{}, stream);
+  return mk_w4_gemm_ex(A, lda, w, C, ldc, M, 0, stream);
 }
 
 int mk_w4_gemm_swiglu(const void* A, long long lda, const mk_w4* w, void* H, long long ldh, int M, void* stream) {
-  return w4_product("mk_w4_gemm_swiglu", A, lda, w, H, ldh, M, MK_W4_GATE_UP, W4_EPI_SWIGLU, RotaryArgs{}, stream);
+  return w4_product("mk_w4_gemm_swiglu", A, lda, w, H, ldh, M, MK_W4_GATE_UP, W4_EPI_SWIGLU, RotaryArgs{}, 0, stream);
 }
 
-int mk_w4_gemm_rotary(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
-                      const void* positions, int pos64, const float* inv_freq, float scale, void* stream) {
+int mk_w4_gemm_rotary_ex(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
+                         const void* positions, int pos64, const float* inv_freq, float scale, int flags, void* stream) {
   if (M > 0 && (!positions || !inv_freq)) return set_error(MK_ERR_INVALID, "mk_w4_gemm_rotary: null positions or frequencies");
   if (reinterpret_cast<uintptr_t>(positions) % (pos64 ? 8 : 4) != 0 || reinterpret_cast<uintptr_t>(inv_freq) % 4 != 0)
     return set_error(MK_ERR_INVALID, "mk_w4_gemm_rotary: misaligned positions or frequencies");
   RotaryArgs r;
   r.positions = positions; r.pos64 = pos64 != 0; r.inv_freq = inv_freq; r.scale = scale;
-  return w4_product("mk_w4_gemm_rotary", A, lda, w, C, ldc, M, MK_W4_ROTARY, W4_EPI_ROTARY, r, stream);
+  return w4_product("mk_w4_gemm_rotary", A, lda, w, C, ldc, M, MK_W4_ROTARY, W4_EPI_ROTARY, r, flags, stream);
+}
+
+int mk_w4_gemm_rotary(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,
+                      const void* positions, int pos64, const float* inv_freq, float scale, void* stream) {
+  return mk_w4_gemm_rotary_ex(A, lda, w, C, ldc, M, positions, pos64, inv_freq, scale, 0, stream);
 }
 
 }  // extern "C"

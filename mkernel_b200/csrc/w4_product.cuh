@@ -28,6 +28,7 @@ struct W4Params {
   uint64_t wait_limit_ns;
   int debug_flags;     // diagnostics build only
   int epilogue;
+  int rest;            // tile kernel: what rounding the weights leaves is multiplied as well
   RotaryArgs rotary;
 };
 

@@ -12,7 +12,8 @@
 // (256 tokens of 8192 x 8192 in groups of 64: 59 us that way, 29 this, or 1180 TFLOP/s).  What the rounding adds is
 // smaller than the output's own (relative to the result 1.4e-3 in bf16, where that is 1.7e-3).  In the
 // SwiGLU form two such sums are multiplied and it would be larger (2.1e-3), so there what the rounding left
-// (REST) is multiplied as well, and nothing is lost.
+// (REST) is multiplied as well, and nothing is lost.  The rule: rounding is taken where what it adds stays below
+// the rounding of the output that follows in any case; MK_W4_EXACT takes the rest in the other forms too.
 //
 // Warps 0..15 decode, in two sets that take turns at the blocks of 128 columns (quadrant warp % 4 of the
 // lanes, half of the columns by warp / 4 % 2), and at the end read the sums; warps 16 and 17 issue the
@@ -398,8 +399,8 @@ static int w4_tile_group(const W4Params& p, const CUtensorMap& map, unsigned gri
 }
 template <typename T, int TOKENS>
 static int w4_tile_rest(const W4Params& p, const CUtensorMap& map, unsigned grid, cudaStream_t stream) {
-  return p.epilogue == W4_EPI_SWIGLU ? w4_tile_group<T, TOKENS, true>(p, map, grid, stream)
-                                     : w4_tile_group<T, TOKENS, false>(p, map, grid, stream);
+  return p.rest ? w4_tile_group<T, TOKENS, true>(p, map, grid, stream)
+                : w4_tile_group<T, TOKENS, false>(p, map, grid, stream);
 }
 
 template <typename T>
@@ -472,7 +473,7 @@ int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
   // Tokens to a CTA and CTAs to a cluster along K: whichever finishes first by what a block and a start and end
   // take in ns (measured at 32, 64, 128 and 256 tokens; 1.5 us more for a cluster of two).  Clusters only where
   // all of them run at once: 64 tokens of 4608 x 4096 take 18.2 us in 36 clusters of 4, 10.5 in 36 of 2.
-  const bool rest = p.epilogue == W4_EPI_SWIGLU;
+  const bool rest = p.rest;
   const int block_ns[2][4] = {{280, 290, 370, 500}, {400, 540, 800, 1250}}, ends_ns[4] = {3000, 3000, 4500, 8000};
   int tokens = 128;
   long long best = -1;

@@ -292,11 +292,17 @@ def _w4_launch(call, A: torch.Tensor, W: W4Weight, C: torch.Tensor, form: str, *
     _call_on(index, call, a, lda, W.view_ref, C.data_ptr(), ldc, M, *more)
 
 
-def w4_gemm(A: torch.Tensor, W: W4Weight, C: torch.Tensor) -> None:
+def w4_gemm(A: torch.Tensor, W: W4Weight, C: torch.Tensor, exact: bool = False) -> None:
     """C[M, N] = A[M, K] @ W^T with 4-bit weights: the single-token and small-batch form of
-    ``gemm_bf16``.  A and C in the type of W's scales, any row strides, sharing no memory; fp32 sums, rounded once.
-    For more than 16 rows the weights are rounded to that type first, as ``W.dequantize()`` gives them."""
-    _w4_launch(_lib.lib().mk_w4_gemm, A, W, C, "plain")
+    ``gemm_bf16``.  A and C in the type of W's scales, rows that do not overlap at any stride, sharing no memory;
+    fp32 sums, rounded once.
+    For more than 16 rows the weights are rounded to that type first, as ``W.dequantize()`` gives them, which
+    adds to the error less than the rounding of C (against 64 bits 1.3 times as much in all).  ``exact``: never, so
+    a token's result is as good in a batch as alone; up to twice the tensor core's work."""
+    if exact:
+        _w4_launch(_lib.lib().mk_w4_gemm_ex, A, W, C, "plain", _lib.MK_W4_EXACT)
+    else:
+        _w4_launch(_lib.lib().mk_w4_gemm, A, W, C, "plain")
 
 
 def w4_gemm_swiglu(A: torch.Tensor, W: W4Weight, H: torch.Tensor) -> None:
@@ -344,13 +350,18 @@ def _rotary_operands(positions: torch.Tensor, inv_freq: torch.Tensor, rows: int,
 
 
 def w4_gemm_rotary(A: torch.Tensor, W: W4Weight, C: torch.Tensor, positions: torch.Tensor,
-                   inv_freq: torch.Tensor, scale: float = 1.0) -> None:
+                   inv_freq: torch.Tensor, scale: float = 1.0, exact: bool = False) -> None:
     """C[M, N] = A @ W^T, W of form "rotary": the query/key/value projection of M tokens with the
-    rotated heads of row m turned by positions[m] before the rounding (see ``rotary``)."""
+    rotated heads of row m turned by positions[m] before the rounding (see ``rotary``).  ``exact`` as in ``w4_gemm``."""
     if not isinstance(W, W4Weight) or W.form != "rotary":
         _require(False, "W must be a W4Weight of form 'rotary' (w4_quantize, w4_pack)")
     wide = _rotary_operands(positions, inv_freq, A.shape[0] if A.dim() else 0, W.rotary_dim // 2, W.index)
-    _w4_launch(_lib.lib().mk_w4_gemm_rotary, A, W, C, "rotary", positions.data_ptr(), wide, inv_freq.data_ptr(), scale)
+    if exact:
+        _w4_launch(_lib.lib().mk_w4_gemm_rotary_ex, A, W, C, "rotary", positions.data_ptr(), wide, inv_freq.data_ptr(),
+                   scale, _lib.MK_W4_EXACT)
+    else:
+        _w4_launch(_lib.lib().mk_w4_gemm_rotary, A, W, C, "rotary", positions.data_ptr(), wide, inv_freq.data_ptr(),
+                   scale)
 
 
 def _share_memory(x: int, xs, y: int, ys, rows: int, heads: int, dim: int, size: int) -> bool:
@@ -504,17 +515,17 @@ class TpMlp:
         self.w4_gate_up = w4_quantize(torch.cat((w_gate, w_up)), group, zero_points, form="gate_up")
         self.w4_down = w4_quantize(w_down, group, zero_points)
 
-    def forward_tokens(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    def forward_tokens(self, x: torch.Tensor, out: torch.Tensor | None = None, exact: bool = False) -> torch.Tensor:
         """The MLP of a few tokens x [m, K] (any m; a decode step) with the 4-bit weights: two launches
         on the current stream.  Returns out [m, N_out], this rank's part of the sum over ranks -- the
-        whole result when there is one rank; with more the caller sums it over them."""
+        whole result when there is one rank; with more the caller sums it over them.  ``exact`` as in ``w4_gemm``."""
         _require(self.w4_gate_up is not None, "call load_weights_w4 first")
         m = x.shape[0]
         h = torch.empty((m, self.I), device=x.device, dtype=x.dtype)
         if out is None:
             out = torch.empty((m, self.N), device=x.device, dtype=x.dtype)
         w4_gemm_swiglu(x, self.w4_gate_up, h)
-        w4_gemm(h, self.w4_down, out)
+        w4_gemm(h, self.w4_down, out, exact)
         return out
 
     def free(self) -> None:
