@@ -311,7 +311,7 @@ int mk_op_status_clear(const mk_symm_view* sync, void* stream);
 int mk_set_option(const char* name, long long value);
 long long mk_get_option(const char* name);
 
-/* ---- introspection used by host-side tests and tools (no GPU needed) ---------------------- */
+/* ---- introspection used by tests and tools (no GPU needed but for mk_w4_plan_product) ------- */
 typedef struct mk_plan {
   int block_n, stages, n_comm, grid, smem_bytes;
   int row_blocks, col_blocks, k_blocks, part_rows, part_blocks, interleave, group_rows;
@@ -331,6 +331,13 @@ int mk_sched_tiles(int op, int rank, int world, int M, int N, int block_n, int g
  * splitting applies (max_parts >= 2; piece = -1 for whole tiles).  Returns the item count. */
 int mk_sched_work_items(int total_tiles, int n_comp, int cg, int k_blocks, int max_parts, int cta,
                         int* tile, int* kb0, int* kb1, int* piece, int cap);
+/* How the current device runs a 4-bit product of M >= 1 rows (w->data is not looked at): which kernel (tile = 0: the
+ * few-token one, 1: the one on the tensor memory), rows of A to a CTA, CTAs to a cluster along K, CTAs in all; tile
+ * kernel: whether it multiplies what rounding the weights leaves; few tokens: tiles of 16 weight rows to a warp, warps to a CTA. */
+typedef struct mk_w4_plan {
+  int tile, tokens, split, ctas, rest, tiles, warps;
+} mk_w4_plan;
+int mk_w4_plan_product(const mk_w4* w, int M, int flags, mk_w4_plan* out);
 /* Rows [row0,row1) that owner `owner` reduces for its k-th item; returns number of items. */
 int mk_sched_owner_items(int op, int world, int M, int N, int block_n, int owner, int* row0,
                          int* row1, int cap);

@@ -63,6 +63,10 @@ class W4View(Structure):
         "interleaved")]
 
 
+class W4Plan(Structure):
+    _fields_ = [(n, c_int) for n in ("tile", "tokens", "split", "ctas", "rest", "tiles", "warps")]
+
+
 class Plan(Structure):
     _fields_ = [(n, c_int) for n in (
         "block_n", "stages", "n_comm", "grid", "smem_bytes", "row_blocks", "col_blocks",
@@ -124,6 +128,7 @@ _SIGNATURES = {
                                   c_int, c_void_p, c_int, c_void_p, c_float, c_void_p]),
     "mk_w4_gemm_rotary_ex": (c_int, [c_void_p, c_longlong, POINTER(W4View), c_void_p, c_longlong,
                                      c_int, c_void_p, c_int, c_void_p, c_float, c_int, c_void_p]),
+    "mk_w4_plan_product": (c_int, [POINTER(W4View), c_int, c_int, POINTER(W4Plan)]),
     "mk_w4_status": (c_int, [POINTER(c_uint32)]),
     "mk_w4_status_clear": (c_int, [c_void_p]),
     "mk_rotary": (c_int, [c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_longlong,
@@ -184,6 +189,13 @@ def plan_op(op: int, rank: int, world: int, M: int, N: int, K: int, b_layout: in
             num_sms: int = 148) -> Plan:
     out = Plan()
     check(lib().mk_plan_op(op, rank, world, M, N, K, b_layout, num_sms, ctypes.byref(out)))
+    return out
+
+
+def w4_plan(view: W4View, M: int, flags: int = 0) -> W4Plan:
+    """How the current device runs a 4-bit product of M rows."""
+    out = W4Plan()
+    check(lib().mk_w4_plan_product(ctypes.byref(view), M, flags, ctypes.byref(out)))
     return out
 
 

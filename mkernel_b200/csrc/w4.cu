@@ -782,6 +782,9 @@ static int w4_stream_type(const W4Params& p, const W4StreamPlan& pl, dim3 grid, 
                          : w4_stream_group<T, 2, 1>(p, grid, pl.warps, s);
 }
 
+// Whether the tile kernel multiplies what rounding the weights leaves.
+static bool w4_rest(int form, int flags) { return form == MK_W4_GATE_UP || (flags & MK_W4_EXACT) != 0; }
+
 static int w4_product(const char* what, const void* A, long long lda, const mk_w4* w, void* C, long long ldc,
                       int M, int form, int epilogue, const RotaryArgs& rotary, int flags, void* stream) {
   int rc = w4_check(w, what, true);
@@ -800,7 +803,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   if (((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(C)) & 1) != 0)
     return set_error(MK_ERR_INVALID, "%s: operands must be 2-byte aligned", what);
   const bool vec = (reinterpret_cast<uintptr_t>(A) & 15) == 0 && (lda % 8 == 0 || M == 1);
-  if (M > 16 && !vec)
+  if (M > kW4StreamTokens && !vec)
     return set_error(MK_ERR_INVALID, "%s: for more than 16 rows A's must start on 16 bytes (mk_align_rows copies them so)",
                      what);
   int sms = 0;
@@ -813,7 +816,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.A = A; p.lda = lda; p.C = C; p.ldc = ldc; p.M = M;
   p.vec = vec;
   p.epilogue = epilogue;
-  p.rest = epilogue == W4_EPI_SWIGLU || (flags & MK_W4_EXACT) != 0;
+  p.rest = w4_rest(form, flags);
   p.rotary = rotary;
   p.wide = (reinterpret_cast<uintptr_t>(C) & 7) == 0 && ldc % 4 == 0;
   p.wait_limit_ns = option_wait_limit_ns();
@@ -821,7 +824,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   // Up to 16 tokens one pass of the stream kernel over the weights does, and the next 16 would take another: 8192 x
   // 8192 takes it 13.1 us for 16 tokens and the tile kernel 14.4 for 17 (1024 x 8192: 6.7 and 9.0; 28672 x 8192: 42
   // and 47).
-  if (M > 16) return w4_tile_launch(p, w->dtype, sms, static_cast<cudaStream_t>(stream));
+  if (M > kW4StreamTokens) return w4_tile_launch(p, w->dtype, sms, static_cast<cudaStream_t>(stream));
   const W4StreamPlan pl = w4_stream_plan(p.form, M, sms);
   p.stage_bytes = pl.stage_bytes;
   p.split = pl.split;
@@ -957,6 +960,29 @@ int mk_align_rows(const void* src, long long ld, int rows, int cols, void* dst, 
   if (blocks > 16LL * sms) blocks = 16LL * sms;
   return w4_launch(align_rows_kernel, dim3((unsigned)blocks), 128, 0, 1, static_cast<cudaStream_t>(stream),
                    static_cast<const uint16_t*>(src), ld, rows, cols, static_cast<uint16_t*>(dst), ld_dst);
+}
+
+int mk_w4_plan_product(const mk_w4* w, int M, int flags, mk_w4_plan* out) {
+  int rc = w4_check(w, "mk_w4_plan_product", false);
+  if (rc != MK_OK) return rc;
+  if (!out || M < 1 || (flags & ~MK_W4_EXACT) != 0)
+    return set_error(MK_ERR_INVALID, "mk_w4_plan_product: null plan, M=%d below 1 or unknown flags %d", M, flags);
+  int sms = 0;
+  rc = device_sm_count(&sms);
+  if (rc != MK_OK) return rc;
+  const W4Form f = w4_form(*w);
+  memset(out, 0, sizeof(*out));
+  if (M > kW4StreamTokens) {
+    W4TilePlan pl;
+    const bool rest = w4_rest(w->form, flags);
+    rc = w4_tile_plan(f, M, rest, sms, &pl);
+    if (rc != MK_OK) return rc;
+    out->tile = 1; out->tokens = pl.tokens; out->split = pl.split; out->ctas = (int)pl.ctas; out->rest = rest;
+    return MK_OK;
+  }
+  const W4StreamPlan pl = w4_stream_plan(f, M, sms);
+  out->tokens = 8 * pl.nt; out->split = pl.split; out->ctas = pl.ctas; out->tiles = pl.tiles; out->warps = pl.warps;
+  return MK_OK;
 }
 
 int mk_w4_gemm_ex(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M, int flags, void* stream) {

@@ -164,7 +164,11 @@ inline int w4_launch(K kern, dim3 grid, int threads, int smem, int cluster, cuda
   return MK_OK;
 }
 
-// The product for more tokens than the stream kernel takes (w4_tile.cu).
+// The product for more tokens than the stream kernel takes (w4_tile.cu), and how it is cut: tokens to a CTA, CTAs to a
+// cluster along K.
+constexpr int kW4StreamTokens = 16;
+struct W4TilePlan { int tokens, split, token_tiles; long long ctas; };
+int w4_tile_plan(const W4Form& f, int M, bool rest, int sms, W4TilePlan* out);
 int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream);
 
 }  // namespace mkb

@@ -467,15 +467,14 @@ static int w4_tile_clusters(int split, int* out) {
   return MK_OK;
 }
 
-int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
-  const W4Form& f = p.form;
+// Tokens to a CTA and CTAs to a cluster along K: whichever finishes first by what a block and a start and end
+// take in ns (measured at 32, 64, 128 and 256 tokens; 1.5 us more for a cluster of two).  Clusters only where
+// all of them run at once: 64 tokens of 4608 x 4096 take 18.2 us in 36 clusters of 4, 10.5 in 36 of 2.
+int w4_tile_plan(const W4Form& f, int M, bool rest, int sms, W4TilePlan* out) {
   const long long row_tiles = (f.strips + 1) / 2;
-  // Tokens to a CTA and CTAs to a cluster along K: whichever finishes first by what a block and a start and end
-  // take in ns (measured at 32, 64, 128 and 256 tokens; 1.5 us more for a cluster of two).  Clusters only where
-  // all of them run at once: 64 tokens of 4608 x 4096 take 18.2 us in 36 clusters of 4, 10.5 in 36 of 2.
-  const bool rest = p.rest;
   const int block_ns[2][4] = {{280, 290, 370, 500}, {400, 540, 800, 1250}}, ends_ns[4] = {3000, 3000, 4500, 8000};
-  int tokens = 128;
+  out->tokens = 128;
+  out->split = 1;
   long long best = -1;
   int clusters[9] = {};
   for (int split = 2; split <= 8; split *= 2) {
@@ -485,22 +484,31 @@ int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
   for (int i = 0; i < 4; ++i)
     for (int split = 1; split <= 8 && split <= f.blocks; split *= 2) {
       const int t = 32 << i;
-      const long long units = row_tiles * (((long long)p.M + t - 1) / t);
+      const long long units = row_tiles * (((long long)M + t - 1) / t);
       if (split > 1 && units > clusters[split]) continue;
       const long long waves = (units * split + sms - 1) / sms;
       const long long each = (long long)((f.blocks + split - 1) / split) * block_ns[rest][i] + ends_ns[i];
       const long long cost = waves * each + (split > 1 ? 750 * split : 0);
-      if (best < 0 || cost < best) { best = cost; tokens = t; p.split = split; }
+      if (best < 0 || cost < best) { best = cost; out->tokens = t; out->split = split; }
     }
-  p.token_tiles = (int)(((long long)p.M + tokens - 1) / tokens);
-  p.stage_bytes = (tokens * 256 + 2 * f.chunk_bytes + 1023) / 1024 * 1024;
-  CUtensorMap map;
-  const int rc = w4_tile_map(&map, p, dtype, tokens);
+  out->token_tiles = (int)(((long long)M + out->tokens - 1) / out->tokens);
+  out->ctas = row_tiles * out->token_tiles * out->split;
+  if (out->ctas > 0x7fffffffLL) return set_error(MK_ERR_INVALID, "4-bit product: M=%d, N=%d is too large", M, f.N);
+  return MK_OK;
+}
+
+int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
+  W4TilePlan pl;
+  int rc = w4_tile_plan(p.form, p.M, p.rest != 0, sms, &pl);
   if (rc != MK_OK) return rc;
-  const long long grid = row_tiles * p.token_tiles * p.split;
-  if (grid > 0x7fffffffLL) return set_error(MK_ERR_INVALID, "4-bit product: M=%d, N=%d is too large", p.M, f.N);
-  return dtype == MK_BF16 ? w4_tile_tokens<__nv_bfloat16>(p, map, tokens, (unsigned)grid, stream)
-                          : w4_tile_tokens<__half>(p, map, tokens, (unsigned)grid, stream);
+  p.split = pl.split;
+  p.token_tiles = pl.token_tiles;
+  p.stage_bytes = (pl.tokens * 256 + 2 * p.form.chunk_bytes + 1023) / 1024 * 1024;
+  CUtensorMap map;
+  rc = w4_tile_map(&map, p, dtype, pl.tokens);
+  if (rc != MK_OK) return rc;
+  return dtype == MK_BF16 ? w4_tile_tokens<__nv_bfloat16>(p, map, pl.tokens, (unsigned)pl.ctas, stream)
+                          : w4_tile_tokens<__half>(p, map, pl.tokens, (unsigned)pl.ctas, stream);
 }
 
 }  // namespace mkb
