@@ -3,6 +3,8 @@ import pytest
 import torch
 
 from mkernel_b200 import ops
+from oracle import w4_oracle as orc
+from tests.test_rotary_gpu import HALF_STEP, make
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -88,3 +90,40 @@ def test_ranges_of_heads_of_one_buffer(dtype, heads_first):
         ops.rotary(whole[:, 1:3], pos, freq, whole[:, 2:4])
     again = whole[:, 1:3]                     # another view of the same elements: in place
     assert torch.equal(ops.rotary(whole[:, 1:3], pos, freq, again), want) and torch.equal(whole[:, 1:3], want)
+
+
+def check(out, x, ref, rot, interleaved, scale, dtype):
+    """The bound of test_rotary_gpu.py, and what it leaves out: below 2^-14 the steps of fp16 no longer shrink with the
+    value, they are 2^-24, so the rounding of such an output is off by up to 2^-25 whatever it is.  Among the
+    millions of outputs here a few of 1e-5 meet that (off by 2.4e-8 and 2.96e-8 for 2^-25 = 2.98e-8).
+    bf16 and fp32 have steps of 2^-133 and 2^-149 there."""
+    out, x = out.cpu().double(), x.double()
+    i = torch.arange(rot // 2)
+    a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + rot // 2)
+    tol = torch.zeros_like(ref)
+    tol[..., a] = tol[..., b] = 2.0 ** -21 * scale * (x[..., a].abs() + x[..., b].abs())
+    least = 2.0 ** -25 if dtype is HF else 0.0
+    bound = torch.clamp(HALF_STEP[dtype] * (ref.abs() + tol), min=least) + tol
+    assert ((out - ref).abs() <= bound).all()
+    assert torch.equal(out[..., rot:], x[..., rot:])
+
+
+@pytest.mark.parametrize("rows,heads,D,rot,dtype", [
+    (700, 41, 256, 128, BF),      # 656 slots a row into Y (328 in place), several rows to a CTA
+    (900, 45, 192, 192, HF),      # 540
+    (333, 64, 128, 128, FP),      # 1024
+    (5, 70, 80, 40, FP),          # 700, one row to a CTA
+    (40, 130, 34, 10, BF),        # pairs of elements: no width that 16 bytes divide
+])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rows_of_more_parts_than_a_block_has_threads(rows, heads, D, rot, dtype, interleaved):
+    x = make(rows, heads, D, dtype, 9)
+    freq, _ = ops.rotary_frequencies(rot, device="cpu")
+    pos = torch.arange(rows) * 977 + 5
+    ref = orc.rotary(x, pos, freq, interleaved, scale=0.75)
+    Y = torch.full((rows, heads, D), float("nan"), device=DEV, dtype=dtype)
+    ops.rotary(x.to(DEV), pos.to(DEV), freq.to(DEV), Y, interleaved=interleaved, scale=0.75)
+    check(Y, x, ref, rot, interleaved, 0.75, dtype)
+    X = x.to(DEV)
+    ops.rotary(X, pos.to(DEV), freq.to(DEV), interleaved=interleaved, scale=0.75)
+    assert torch.equal(X, Y)
