@@ -146,7 +146,9 @@ __device__ __forceinline__ void w4_decode(uint32_t word, uint32_t off0, uint32_t
 // The same as the weights themselves, rounded to T: (code - zero) * scale.  sc0, sc1: the scales of rows g and
 // g + 8, each twice; off0, off1: their zero points as the layout holds them.  With `rest`, what the rounding
 // left: the two together are the weight exactly (8 bits times 8 in bf16, 8 times 11 in fp16, and the two
-// parts have 16 and 22), down to fp16's smallest subnormal and up to the type's largest number.
+// parts have 16 and 22), down to fp16's smallest subnormal.  At the other end a weight beyond the type's
+// largest number is an infinity here, its rest the other one and their products NaN; in bf16 so is any weight with a
+// scale of 2^122 or more, which is held 64 times as large.
 template <typename T>
 struct W4Round;
 template <>
@@ -177,7 +179,8 @@ struct W4Round<__nv_bfloat16> {
 template <>
 struct W4Round<__half> {
   // fp16 has not, so the code is made whole another way: in the low bits of 1024 (or, 16 times as much, four
-  // bits up), less 1024 (64) and the zero point.
+  // bits up), less 1024 (64) and the zero point; a known way to turn whole numbers into fp16 (Kim, Henry, Fahim,
+  // Awadalla: Who Says Elephants Can't Run, 2022).
   uint32_t less0, less1, sc0, sc1;
   __device__ __forceinline__ W4Round(uint32_t o0, uint32_t o1, uint32_t s0, uint32_t s1) : sc0(s0), sc1(s1) {
     less0 = W4Traits<__half>::fma2(o0, W4Traits<__half>::kBack, 0xe400e400u);   // -zero - 1024

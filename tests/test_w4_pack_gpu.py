@@ -51,3 +51,30 @@ def test_products_take_any_zero_point(M, group, dtype):
     tol = 1.1 * tg * (up.abs() + tu) + (gate * torch.sigmoid(gate)).abs() * tu
     tol = tol + (10 + 1.2 * gate.abs()) * 2.0 ** -23 * ref.abs()
     check(H, ref, tol, dtype)
+
+
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("dtype,scale,code,x,above", [
+    (BF, 2.0 ** 121, 9, 2.0 ** -100, True),     # 2^121: the last scale that more than 16 rows take
+    (BF, 2.0 ** 122, 9, 2.0 ** -100, False),    # held 64 times as large it is beyond the type
+    (HF, 4096.0, 15, 2.0 ** -6, True),          # 28672
+    (HF, 16384.0, 15, 2.0 ** -6, False),        # 114688, beyond fp16's 65504
+])
+def test_weights_at_the_top_of_the_range(dtype, scale, code, x, above, exact):
+    """Up to 16 rows a weight may be beyond the type, its product need not be; for more it is not finite, as documented."""
+    N, K = 64, 128
+    codes = torch.full((N, K), 8)
+    codes[:, 5] = code
+    scales = torch.full((N, 1), scale, dtype=dtype)
+    W, G = (pack(codes, scales, torch.full((N, 1), 8), False, **f) for f in ({}, dict(form="gate_up")))
+    want = (code - 8) * scale * x
+    for M in (16, 17):
+        A = torch.zeros((M, K), dtype=dtype, device=DEV)
+        A[:, 5] = x
+        C, H = torch.zeros((M, N), dtype=dtype, device=DEV), torch.zeros((M, N // 2), dtype=dtype, device=DEV)
+        ops.w4_gemm(A, W, C, exact=exact)
+        ops.w4_gemm_swiglu(A, G, H)
+        if M == 16 or above:
+            assert (C.double() == want).all()
+        else:
+            assert not torch.isfinite(C).any() and not torch.isfinite(H).any()
