@@ -206,7 +206,8 @@ __device__ __forceinline__ float w4_quotient(float w, float d, float r) {
 // there, and then w4_quotient is exact too, so both go the same way.  Nor a clamp below: the
 // quotient of the largest magnitude is within 2^-8 of 7, that of hi - lo of 15.  Both need a scale that
 // is no subnormal (or 0, when all quotients round to 0); for others, and for fp32 weights, it is divided and
-// clamped as the definition says.  8192 x 8192 in bf16: 39 us, 4.4 TB/s.
+// clamped as the definition says.  8192 x 8192 in bf16: 37.8 us, 4.5 TB/s; 16 instructions a weight keep the issue slots
+// 79 % busy.
 template <typename T, typename S, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParams p) {
   ptx::grid_dependency_wait();
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(kW4PackThreads) w4_quantize_kernel(W4PackParam
 
 // The matrix back from its layout, 8 consecutive columns of a row as one 16-byte store (two for fp32).
 // code - zero times scale is exact in fp32 (8 bits times at most 11), so it is rounded once.  8192 x 8192 to
-// bf16: 32 us, 5.3 TB/s.
+// bf16: 27.3 us, 6.2 TB/s.
 template <typename T, typename O>
 __global__ void __launch_bounds__(kW4PackThreads) w4_dequantize_kernel(W4Form f, const uint8_t* data, O* out,
                                                                        long long ld, int vec) {
@@ -409,8 +410,8 @@ __device__ __forceinline__ void w4_mma(float (&d)[4], const uint32_t (&a)[4], ui
 // meet it, in a shared-memory ring of its own that asynchronous 16-byte copies fill.  A lane copies
 // just the pieces that it will itself use, so the ring needs no barrier between warps and no
 // registers while the copies fly; lanes meet only over the scales, which four of them share.  One token
-// of 8192 x 8192 takes 8.6 us (4.0 TB/s, of which 2 us are a launch and the last CTA's end); an SM then takes in 40
-// bytes a ns, near the 44 that are its share of the memory, and the 128 strips leave 20 SMs without one.
+// of 8192 x 8192 takes 8.8 us (2 of them a launch and the last CTA's end) with the weights in L2 and 9.3 from memory, so
+// neither's bandwidth is the bound; the 128 strips leave 20 SMs without one, and issue slots are half busy.
 constexpr int kW4Stages = 2;      // the kernel switches between two offsets
 constexpr int kW4SmemMax = 227 * 1024;
 constexpr int kW4Pitch = 34;   // float2 per token: the four tokens a warp writes at once hit different banks
@@ -728,17 +729,17 @@ static W4StreamPlan w4_stream_plan(const W4Form& f, int M, int sms) {
   W4StreamPlan pl;
   pl.nt = M <= 8 ? 1 : 2;
   // Four tiles of rows to a warp share each load of activations, but a narrow matrix gives too few
-  // CTAs then: 1280 x 8192 takes 8.4 with 4 tiles, 5.7 with 2, 4.4 with 1; 3584 x 8192: 8.5, 5.8, 7.1;
-  // 8192 x 8192: 8.6, 9.7, 12.3.
+  // CTAs then: 1280 x 8192 takes 8.5 with 4 tiles, 6.0 with 2, 4.6 with 1; 3584 x 8192: 8.6, 6.2, 7.2;
+  // 8192 x 8192: 8.6, 10.3, 13.2.
   pl.tiles = f.strips * 2 > sms ? 4 : f.strips * 4 > sms ? 2 : 1;
   pl.ctas = f.strips * (4 / pl.tiles);
   // One CTA to an SM brings as many warps as fit; more CTAs than SMs share them with fewer (28672 x
-  // 8192: 28 with 8 warps, 33 with 16; 13 tokens, whose CTAs are larger: 42 with 4, 48 with 8, 50 with 12).  A
+  // 8192: 28 with 8 warps, 33 with 16; 13 tokens, whose CTAs are larger: 41 with 4, 47 with 8, 48 with 12).  A
   // warp without a chunk is of no use.
   pl.warps = pl.ctas > sms ? (pl.nt == 1 ? 8 : 4) : pl.nt == 1 ? 16 : 12;
   if (pl.warps > f.blocks) pl.warps = f.blocks < 4 ? 4 : f.blocks;
   // Clusters along K only where most SMs would be idle and a CTA keeps 8 blocks or more: 256 x 8192 takes 4.1
-  // in clusters of 4 and 4.3 without, 1024 x 1024 3.5 in clusters of 2 and 2.1 without.
+  // in clusters of 4 and 4.4 without, 1024 x 1024 3.5 in clusters of 2 and 2.1 without.
   pl.split = 1;
   while (pl.split < 8 && pl.ctas * pl.split * 4 <= sms && pl.split * 16 <= f.blocks) pl.split *= 2;
   if (pl.split > 1) pl.warps = 8;
@@ -822,7 +823,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.wait_limit_ns = option_wait_limit_ns();
   p.debug_flags = option_debug_flags();
   // Up to 16 tokens one pass of the stream kernel over the weights does, and the next 16 would take another: 8192 x
-  // 8192 takes it 13.1 us for 16 tokens and the tile kernel 14.4 for 17 (1024 x 8192: 6.7 and 9.0; 28672 x 8192: 42
+  // 8192 takes it 12.8 us for 16 tokens and the tile kernel 14.6 for 17 (1024 x 8192: 8.1 and 11.5; 28672 x 8192: 42
   // and 47).
   if (M > kW4StreamTokens) return w4_tile_launch(p, w->dtype, sms, static_cast<cudaStream_t>(stream));
   const W4StreamPlan pl = w4_stream_plan(p.form, M, sms);

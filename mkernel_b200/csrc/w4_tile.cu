@@ -18,10 +18,10 @@
 // Warps 0..15 decode, in two sets that take turns at the blocks of 128 columns (quadrant warp % 4 of the
 // lanes, half of the columns by warp / 4 % 2), and at the end read the sums; warps 16 and 17 issue the
 // MMAs; a thread each of warps 18 to 21 copies a ring of stages (a block: codes of two strips, tokens in the
-// 128-byte swizzle; one thread for it all needs 0.33 us a block).  A block is little work and a long way: a wait for
-// a barrier alone takes some 150 cycles, issuing eight MMAs and a commit 350, whatever the tokens.  So what
-// bounds a narrow product is how many blocks are under way, and up to 128 tokens two warps issue, every
-// other block each, into sums of their own (one warp: 0.39 us a block at 64 tokens).
+// 128-byte swizzle).  A block is little work and a long way, from a barrier to the next whatever the tokens: in a
+// grid of 128 CTAs it takes 324, 335, 516 and 841 ns for 32, 64, 128 and 256 tokens, of which its MMAs at the tensor
+// core's rate are 92, 184, 368 and 736.  So what bounds a narrow product is how many blocks are under way, and up to
+// 128 tokens two warps issue, every other block each, into sums of their own.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -468,8 +468,9 @@ static int w4_tile_clusters(int split, int* out) {
 }
 
 // Tokens to a CTA and CTAs to a cluster along K: whichever finishes first by what a block and a start and end
-// take in ns (measured at 32, 64, 128 and 256 tokens; 1.5 us more for a cluster of two).  Clusters only where
-// all of them run at once: 64 tokens of 4608 x 4096 take 18.2 us in 36 clusters of 4, 10.5 in 36 of 2.
+// take in ns (at 32, 64, 128 and 256 tokens, in grids that leave the chip room; 1.5 us more for a cluster of two).
+// Clusters only where all of them run at once: 64 tokens of 4608 x 4096 take 18.7 us in 36 clusters of 4, 10.5 in 36
+// of 2.  Against all other cuts of 41 shapes: within 2 % of the best at 35, 10 % from it at most.
 int w4_tile_plan(const W4Form& f, int M, bool rest, int sms, W4TilePlan* out) {
   const long long row_tiles = (f.strips + 1) / 2;
   const int block_ns[2][4] = {{280, 290, 370, 500}, {400, 540, 800, 1250}}, ends_ns[4] = {3000, 3000, 4500, 8000};
