@@ -228,7 +228,8 @@ int mk_align_rows(const void* src, long long ld, int rows, int cols, void* dst, 
  * For M <= 16 the products are of the weights as they are.  For more the weights are rounded to w's
  * dtype first, as mk_w4_dequantize gives them (not in the SwiGLU form, which takes what the rounding
  * leaves as well) -- in every form one beyond the dtype's range, and any with a bf16 scale of 2^122 or more, is
- * not finite for more than 16 rows, though it may be for fewer --, and rows of A must start on 16 bytes (A aligned, lda a multiple of 8).
+ * not finite for more than 16 rows, though it may be for fewer; where what the rounding leaves is multiplied an infinite
+ * activation gives NaN in its row where the definition may give an infinity --, and rows of A must start on 16 bytes (A aligned, lda a multiple of 8).
  * C and A share no memory.  A device wait that runs out (see "wait_limit_ms"; only for M > 16) leaves NaN in
  * the rows and columns of C that it was for, and a record that mk_w4_status reads. */
 int mk_w4_gemm(const void* A, long long lda, const mk_w4* w, void* C, long long ldc, int M,

@@ -78,3 +78,32 @@ def test_weights_at_the_top_of_the_range(dtype, scale, code, x, above, exact):
             assert (C.double() == want).all()
         else:
             assert not torch.isfinite(C).any() and not torch.isfinite(H).any()
+
+
+@pytest.mark.parametrize("M", [1, 16, 17, 130])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_infinite_activations_stay_in_their_row(M, dtype):
+    """Weights that are not 0 times one infinite activation: infinities of their signs; not finite, at the least, where the
+    rest of a rounded weight is multiplied as well.  The other rows are as without it."""
+    N, K = 70, 200
+    g = torch.Generator().manual_seed(33)
+    codes = torch.randint(0, 16, (N, K), generator=g)
+    codes[:, 77] = torch.where(torch.arange(N) % 2 == 0, 3, 13)
+    scales = (torch.rand((N, 4), generator=g) * 0.02 + 0.001).to(dtype)
+    zp = torch.full((N, 4), 8)
+    w = orc.dequantize(codes, scales, zp, 64)
+    x = activations(M, K, dtype)
+    x[M // 2, 77] = float("inf")
+    W = pack(codes, scales, zp, False)
+    keep = [m for m in range(M) if m != M // 2]
+    for exact in (False, True):
+        C = torch.zeros((M, N), device=DEV, dtype=dtype)
+        ops.w4_gemm(x.to(DEV), W, C, exact=exact)
+        C = C.cpu()
+        if exact and M > 16:
+            assert not torch.isfinite(C[M // 2]).any()
+        else:
+            assert torch.equal(C[M // 2].double(), w[:, 77] * float("inf"))
+        h = w if exact else held(w, dtype, M)
+        if keep:
+            check(C[keep], x[keep].double() @ h.t(), 2 * slack(x[keep], h), dtype)
