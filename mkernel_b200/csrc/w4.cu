@@ -817,7 +817,6 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.A = A; p.lda = lda; p.C = C; p.ldc = ldc; p.M = M;
   p.vec = vec;
   p.epilogue = epilogue;
-  p.rest = w4_rest(form, flags);
   p.rotary = rotary;
   p.wide = (reinterpret_cast<uintptr_t>(C) & 7) == 0 && ldc % 4 == 0;
   p.wait_limit_ns = option_wait_limit_ns();
@@ -825,7 +824,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   // Up to 16 tokens one pass of the stream kernel over the weights does, and the next 16 would take another: 8192 x
   // 8192 takes it 12.8 us for 16 tokens and the tile kernel 14.6 for 17 (1024 x 8192: 8.1 and 11.5; 28672 x 8192: 42
   // and 47).
-  if (M > kW4StreamTokens) return w4_tile_launch(p, w->dtype, sms, static_cast<cudaStream_t>(stream));
+  if (M > kW4StreamTokens) return w4_tile_launch(p, w->dtype, w4_rest(form, flags), sms, static_cast<cudaStream_t>(stream));
   const W4StreamPlan pl = w4_stream_plan(p.form, M, sms);
   p.stage_bytes = pl.stage_bytes;
   p.split = pl.split;

@@ -28,9 +28,10 @@ struct W4Params {
   uint64_t wait_limit_ns;
   int debug_flags;     // diagnostics build only
   int epilogue;
-  int rest;            // tile kernel: what rounding the weights leaves is multiplied as well
   RotaryArgs rotary;
 };
+// A launch with 8 bytes more costs the host 0.4 us more (3.2 for a token of 1024 x 1024, 3.6 with 168 bytes).
+static_assert(sizeof(W4Params) <= 160, "parameters of the products");
 
 // silu(gate) up in fp32; for a gate below -88 the exponential is inf and the quotient -0, as it should be.
 __device__ __forceinline__ float w4_silu_mul(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
@@ -165,10 +166,10 @@ inline int w4_launch(K kern, dim3 grid, int threads, int smem, int cluster, cuda
 }
 
 // The product for more tokens than the stream kernel takes (w4_tile.cu), and how it is cut: tokens to a CTA, CTAs to a
-// cluster along K.
+// cluster along K.  rest: what rounding the weights leaves is multiplied as well.
 constexpr int kW4StreamTokens = 16;
 struct W4TilePlan { int tokens, split, token_tiles; long long ctas; };
 int w4_tile_plan(const W4Form& f, int M, bool rest, int sms, W4TilePlan* out);
-int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream);
+int w4_tile_launch(W4Params& p, int dtype, bool rest, int sms, cudaStream_t stream);
 
 }  // namespace mkb

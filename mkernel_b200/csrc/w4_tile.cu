@@ -398,18 +398,18 @@ static int w4_tile_group(const W4Params& p, const CUtensorMap& map, unsigned gri
   return w4_tile_kernel_launch<T, TOKENS, 128, REST>(p, map, grid, stream);
 }
 template <typename T, int TOKENS>
-static int w4_tile_rest(const W4Params& p, const CUtensorMap& map, unsigned grid, cudaStream_t stream) {
-  return p.rest ? w4_tile_group<T, TOKENS, true>(p, map, grid, stream)
-                : w4_tile_group<T, TOKENS, false>(p, map, grid, stream);
+static int w4_tile_rest(const W4Params& p, const CUtensorMap& map, bool rest, unsigned grid, cudaStream_t stream) {
+  return rest ? w4_tile_group<T, TOKENS, true>(p, map, grid, stream) : w4_tile_group<T, TOKENS, false>(p, map, grid, stream);
 }
 
 template <typename T>
-static int w4_tile_tokens(const W4Params& p, const CUtensorMap& map, int tokens, unsigned grid, cudaStream_t stream) {
+static int w4_tile_tokens(const W4Params& p, const CUtensorMap& map, int tokens, bool rest, unsigned grid,
+                          cudaStream_t stream) {
   switch (tokens) {
-    case 32: return w4_tile_rest<T, 32>(p, map, grid, stream);
-    case 64: return w4_tile_rest<T, 64>(p, map, grid, stream);
-    case 128: return w4_tile_rest<T, 128>(p, map, grid, stream);
-    default: return w4_tile_rest<T, 256>(p, map, grid, stream);
+    case 32: return w4_tile_rest<T, 32>(p, map, rest, grid, stream);
+    case 64: return w4_tile_rest<T, 64>(p, map, rest, grid, stream);
+    case 128: return w4_tile_rest<T, 128>(p, map, rest, grid, stream);
+    default: return w4_tile_rest<T, 256>(p, map, rest, grid, stream);
   }
 }
 
@@ -498,9 +498,9 @@ int w4_tile_plan(const W4Form& f, int M, bool rest, int sms, W4TilePlan* out) {
   return MK_OK;
 }
 
-int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
+int w4_tile_launch(W4Params& p, int dtype, bool rest, int sms, cudaStream_t stream) {
   W4TilePlan pl;
-  int rc = w4_tile_plan(p.form, p.M, p.rest != 0, sms, &pl);
+  int rc = w4_tile_plan(p.form, p.M, rest, sms, &pl);
   if (rc != MK_OK) return rc;
   p.split = pl.split;
   p.token_tiles = pl.token_tiles;
@@ -508,8 +508,8 @@ int w4_tile_launch(W4Params& p, int dtype, int sms, cudaStream_t stream) {
   CUtensorMap map;
   rc = w4_tile_map(&map, p, dtype, pl.tokens);
   if (rc != MK_OK) return rc;
-  return dtype == MK_BF16 ? w4_tile_tokens<__nv_bfloat16>(p, map, pl.tokens, (unsigned)pl.ctas, stream)
-                          : w4_tile_tokens<__half>(p, map, pl.tokens, (unsigned)pl.ctas, stream);
+  return dtype == MK_BF16 ? w4_tile_tokens<__nv_bfloat16>(p, map, pl.tokens, rest, (unsigned)pl.ctas, stream)
+                          : w4_tile_tokens<__half>(p, map, pl.tokens, rest, (unsigned)pl.ctas, stream);
 }
 
 }  // namespace mkb
