@@ -488,8 +488,11 @@ __device__ __forceinline__ void w4_ld_tiles(const uint8_t* p, uint32_t (&v)[1]) 
   v[0] = *reinterpret_cast<const uint32_t*>(p);
 }
 
+// One CTA to an SM is asked for by name where a warp has one or two tiles: left to itself the compiler makes room for two
+// by spilling (12 tokens of 3584 x 8192: 8.6 us so, 7.5 by name; 1 token 5.65 and 5.45; 4 tokens of 1280 x 8192, rotary,
+// 4.95 and 4.83).  With four tiles it finds 168 registers at most by itself, and asked by name it spills.
 template <typename T, int NT, int TILES, int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(NT == 1 ? 512 : 384) w4_stream_kernel(const __grid_constant__ W4Params p) {
+__global__ void __launch_bounds__(NT == 1 ? 512 : 384, TILES <= 2 ? 1 : 0) w4_stream_kernel(const __grid_constant__ W4Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kGroups = kW4Block / GROUP;
   constexpr int kTail = kGroups * 128 * (ZEROS ? 2 : 1);
