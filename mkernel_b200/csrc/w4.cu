@@ -410,7 +410,7 @@ __device__ __forceinline__ void w4_mma(float (&d)[4], const uint32_t (&a)[4], ui
 // meet it, in a shared-memory ring of its own that asynchronous 16-byte copies fill.  A lane copies
 // just the pieces that it will itself use, so the ring needs no barrier between warps and no
 // registers while the copies fly; lanes meet only over the scales, which four of them share.  One token
-// of 8192 x 8192 takes 8.8 us (2 of them a launch and the last CTA's end) with the weights in L2 and 9.3 from memory, so
+// of 8192 x 8192 takes 8.7 us (2 of them a launch and the last CTA's end) with the weights in L2 and 9.3 from memory, so
 // neither's bandwidth is the bound; the 128 strips leave 20 SMs without one, and issue slots are half busy.
 constexpr int kW4Stages = 2;      // the kernel switches between two offsets
 constexpr int kW4SmemMax = 227 * 1024;
@@ -732,8 +732,8 @@ static W4StreamPlan w4_stream_plan(const W4Form& f, int M, int sms) {
   W4StreamPlan pl;
   pl.nt = M <= 8 ? 1 : 2;
   // Four tiles of rows to a warp share each load of activations, but a narrow matrix gives too few
-  // CTAs then: 1280 x 8192 takes 8.5 with 4 tiles, 6.0 with 2, 4.6 with 1; 3584 x 8192: 8.6, 6.2, 7.2;
-  // 8192 x 8192: 8.6, 10.3, 13.2.
+  // CTAs then: 1280 x 8192 takes 8.5 with 4 tiles, 5.3 with 2, 4.2 with 1; 3584 x 8192: 8.5, 5.4, 8.1;
+  // 8192 x 8192: 8.6, 10.6, 15.7.
   pl.tiles = f.strips * 2 > sms ? 4 : f.strips * 4 > sms ? 2 : 1;
   pl.ctas = f.strips * (4 / pl.tiles);
   // One CTA to an SM brings as many warps as fit; more CTAs than SMs share them with fewer (28672 x
@@ -741,8 +741,8 @@ static W4StreamPlan w4_stream_plan(const W4Form& f, int M, int sms) {
   // warp without a chunk is of no use.
   pl.warps = pl.ctas > sms ? (pl.nt == 1 ? 8 : 4) : pl.nt == 1 ? 16 : 12;
   if (pl.warps > f.blocks) pl.warps = f.blocks < 4 ? 4 : f.blocks;
-  // Clusters along K only where most SMs would be idle and a CTA keeps 8 blocks or more: 256 x 8192 takes 4.1
-  // in clusters of 4 and 4.4 without, 1024 x 1024 3.5 in clusters of 2 and 2.1 without.
+  // Clusters along K only where most SMs would be idle and a CTA keeps 8 blocks or more: 256 x 8192 takes 3.9
+  // in clusters of 4 and 4.1 without, 1024 x 1024 3.5 in clusters of 2 and 2.1 without.
   pl.split = 1;
   while (pl.split < 8 && pl.ctas * pl.split * 4 <= sms && pl.split * 16 <= f.blocks) pl.split *= 2;
   if (pl.split > 1) pl.warps = 8;
@@ -825,7 +825,7 @@ static int w4_product(const char* what, const void* A, long long lda, const mk_w
   p.wait_limit_ns = option_wait_limit_ns();
   p.debug_flags = option_debug_flags();
   // Up to 16 tokens one pass of the stream kernel over the weights does, and the next 16 would take another: 8192 x
-  // 8192 takes it 12.8 us for 16 tokens and the tile kernel 14.6 for 17 (1024 x 8192: 8.1 and 11.5; 28672 x 8192: 42
+  // 8192 takes it 12.7 us for 16 tokens and the tile kernel 14.5 for 17 (1024 x 8192: 7.1 and 10.5; 28672 x 8192: 43
   // and 47).
   if (M > kW4StreamTokens) return w4_tile_launch(p, w->dtype, w4_rest(form, flags), sms, static_cast<cudaStream_t>(stream));
   const W4StreamPlan pl = w4_stream_plan(p.form, M, sms);

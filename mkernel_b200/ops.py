@@ -282,8 +282,8 @@ def _w4_launch(call, A: torch.Tensor, W: W4Weight, C: torch.Tensor, form: str, *
     a = A.data_ptr()
     if (a & 15 or (lda & 7 and M > 1)) and (M > 16 or M * K > 32768):
         # Rows that no 16-byte access can start on: more than 16 are copied, and few where a launch more costs less
-        # than reading them element by element (8 rows of 8191, 1024 outputs: 7.2 us copied, 9.8 not; 2 rows of
-        # 1023: 3.7 and 2.6; in between it gains less than the launch costs the host).
+        # than reading them element by element (8 rows of 8191, 1024 outputs: 6.4 us copied, 8.4 not; 2 rows of
+        # 1023: 3.6 and 2.5; in between it gains less than the launch costs the host).
         lda = (K + 7) // 8 * 8
         rows = torch.empty((M, lda), dtype=dtype, device=W.device)
         if M:
