@@ -390,9 +390,10 @@ def rotary(X: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     torch.no_grad()), and it counts as changed, so a backward pass that needs its old value says so.
     Features contiguous, any row and head strides: the queries and keys of a projection
     [rows, (heads + ...) * head_dim] are a view of its output."""
-    if not isinstance(X, torch.Tensor) or not X.is_cuda or X.dtype not in _DTYPES or X.dim() != 3:
+    shape, index, dtype = (X.shape, X.get_device(), X.dtype) if isinstance(X, torch.Tensor) else ((), -1, None)
+    if index < 0 or dtype not in _DTYPES or len(shape) != 3:
         _require(False, "X must be a CUDA tensor [rows, heads, head_dim] of bfloat16, float16 or float32")
-    shape, xs, index, dtype, x = X.shape, X.stride(), X.get_device(), X.dtype, X.data_ptr()
+    xs, x = X.stride(), X.data_ptr()
     rows, heads, dim = shape
     if heads > 0x7fffffff or dim > 0x7fffffff:
         _require(False, "too many heads or features")
